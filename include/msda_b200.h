@@ -64,7 +64,7 @@ extern "C" {
 #define MSDA_API
 #endif
 
-#define MSDA_B200_ABI_VERSION 3
+#define MSDA_B200_ABI_VERSION 4
 #define MSDA_MAX_LEVELS 16
 
 typedef enum msda_dtype {
@@ -293,6 +293,118 @@ MSDA_API size_t msda_fused_bwd_workspace_bytes(int ndim, int value_dtype, int64_
                                                int64_t channels, const int32_t* spatial_shapes,
                                                int spatial_shapes_on_device, int64_t num_levels,
                                                int64_t num_queries, int64_t num_points);
+
+/* ---------------------------------------------------------------------------
+ * Operators that stand next to the sampling in a model.  They have no
+ * counterpart in the reference.  The rules above hold: the caller owns every
+ * buffer, nothing is allocated, calls are asynchronous on `stream` and keep
+ * no state.
+ * ------------------------------------------------------------------------- */
+
+typedef enum msda_activation {
+  MSDA_ACT_NONE = 0,
+  MSDA_ACT_RELU = 1,
+  MSDA_ACT_SILU = 2,
+  MSDA_ACT_GELU = 3 /* 0.5 z (1 + erf(z / sqrt 2)) */
+} msda_activation;
+
+typedef enum msda_position_dtype {
+  MSDA_POSITION_FLOAT32 = 0,
+  MSDA_POSITION_INT32 = 1,
+  MSDA_POSITION_INT64 = 2
+} msda_position_dtype;
+
+/* Group norm with an affine map and an activation over each level of a
+ * channels-last pyramid:  y = act((x - mean) / sqrt(var + eps) * weight + bias),
+ * mean and var over the rows of one level of one batch entry and the channels
+ * of one of num_groups groups.
+ *   rows            num_levels sizes (host)
+ *   x               num_levels device pointers (host table), level l (batch,
+ *                   rows[l], channels) with strides x_strides[2l] (batch) and
+ *                   x_strides[2l+1] (row) in elements and dense channels
+ *   weight, bias    (channels), or (num_levels, channels) with
+ *                   affine_per_level, of affine_dtype; NULL: ones, zeros
+ *   y               (batch, sum of rows, channels), dense
+ *   stats           (batch, num_levels, num_groups, 2) fp32: mean and
+ *                   1 / sqrt(var + eps), for the backward; always written
+ *   workspace       msda_group_norm_workspace_bytes(..., backward), 256-byte
+ *                   aligned
+ * Statistics are carried in fp32.  Results do not depend on the schedule. */
+MSDA_API size_t msda_group_norm_workspace_bytes(int dtype, int64_t batch, int64_t channels,
+                                                int64_t num_groups, int64_t num_levels,
+                                                const int64_t* rows, int backward);
+
+MSDA_API int msda_group_norm_fwd(int dtype, int64_t batch, int64_t channels, int64_t num_groups,
+               int64_t num_levels, const int64_t* rows, const void* const* x,
+               const int64_t* x_strides, const void* weight, const void* bias, int affine_dtype,
+               int affine_per_level, double eps, int activation, void* y, float* stats,
+               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of x (num_levels pointers and strides, as x), and of weight and
+ * bias in their dtype and shape (either may be NULL). */
+MSDA_API int msda_group_norm_bwd(int dtype, int64_t batch, int64_t channels, int64_t num_groups,
+               int64_t num_levels, const int64_t* rows, const void* const* x,
+               const int64_t* x_strides, const void* weight, const void* bias, int affine_dtype,
+               int affine_per_level, int activation, const float* stats, const void* grad_y,
+               void* const* grad_x, const int64_t* grad_x_strides, void* grad_weight,
+               void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions on num_axes (1 to 4) axes, for one or two tensors (queries
+ * and keys) of the same batch, tokens, channels and dtype: pair j of a head's
+ * first 2 num_pairs channels, (j, j + num_pairs) or with `interleaved`
+ * (2j, 2j + 1), turns by positions[b, t, axis_index[j]] * inv_freq[j]; the
+ * other channels are copied.  With `inverse` it turns back, which is the
+ * backward: x is then the output's gradient and y the input's.
+ *   heads              num_tensors numbers of heads (host)
+ *   x, y               device pointers (host tables) of (batch, num_tokens,
+ *                      heads[i], channels) with dense channels; strides of
+ *                      batch, token and head in elements, three per tensor.
+ *                      y may be x.
+ *   positions          (batch, num_tokens, num_axes) of position_dtype,
+ *                      position_batch elements between batch entries (0: one
+ *                      set for all); integers are exact up to 2^24
+ *   inv_freq           (num_pairs) fp32;  axis_index (num_pairs) int32 in
+ *                      [0, num_axes), not checked
+ *   grad_positions     NULL, or (batch, num_tokens, num_axes) fp32 for the
+ *                      positions' gradient (with `inverse`); `inputs` then
+ *                      holds the forward's inputs and their strides */
+MSDA_API int msda_rotary(int dtype, int64_t batch, int64_t num_tokens, int64_t channels,
+               int num_tensors, const int64_t* heads, const void* const* x,
+               const int64_t* x_strides, void* const* y, const int64_t* y_strides,
+               const void* positions, int position_dtype, int64_t position_batch,
+               int64_t num_axes, const float* inv_freq, const int32_t* axis_index,
+               int64_t num_pairs, int interleaved, int inverse, const void* const* inputs,
+               const int64_t* input_strides, float* grad_positions, void* stream);
+
+/* One AdamW step over num_tensors dense tensors of one dtype:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2   (g times *grad_scale)
+ *   p = p (1 - lr weight_decay)
+ *       - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ *   params, grads, counts, steps   host tables; a NULL gradient leaves a
+ *                   tensor and its states as they are; steps are t, from 1
+ *   exp_avg, exp_avg_sq   states of all tensors, 16-byte aligned, state_elements
+ *                   each: tensor i's start at the sum of the earlier counts,
+ *                   each rounded up to 128.  fp32, or with state_bits = 8 one
+ *                   byte an element and an exponent byte for every 128
+ *                   (msda_adamw.cu describes the format); all-zero bytes are
+ *                   zero moments in both
+ *   master          NULL, or fp32 copies of 16-bit parameters, laid out as the
+ *                   states: the step then reads and updates these and rounds
+ *                   them into params
+ *   seed            of the 8-bit states' random rounding
+ *   grad_scale      NULL, or one fp32 value on the device */
+MSDA_API int msda_adamw_step(int dtype, int state_bits, int64_t num_tensors,
+               void* const* params, const void* const* grads, const int64_t* counts,
+               const int64_t* steps, double lr, double beta1, double beta2, double eps,
+               double weight_decay, uint32_t seed, const float* grad_scale, void* exp_avg,
+               void* exp_avg_sq, uint8_t* exp_avg_exponent, uint8_t* exp_avg_sq_exponent,
+               float* master, int64_t state_elements, void* stream);
+
+/* The values that 8-bit states stand for, as bf16 (which holds them exactly). */
+MSDA_API int msda_adamw_values(const uint8_t* exp_avg, const uint8_t* exp_avg_exponent,
+               const uint8_t* exp_avg_sq, const uint8_t* exp_avg_sq_exponent,
+               int64_t state_elements, void* exp_avg_values, void* exp_avg_sq_values,
+               void* stream);
 
 /* Name of a status code ("MSDA_SUCCESS", ...). */
 MSDA_API const char* msda_status_string(int status);

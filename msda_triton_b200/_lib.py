@@ -35,7 +35,7 @@ BFLOAT16 = 2
 VALUE_HEAD_MAJOR = 0x100
 
 MAX_LEVELS = 16
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 EXPORTED_SYMBOLS = (
     "msda2d_fwd",
@@ -54,6 +54,12 @@ EXPORTED_SYMBOLS = (
     "msda_fused_bwd_workspace_bytes",
     "msda_prologue_fwd",
     "msda_prologue_bwd",
+    "msda_group_norm_workspace_bytes",
+    "msda_group_norm_fwd",
+    "msda_group_norm_bwd",
+    "msda_rotary",
+    "msda_adamw_step",
+    "msda_adamw_values",
     "msda_status_string",
     "msda_last_error",
     "msda_abi_version",
@@ -111,6 +117,34 @@ _ACC_ARGS = _FWD_ARGS[:-2] + [
 ]
 
 
+_NORM_ARGS = [
+    _int, _i64, _i64, _i64, _i64, _vp,   # dtype, B, C, groups, L, rows
+    _vp, _vp, _vp, _vp, _int, _int,      # x, x_strides, weight, bias, affine_dtype, per_level
+]
+_NORM_FWD_ARGS = _NORM_ARGS + [
+    ctypes.c_double, _int, _vp, _vp,     # eps, activation, y, stats
+    _vp, ctypes.c_size_t, _vp,           # workspace, workspace_bytes, stream
+]
+_NORM_BWD_ARGS = _NORM_ARGS + [
+    _int, _vp, _vp, _vp, _vp, _vp, _vp,  # activation, stats, grad_y, grad_x, strides, grad_weight,
+                                         # grad_bias
+    _vp, ctypes.c_size_t, _vp,           # workspace, workspace_bytes, stream
+]
+_ROTARY_ARGS = [
+    _int, _i64, _i64, _i64, _int, _vp,   # dtype, B, Q, C, num_tensors, heads
+    _vp, _vp, _vp, _vp,                  # x, x_strides, y, y_strides
+    _vp, _int, _i64, _i64,               # positions, dtype, batch stride, axes
+    _vp, _vp, _i64, _int, _int,          # inv_freq, axis_index, pairs, interleaved, inverse
+    _vp, _vp, _vp, _vp,                  # inputs, input_strides, grad_positions, stream
+]
+_ADAMW_ARGS = [
+    _int, _int, _i64, _vp, _vp, _vp, _vp,  # dtype, state_bits, tensors, params, grads, counts, steps
+    *[ctypes.c_double] * 5,              # lr, beta1, beta2, eps, weight_decay
+    ctypes.c_uint32, _vp, _vp, _vp,      # seed, grad_scale, exp_avg, exp_avg_sq
+    _vp, _vp, _vp, _i64, _vp,            # exponents, master, state_elements, stream
+]
+
+
 def lib() -> ctypes.CDLL:
     """Load (once) and return the library, with argument types declared."""
     global _lib
@@ -154,6 +188,18 @@ def lib() -> ctypes.CDLL:
             handle.msda_prologue_fwd.restype = _int
             handle.msda_prologue_bwd.argtypes = _PROLOGUE_BWD_ARGS
             handle.msda_prologue_bwd.restype = _int
+            handle.msda_group_norm_workspace_bytes.argtypes = _NORM_ARGS[:6] + [_int]
+            handle.msda_group_norm_workspace_bytes.restype = ctypes.c_size_t
+            handle.msda_group_norm_fwd.argtypes = _NORM_FWD_ARGS
+            handle.msda_group_norm_fwd.restype = _int
+            handle.msda_group_norm_bwd.argtypes = _NORM_BWD_ARGS
+            handle.msda_group_norm_bwd.restype = _int
+            handle.msda_rotary.argtypes = _ROTARY_ARGS
+            handle.msda_rotary.restype = _int
+            handle.msda_adamw_step.argtypes = _ADAMW_ARGS
+            handle.msda_adamw_step.restype = _int
+            handle.msda_adamw_values.argtypes = [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp]
+            handle.msda_adamw_values.restype = _int
             handle.msda_status_string.argtypes = [_int]
             handle.msda_status_string.restype = ctypes.c_char_p
             handle.msda_last_error.argtypes = []

@@ -1,0 +1,399 @@
+// msda_adamw.cu -- one AdamW step over many tensors in one launch, with the
+// two moments in fp32 or in 8 bits.
+//
+//   g' = s g,  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+//   p  = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// in fp32, the parameter rounded once to its type (from an fp32 master copy,
+// if there is one).  Bound by memory: 28 bytes a parameter in fp32, 10 with
+// bf16 parameters and 8-bit moments.
+//
+// States of all tensors lie in one array each; tensor i's elements start at
+// the sum of the earlier tensors' sizes, each rounded up to kBlock.
+//
+// 8-bit moments.  A block of kBlock = 128 elements shares an exponent byte E.
+// With the fp32 bits b of a magnitude, its code is (b >> 20) - 8 (E - top): a
+// float of 3 mantissa bits whose exponent counts down from the block's. The
+// second moment takes 5 exponent bits (top = 31, a range of 2^31), the first
+// its sign and 4 (top = 15).  E is the largest magnitude's exponent after it
+// is rounded up by one code more than it can be, so the highest code is never
+// reached by rounding; it stands for a value that is not finite.
+//
+// Moments are rounded at random, up with the probability of the part cut off:
+// a change of 0.1 % a step (b2 = 0.999) is far below the spacing of 12.5 %, and
+// rounding to the nearest code would freeze the second moment where it is.
+// The random bits are a mixed counter of the element's index, the seed and the
+// step, so a step can be repeated.  A second moment above zero keeps a code
+// above zero: decoded as zero it would divide by eps alone.
+//
+// A warp takes a block, a lane four neighbouring elements: 16-byte (8-byte)
+// accesses of fp32 (16-bit) parameters and whole 128-byte lines of codes, and
+// the block's maximum is one redux instruction.  Tensors are listed in the
+// kernel's own parameters: no copy to the device precedes the launch.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "msda_common.cuh"
+#include "msda_status.cuh"
+
+namespace msda {
+namespace {
+
+constexpr int kAdamThreads = 256;
+constexpr int kBlock = 128;                                 // elements per exponent
+constexpr int kAdamUnroll = 4;                              // blocks per warp
+constexpr int kChunk = kAdamThreads / 32 * kBlock * kAdamUnroll;  // elements per CTA
+constexpr int kFewTensors = 64, kManyTensors = 640;         // per launch: 4 KB and 32 KB of parameters
+
+struct AdamTensor {
+  void* p;
+  const void* g;
+  int64_t n;
+  int64_t offset;  // of its states
+  float step_size, inv_sqrt_bc2;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  uint32_t key;
+  uint32_t chunk0;  // first CTA of the launch
+};
+
+struct AdamArgs {
+  float b1, c1, b2, c2, eps, decay;  // c = 1 - b, decay = 1 - lr wd
+  const float* grad_scale;
+  void *m, *v;
+  uint8_t *me, *ve;
+  float* master;
+  int32_t tensors;
+};
+
+template <int N> struct AdamTable {
+  AdamArgs a;
+  AdamTensor t[N];
+};
+
+constexpr uint32_t kMaxFinite = 0x7f7fffffu;
+
+template <int TOP, bool SIGNED>
+__device__ __forceinline__ float adam_decode(uint32_t code, uint32_t e) {
+  constexpr uint32_t kTopCode = SIGNED ? 127u : 255u;
+  const uint32_t size = SIGNED ? code & 127u : code;
+  uint32_t bits = (size + ((e - TOP) << 3)) << 20;
+  if (size == 0u) bits = 0u;
+  if (size == kTopCode) bits = 0x7fc00000u;
+  if (SIGNED) bits |= (code & 128u) << 24;
+  return __uint_as_float(bits);
+}
+
+// The codes of four values per lane; `r` holds 20 random bits each.
+template <int TOP, bool SIGNED>
+__device__ __forceinline__ uint32_t adam_encode(const float* x, const uint32_t* r, uint32_t& e) {
+  constexpr uint32_t kTopCode = SIGNED ? 127u : 255u;
+  uint32_t b[4], most = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    b[i] = __float_as_uint(x[i]) & 0x7fffffffu;
+    most = max(most, b[i] > kMaxFinite ? 0u : b[i]);
+  }
+  most = __reduce_max_sync(~0u, most);
+  e = max((most + 0x1fffffu) >> 23, static_cast<uint32_t>(TOP));
+  uint32_t word = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    int code = static_cast<int>(min(b[i] + r[i], kMaxFinite) >> 20) -
+               (static_cast<int>(e - TOP) << 3);
+    code = max(code, !SIGNED && b[i] != 0u ? 1 : 0);
+    uint32_t c = b[i] > kMaxFinite ? kTopCode : static_cast<uint32_t>(code);
+    if (SIGNED && code > 0) c |= (__float_as_uint(x[i]) >> 31) << 7;
+    word |= c << (8 * i);
+  }
+  return word;
+}
+
+__device__ __forceinline__ uint32_t adam_random(uint32_t index, uint32_t key) {
+  uint32_t x = index * 0x9e3779b1u + key;
+  x = (x ^ (x >> 16)) * 0x85ebca77u;
+  x = (x ^ (x >> 13)) * 0xc2b2ae3du;
+  return x ^ (x >> 16);
+}
+
+// Up to four elements of the tensor at p, the rest zeros.
+template <typename T>
+__device__ __forceinline__ void adam_load(const T* p, int valid, bool vec, float* f) {
+  if (vec && valid == 4) {
+    const Raw<4 * sizeof(T)> r = [&] {
+      Raw<4 * sizeof(T)> w;
+      if constexpr (sizeof(T) == 4) {
+        const uint4 q = *reinterpret_cast<const uint4*>(p);
+        w.w[0] = q.x; w.w[1] = q.y; w.w[2] = q.z; w.w[3] = q.w;
+      } else {
+        const uint2 q = *reinterpret_cast<const uint2*>(p);
+        w.w[0] = q.x; w.w[1] = q.y;
+      }
+      return w;
+    }();
+    Chunk<T, 4 * sizeof(T)>::unpack(r, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = i < valid ? Elem<T>::to_f(p[i]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void adam_store(T* p, int valid, bool vec, const float* f) {
+  if (vec && valid == 4) {
+    st_chunk<4 * sizeof(T)>(p, Chunk<T, 4 * sizeof(T)>::pack(f));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < valid) p[i] = Elem<T>::from_f(f[i]);
+  }
+}
+
+template <typename T, bool SMALL, bool MASTER, int N>
+__global__ void __launch_bounds__(kAdamThreads)
+adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
+  const AdamArgs& a = tab.a;
+  int lo = 0, hi = a.tensors;  // the last tensor whose first CTA is not after this one
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tab.t[mid].chunk0 <= blockIdx.x) lo = mid;
+    else hi = mid;
+  }
+  const AdamTensor& t = tab.t[lo];
+  const int lane = threadIdx.x & 31;
+  const int64_t first = static_cast<int64_t>(blockIdx.x - t.chunk0) * kChunk +
+                        (threadIdx.x >> 5) * (kBlock * kAdamUnroll) + lane * 4;
+  T* p = static_cast<T*>(t.p);
+  const T* g = static_cast<const T*>(t.g);
+  const bool vec = (reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) %
+                       (4 * sizeof(T)) == 0;
+  const float scale = a.grad_scale == nullptr ? 1.f : __ldg(a.grad_scale);
+
+#pragma unroll
+  for (int u = 0; u < kAdamUnroll; ++u) {
+    const int64_t e0 = first + u * kBlock;
+    if (e0 - lane * 4 >= t.n) break;  // the whole warp: a block that does not exist
+    const int valid = static_cast<int>(min(max(t.n - e0, int64_t{0}), int64_t{4}));
+    const int64_t s0 = t.offset + e0;
+    float x[4], d[4], m[4], v[4];
+    adam_load(g + e0, valid, vec, d);
+    if (MASTER) adam_load(a.master + s0, 4, true, x);
+    else adam_load(p + e0, valid, vec, x);
+    if (SMALL) {
+      const uint32_t cm = *reinterpret_cast<const uint32_t*>(static_cast<uint8_t*>(a.m) + s0);
+      const uint32_t cv = *reinterpret_cast<const uint32_t*>(static_cast<uint8_t*>(a.v) + s0);
+      const uint32_t em = a.me[s0 / kBlock], ev = a.ve[s0 / kBlock];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        m[i] = adam_decode<15, true>(cm >> (8 * i) & 255u, em);
+        v[i] = adam_decode<31, false>(cv >> (8 * i) & 255u, ev);
+      }
+    } else {
+      adam_load(static_cast<const float*>(a.m) + s0, 4, true, m);
+      adam_load(static_cast<const float*>(a.v) + s0, 4, true, v);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float e = d[i] * scale;
+      m[i] = a.b1 * m[i] + a.c1 * e;
+      v[i] = a.b2 * v[i] + a.c2 * e * e;
+      x[i] = a.decay * x[i] - t.step_size * __fdividef(m[i], sqrtf(v[i]) * t.inv_sqrt_bc2 + a.eps);
+      if (i >= valid) m[i] = v[i] = x[i] = 0.f;  // between tensors
+    }
+    adam_store(p + e0, valid, vec, x);
+    if (MASTER) adam_store(a.master + s0, 4, true, x);
+    if (SMALL) {
+      uint32_t rm[4], rv[4], em, ev;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t r = adam_random(static_cast<uint32_t>(s0) + i, t.key);
+        rm[i] = ((r & 0xffffu) << 4) + 8u;
+        rv[i] = ((r >> 16) << 4) + 8u;
+      }
+      const uint32_t cm = adam_encode<15, true>(m, rm, em);
+      const uint32_t cv = adam_encode<31, false>(v, rv, ev);
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + s0) = cm;
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + s0) = cv;
+      if (lane == 0) {
+        a.me[s0 / kBlock] = static_cast<uint8_t>(em);
+        a.ve[s0 / kBlock] = static_cast<uint8_t>(ev);
+      }
+    } else {
+      adam_store(static_cast<float*>(a.m) + s0, 4, true, m);
+      adam_store(static_cast<float*>(a.v) + s0, 4, true, v);
+    }
+  }
+}
+
+// The values that 8-bit moments stand for; bf16 holds them exactly.
+__global__ void __launch_bounds__(kAdamThreads)
+adamw_values_kernel(const uint8_t* m, const uint8_t* me, const uint8_t* v, const uint8_t* ve,
+                    int64_t n, __nv_bfloat16* mo, __nv_bfloat16* vo) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * kAdamThreads + threadIdx.x) * 8;
+  if (i >= n) return;
+  const uint2 cm = __ldg(reinterpret_cast<const uint2*>(m + i));
+  const uint2 cv = __ldg(reinterpret_cast<const uint2*>(v + i));
+  const uint32_t em = __ldg(me + i / kBlock), ev = __ldg(ve + i / kBlock);
+  float fm[8], fv[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    fm[k] = adam_decode<15, true>((k < 4 ? cm.x : cm.y) >> (8 * (k & 3)) & 255u, em);
+    fv[k] = adam_decode<31, false>((k < 4 ? cv.x : cv.y) >> (8 * (k & 3)) & 255u, ev);
+  }
+  st_chunk<16>(mo + i, Chunk<__nv_bfloat16, 16>::pack(fm));
+  st_chunk<16>(vo + i, Chunk<__nv_bfloat16, 16>::pack(fv));
+}
+
+template <typename T, int N>
+cudaError_t adamw_launch(const AdamTable<N>& tab, bool small, unsigned int grid, cudaStream_t st) {
+  if (tab.a.master != nullptr) {
+    if constexpr (sizeof(T) == 2) {
+      if (small) adamw_kernel<T, true, true, N><<<grid, kAdamThreads, 0, st>>>(tab);
+      else adamw_kernel<T, false, true, N><<<grid, kAdamThreads, 0, st>>>(tab);
+    }
+  } else {
+    if (small) adamw_kernel<T, true, false, N><<<grid, kAdamThreads, 0, st>>>(tab);
+    else adamw_kernel<T, false, false, N><<<grid, kAdamThreads, 0, st>>>(tab);
+  }
+  return cudaGetLastError();
+}
+
+struct Step {
+  int dtype;
+  bool small;
+  int64_t tensors;
+  void* const* params;
+  const void* const* grads;
+  const int64_t *counts, *steps;
+  double lr, b1, b2;
+  uint32_t seed;
+};
+
+template <int N> cudaError_t adamw_all(const Step& s, const AdamArgs& args, cudaStream_t st) {
+  AdamTable<N> tab;
+  tab.a = args;
+  int used = 0;
+  int64_t chunks = 0, offset = 0, known = -1;
+  float step_size = 0.f, inv_sqrt_bc2 = 0.f;
+  auto flush = [&]() {
+    if (used == 0) return cudaSuccess;
+    tab.a.tensors = used;
+    const unsigned int grid = static_cast<unsigned int>(chunks);
+    used = 0;
+    chunks = 0;
+    if (s.dtype == MSDA_FLOAT32) return adamw_launch<float, N>(tab, s.small, grid, st);
+    if (s.dtype == MSDA_FLOAT16) return adamw_launch<__half, N>(tab, s.small, grid, st);
+    return adamw_launch<__nv_bfloat16, N>(tab, s.small, grid, st);
+  };
+  for (int64_t i = 0; i < s.tensors; ++i) {
+    const int64_t n = s.counts[i], at = offset;
+    offset += (n + kBlock - 1) / kBlock * kBlock;
+    if (n == 0 || s.grads[i] == nullptr) continue;
+    if (s.steps[i] != known) {
+      known = s.steps[i];
+      const double t = static_cast<double>(known);
+      step_size = static_cast<float>(s.lr / (1.0 - std::pow(s.b1, t)));
+      inv_sqrt_bc2 = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(s.b2, t)));
+    }
+    const int64_t own = (n + kChunk - 1) / kChunk;
+    if (used == N || chunks + own > 0x7fffffff) {
+      const cudaError_t err = flush();
+      if (err != cudaSuccess) return err;
+    }
+    tab.t[used++] = AdamTensor{s.params[i], s.grads[i], n, at, step_size, inv_sqrt_bc2,
+                               s.seed + static_cast<uint32_t>(known) * 0x632be5abu,
+                               static_cast<uint32_t>(chunks)};
+    chunks += own;
+  }
+  return flush();
+}
+
+}  // namespace
+}  // namespace msda
+
+using namespace msda;
+
+int msda_adamw_step(int dtype, int state_bits, int64_t num_tensors, void* const* params,
+                    const void* const* grads, const int64_t* counts, const int64_t* steps,
+                    double lr, double beta1, double beta2, double eps, double weight_decay,
+                    uint32_t seed, const float* grad_scale, void* exp_avg, void* exp_avg_sq,
+                    uint8_t* exp_avg_exponent, uint8_t* exp_avg_sq_exponent, float* master,
+                    int64_t state_elements, void* stream) {
+  const int64_t es = elem_bytes(dtype);
+  if (es == 0) return report(MSDA_ERROR_UNSUPPORTED_DTYPE, "AdamW supports fp32, fp16 and bf16");
+  if (state_bits != 32 && state_bits != 8)
+    return report(MSDA_ERROR_INVALID_ARGUMENT, "states of 32 or 8 bits expected, got %d",
+                  state_bits);
+  if (master != nullptr && dtype == MSDA_FLOAT32)
+    return report(MSDA_ERROR_INVALID_ARGUMENT, "fp32 parameters take no master copy");
+  if (num_tensors < 0 || (num_tensors > 0 && (params == nullptr || grads == nullptr ||
+                                              counts == nullptr || steps == nullptr)))
+    return report(MSDA_ERROR_INVALID_ARGUMENT, "NULL tensor table");
+  if (!(lr >= 0) || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) ||
+      !(weight_decay >= 0))
+    return report(MSDA_ERROR_INVALID_ARGUMENT,
+                  "lr, eps and weight_decay must not be negative, betas lie in [0, 1)");
+  int64_t total = 0;
+  for (int64_t i = 0; i < num_tensors; ++i) {
+    if (counts[i] < 0 || counts[i] > (int64_t{1} << 40) || steps[i] < 1)
+      return report(MSDA_ERROR_INVALID_ARGUMENT, "tensor %lld: bad size or step (from 1)",
+                    static_cast<long long>(i));
+    total += (counts[i] + kBlock - 1) / kBlock * kBlock;
+    if (counts[i] > 0 && grads[i] != nullptr &&
+        (params[i] == nullptr || !is_aligned(params[i], es) || !is_aligned(grads[i], es)))
+      return report(MSDA_ERROR_MISALIGNED, "tensor %lld: NULL or unaligned",
+                    static_cast<long long>(i));
+  }
+  if (state_elements < total)
+    return report(MSDA_ERROR_SHAPE_MISMATCH, "states of %lld elements where %lld are needed",
+                  static_cast<long long>(state_elements), static_cast<long long>(total));
+  if (total == 0) return report_ok();
+  const bool small = state_bits == 8;
+  if (exp_avg == nullptr || exp_avg_sq == nullptr || !is_aligned(exp_avg, 16) ||
+      !is_aligned(exp_avg_sq, 16) || !is_aligned(master, 16) || !is_aligned(grad_scale, 4) ||
+      (small && (exp_avg_exponent == nullptr || exp_avg_sq_exponent == nullptr)))
+    return report(MSDA_ERROR_MISALIGNED, "NULL or unaligned state");
+  AdamArgs a{};
+  a.b1 = static_cast<float>(beta1);
+  a.c1 = static_cast<float>(1.0 - beta1);
+  a.b2 = static_cast<float>(beta2);
+  a.c2 = static_cast<float>(1.0 - beta2);
+  a.eps = static_cast<float>(eps);
+  a.decay = static_cast<float>(1.0 - lr * weight_decay);
+  a.grad_scale = grad_scale;
+  a.m = exp_avg;
+  a.v = exp_avg_sq;
+  a.me = exp_avg_exponent;
+  a.ve = exp_avg_sq_exponent;
+  a.master = master;
+  const Step s{dtype, small, num_tensors, params, grads, counts, steps, lr, beta1, beta2, seed};
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // a launch copies its parameters: the short table where it is enough
+  return report_cuda(num_tensors <= kFewTensors ? adamw_all<kFewTensors>(s, a, st)
+                                                : adamw_all<kManyTensors>(s, a, st),
+                     "AdamW launch");
+}
+
+int msda_adamw_values(const uint8_t* exp_avg, const uint8_t* exp_avg_exponent,
+                      const uint8_t* exp_avg_sq, const uint8_t* exp_avg_sq_exponent,
+                      int64_t state_elements, void* exp_avg_values, void* exp_avg_sq_values,
+                      void* stream) {
+  if (state_elements < 0 || state_elements % kBlock != 0)
+    return report(MSDA_ERROR_INVALID_ARGUMENT, "state_elements must be a multiple of %d", kBlock);
+  if (state_elements == 0) return report_ok();
+  if (exp_avg_exponent == nullptr || exp_avg_sq_exponent == nullptr)
+    return report(MSDA_ERROR_MISALIGNED, "NULL state");
+  for (const void* p : {static_cast<const void*>(exp_avg), static_cast<const void*>(exp_avg_sq),
+                        static_cast<const void*>(exp_avg_values),
+                        static_cast<const void*>(exp_avg_sq_values)})
+    if (p == nullptr || !is_aligned(p, 16))
+      return report(MSDA_ERROR_MISALIGNED, "NULL or unaligned state");
+  const int64_t grid = (state_elements / 8 + kAdamThreads - 1) / kAdamThreads;
+  if (grid > 0x7fffffff)
+    return report(MSDA_ERROR_INT32_OVERFLOW, "too many elements for one launch");
+  adamw_values_kernel<<<static_cast<unsigned int>(grid), kAdamThreads, 0,
+                        static_cast<cudaStream_t>(stream)>>>(
+      exp_avg, exp_avg_exponent, exp_avg_sq, exp_avg_sq_exponent, state_elements,
+      static_cast<__nv_bfloat16*>(exp_avg_values), static_cast<__nv_bfloat16*>(exp_avg_sq_values));
+  return report_cuda(cudaGetLastError(), "AdamW values launch");
+}

@@ -1,0 +1,368 @@
+// msda_rotary.cu -- rotary positions on several axes, applied to one or two
+// tensors of heads (queries and keys) in one launch; the same kernel turns the
+// output gradients back, and can form the positions' gradient on the way.
+//
+// Pair j of a head's first 2P channels -- (j, j + P), or (2j, 2j + 1) with
+// interleaved pairs -- turns by the angle  th_j = position[axis_j] * f_j:
+//   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin
+// and the gradient by its negative.  d y / d th is y turned by a quarter, so
+//   gpos[a] = sum over heads and the pairs on axis a of  f_j (x1 gx2 - x2 gx1).
+//
+// Bound by memory: 2 bytes moved per byte of input, 6 flops a pair.  The
+// angles are the same for every head, so a CTA takes some tokens, turns their
+// P angles into (cos, sin) in shared memory once, and its threads then walk
+// all heads' vectors in memory order.  The first vectors are loaded before the
+// angles are computed.
+//
+// The angle is formed in half turns as a pair of floats, th / pi = u + v, and
+// reduced by the nearest even integer, which is exact; cospi and sinpi take
+// the rest.  An angle of 10^5 radians is then as exact as a small one, where
+// an fp32 product alone would be 0.004 off.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "msda_common.cuh"
+#include "msda_status.cuh"
+
+namespace msda {
+namespace {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotPairs = 2048;  // (token, pair) angles of a CTA
+constexpr int kRotUnits = 1024;  // vectors of a CTA's pass: four a thread
+constexpr int kRotAxes = 4;
+
+// n / d for 0 <= n < 2^31 as a multiply and shift: with m = ceil(2^(31+l) / d)
+// and l = ceil(log2 d) the error stays below 1/d.
+struct Divider {
+  uint32_t m, s, d;
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+    return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> s);
+  }
+};
+Divider divider(uint32_t d) {
+  if (d == 0) d = 1;
+  uint32_t l = 0;
+  while ((uint64_t{1} << l) < d) ++l;
+  return Divider{static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + d - 1) / d), 31 + l, d};
+}
+
+// Strides in elements: batch entry, token, head.
+struct RotTensor {
+  const char* x;  // what is turned: the input, or the output's gradient
+  char* y;
+  const char* in; // with a gradient for the positions: the input
+  int64_t xb, xq, xh, yb, yq, yh, ib, iq, ih;
+};
+
+struct RotArgs {
+  RotTensor t[2];
+  int32_t heads0, heads;   // of the first tensor, of both
+  int32_t P, units;        // pairs; vectors per head (turned, then copied)
+  int32_t turned;          // vectors per head that are turned
+  int32_t tokens;          // per CTA
+  int32_t total;           // B * Q
+  Divider dq, dunit, dhead, dpair;
+  const void* pos;
+  int64_t pos_batch;       // elements between batch entries' positions: 0 if shared
+  int32_t pos_dtype, axes;
+  const float* inv_freq;
+  const int32_t* axis;
+  float sign;              // -1 turns back
+  float* gpos;             // (B, Q, axes)
+};
+
+__device__ __forceinline__ float rot_position(const RotArgs& a, int64_t i) {
+  if (a.pos_dtype == MSDA_POSITION_INT32) return static_cast<float>(__ldg(static_cast<const int32_t*>(a.pos) + i));
+  if (a.pos_dtype == MSDA_POSITION_INT64)
+    return static_cast<float>(__ldg(static_cast<const long long*>(a.pos) + i));
+  return __ldg(static_cast<const float*>(a.pos) + i);
+}
+
+__device__ __forceinline__ float2 rot_angle(float p, float f, float sign) {
+  const float kHi = 0.318309873f, kLo = 1.28412765e-8f;  // 1 / pi in two floats
+  const float t = __fmul_rn(p, f), tl = __fmaf_rn(p, f, -t);
+  const float u = __fmul_rn(t, kHi);
+  const float v = __fmaf_rn(t, kHi, -u) + __fmaf_rn(t, kLo, tl * kHi);
+  const float r = __fsub_rn(u, 2.f * rintf(0.5f * u)) + v;
+  float s, c;
+  sincospif(r, &s, &c);
+  return make_float2(c, s * sign);
+}
+
+// Loads that may be of memory that this thread writes later (in place).
+template <int VB> __device__ __forceinline__ Raw<VB> rot_load(const void* p) {
+  Raw<VB> r;
+  if constexpr (VB == 16) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+  } else if constexpr (VB == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    r.w[0] = v.x; r.w[1] = v.y;
+  } else if constexpr (VB == 4) {
+    r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    r.h = *reinterpret_cast<const uint16_t*>(p);
+  }
+  return r;
+}
+
+template <typename T, int VB, bool PAIRS, bool GPOS>
+__global__ void __launch_bounds__(kRotThreads)
+rotary_kernel(const __grid_constant__ RotArgs a) {
+  constexpr int N = Chunk<T, VB>::EPV;            // pairs per turned vector
+  constexpr int U = GPOS ? 2 : 4;                 // vectors in flight per thread
+  __shared__ __align__(16) float2 turn[kRotPairs];
+  __shared__ float sums[GPOS ? kRotUnits : 1][kRotAxes];
+  const int token0 = blockIdx.x * a.tokens;
+  const int tokens = min(a.tokens, a.total - token0);
+  const int per_token = a.heads * a.units;
+  const int count = tokens * per_token;
+
+  Raw<VB> va[U], vb[U], ia[U], ib[U];
+  T* out[U];
+  int at[U];  // first angle in `turn`, -1 for a vector that is copied
+  auto load = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = base + i * kRotThreads + threadIdx.x;
+      if (u >= count) continue;
+      const int t = a.dhead(u), rest = u - t * per_token;
+      int h = a.dunit(rest);
+      const int j = rest - h * a.units;
+      const uint32_t n = token0 + t, b = a.dq(n), q = n - b * a.dq.d;
+      const bool second = h >= a.heads0;
+      const RotTensor& x = a.t[second];
+      if (second) h -= a.heads0;
+      int c = PAIRS ? 2 * N * j : N * j, gap = PAIRS ? N : a.P;
+      at[i] = t * a.P + j * N;
+      if (j >= a.turned) {
+        c = 2 * a.P + (j - a.turned) * N;
+        gap = 0;
+        at[i] = -1;
+      }
+      const T* p = reinterpret_cast<const T*>(x.x) + b * x.xb + q * x.xq + h * x.xh + c;
+      out[i] = reinterpret_cast<T*>(x.y) + b * x.yb + q * x.yq + h * x.yh + c;
+      va[i] = rot_load<VB>(p);
+      vb[i] = rot_load<VB>(p + gap);
+      if (GPOS) {
+        const T* s = reinterpret_cast<const T*>(x.in) + b * x.ib + q * x.iq + h * x.ih + c;
+        ia[i] = rot_load<VB>(s);
+        ib[i] = rot_load<VB>(s + gap);
+      }
+    }
+  };
+
+  load(0);
+  for (int i = threadIdx.x; i < tokens * a.P; i += kRotThreads) {
+    const int t = a.dpair(i), j = i - t * a.P;
+    const uint32_t n = token0 + t, b = a.dq(n), q = n - b * a.dq.d;
+    const float p = rot_position(a, b * a.pos_batch + static_cast<int64_t>(q) * a.axes +
+                                        __ldg(a.axis + j));
+    turn[i] = rot_angle(p, __ldg(a.inv_freq + j), a.sign);
+  }
+  __syncthreads();
+
+  for (int base = 0; base < count; base += U * kRotThreads) {
+    if (base > 0) load(base);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = base + i * kRotThreads + threadIdx.x;
+      if (u >= count) continue;
+      float ax[kRotAxes] = {0.f, 0.f, 0.f, 0.f};
+      if (at[i] < 0) {
+        st_chunk<VB>(out[i], va[i]);
+      } else {
+        float f[2 * N], s[2 * N];
+        Chunk<T, VB>::unpack(va[i], f);
+        Chunk<T, VB>::unpack(vb[i], f + N);
+        if (GPOS) {
+          Chunk<T, VB>::unpack(ia[i], s);
+          Chunk<T, VB>::unpack(ib[i], s + N);
+        }
+        const int j0 = GPOS ? at[i] - static_cast<int>(a.dpair(at[i])) * a.P : 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const float2 cs = turn[at[i] + k];
+          const int x1 = PAIRS ? 2 * k : k, x2 = PAIRS ? 2 * k + 1 : k + N;
+          const float y1 = f[x1] * cs.x - f[x2] * cs.y, y2 = f[x2] * cs.x + f[x1] * cs.y;
+          f[x1] = y1;
+          f[x2] = y2;
+          if (GPOS) {
+            const float g = __ldg(a.inv_freq + j0 + k) * (s[x1] * y2 - s[x2] * y1);
+            const int on = __ldg(a.axis + j0 + k);
+#pragma unroll
+            for (int d = 0; d < kRotAxes; ++d) ax[d] += on == d ? g : 0.f;
+          }
+        }
+        st_chunk<VB>(out[i], Chunk<T, VB>::pack(f));
+        st_chunk<VB>(out[i] + (PAIRS ? N : a.P), Chunk<T, VB>::pack(f + N));
+      }
+      if (GPOS) {
+        // one token's vectors may take several passes over the same slots
+        const int slot = u & (kRotUnits - 1);
+#pragma unroll
+        for (int d = 0; d < kRotAxes; ++d)
+          sums[slot][d] = u < kRotUnits ? ax[d] : sums[slot][d] + ax[d];
+      }
+    }
+  }
+  if (GPOS) {
+    __syncthreads();
+    // a warp per (token, axis), in the same order every time
+    const int slots = min(per_token, kRotUnits);
+    for (int i = threadIdx.x >> 5; i < tokens * a.axes; i += kRotThreads / 32) {
+      const int t = i / a.axes, d = i - t * a.axes;
+      float g = 0.f;
+      for (int k = threadIdx.x & 31; k < slots; k += 32) g += sums[t * slots + k][d];
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) g += __shfl_xor_sync(~0u, g, s);
+      if ((threadIdx.x & 31) == 0)
+        a.gpos[static_cast<int64_t>(token0 + t) * a.axes + d] = g;
+    }
+  }
+}
+
+template <typename T, int VB>
+cudaError_t rotary_launch(const RotArgs& a, bool pairs, cudaStream_t st) {
+  const unsigned int grid = (a.total + a.tokens - 1) / a.tokens;
+  if (a.gpos != nullptr) {
+    if (pairs) rotary_kernel<T, VB, true, true><<<grid, kRotThreads, 0, st>>>(a);
+    else rotary_kernel<T, VB, false, true><<<grid, kRotThreads, 0, st>>>(a);
+  } else {
+    if (pairs) rotary_kernel<T, VB, true, false><<<grid, kRotThreads, 0, st>>>(a);
+    else rotary_kernel<T, VB, false, false><<<grid, kRotThreads, 0, st>>>(a);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t rotary_dispatch(const RotArgs& a, int vb, bool pairs, cudaStream_t st) {
+  switch (vb) {
+    case 16: return rotary_launch<T, 16>(a, pairs, st);
+    case 8: return rotary_launch<T, 8>(a, pairs, st);
+    case 4: return rotary_launch<T, 4>(a, pairs, st);
+    default:
+      if constexpr (sizeof(T) == 2) return rotary_launch<T, 2>(a, pairs, st);
+      return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace
+}  // namespace msda
+
+using namespace msda;
+
+int msda_rotary(int dtype, int64_t batch, int64_t num_tokens, int64_t channels, int num_tensors,
+                const int64_t* heads, const void* const* x, const int64_t* x_strides,
+                void* const* y, const int64_t* y_strides, const void* positions,
+                int position_dtype, int64_t position_batch, int64_t num_axes,
+                const float* inv_freq, const int32_t* axis_index, int64_t num_pairs,
+                int interleaved, int inverse, const void* const* inputs,
+                const int64_t* input_strides, float* grad_positions, void* stream) {
+  const int64_t es = elem_bytes(dtype);
+  if (es == 0) return report(MSDA_ERROR_UNSUPPORTED_DTYPE, "rotary supports fp32, fp16 and bf16");
+  if (num_tensors < 1 || num_tensors > 2 || batch < 0 || num_tokens < 0 || channels < 0)
+    return report(MSDA_ERROR_INVALID_ARGUMENT, "one or two tensors of non-negative sizes expected");
+  if (num_axes < 1 || num_axes > kRotAxes)
+    return report(MSDA_ERROR_INVALID_ARGUMENT, "num_axes must be 1 to %d", kRotAxes);
+  if (num_pairs < 0 || 2 * num_pairs > channels || num_pairs > kRotPairs)
+    return report(MSDA_ERROR_INVALID_ARGUMENT,
+                  "num_pairs (%lld) must fit the channels (%lld) and be at most %d",
+                  static_cast<long long>(num_pairs), static_cast<long long>(channels), kRotPairs);
+  if (position_dtype < MSDA_POSITION_FLOAT32 || position_dtype > MSDA_POSITION_INT64)
+    return report(MSDA_ERROR_UNSUPPORTED_DTYPE, "positions must be fp32, int32 or int64");
+  if (heads == nullptr || x == nullptr || y == nullptr || x_strides == nullptr ||
+      y_strides == nullptr)
+    return report(MSDA_ERROR_INVALID_ARGUMENT, "NULL tensor table");
+  if (grad_positions != nullptr && (inputs == nullptr || input_strides == nullptr))
+    return report(MSDA_ERROR_INVALID_ARGUMENT, "the positions' gradient needs the inputs");
+  int64_t all_heads = 0;
+  for (int i = 0; i < num_tensors; ++i) {
+    if (heads[i] < 0) return report(MSDA_ERROR_INVALID_ARGUMENT, "negative number of heads");
+    all_heads += heads[i];
+  }
+  constexpr int64_t kMost = 0x7fffffff;
+  if (batch > kMost || num_tokens > kMost || batch * num_tokens > kMost - kRotUnits ||
+      channels > kMost || all_heads > kMost || all_heads * channels > kMost / 2)
+    return report(MSDA_ERROR_INT32_OVERFLOW, "batch * tokens or heads * channels exceeds int32");
+  if (batch * num_tokens == 0) return report_ok();
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (all_heads * channels == 0) {
+    return grad_positions == nullptr
+               ? report_ok()
+               : report_cuda(cudaMemsetAsync(grad_positions, 0,
+                                             batch * num_tokens * num_axes * 4, st),
+                             "rotary launch");
+  }
+  const int64_t ps = position_dtype == MSDA_POSITION_INT64 ? 8 : 4;
+  if (positions == nullptr || !is_aligned(positions, ps) || !is_aligned(grad_positions, 4) ||
+      (num_pairs > 0 && (inv_freq == nullptr || axis_index == nullptr ||
+                         !is_aligned(inv_freq, 4) || !is_aligned(axis_index, 4))))
+    return report(MSDA_ERROR_MISALIGNED, "NULL or unaligned positions or frequencies");
+  RotArgs a{};
+  // the largest vector that divides both halves, the rest, every stride and address
+  int64_t vb = 16;
+  auto fit = [&](int64_t bytes) {
+    while (vb > es && bytes % vb != 0) vb >>= 1;
+  };
+  fit(num_pairs * es);
+  bool in_place = true;
+  for (int i = 0; i < num_tensors; ++i) {
+    RotTensor& t = a.t[i];
+    t.x = static_cast<const char*>(x[i]);
+    t.y = static_cast<char*>(y[i]);
+    t.in = grad_positions == nullptr ? nullptr : static_cast<const char*>(inputs[i]);
+    const int64_t *xs = x_strides + 3 * i, *ys = y_strides + 3 * i;
+    t.xb = xs[0]; t.xq = xs[1]; t.xh = xs[2];
+    t.yb = ys[0]; t.yq = ys[1]; t.yh = ys[2];
+    if (heads[i] == 0) continue;
+    if (t.x == nullptr || t.y == nullptr || !is_aligned(t.x, es) || !is_aligned(t.y, es))
+      return report(MSDA_ERROR_MISALIGNED, "NULL or unaligned tensor");
+    in_place = in_place && t.x == t.y && t.xb == t.yb && t.xq == t.yq && t.xh == t.yh;
+    for (int64_t s : {t.xb, t.xq, t.xh, t.yb, t.yq, t.yh}) fit(s * es);
+    fit(static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.x) % 16));
+    fit(static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.y) % 16));
+    if (t.in != nullptr || grad_positions != nullptr) {
+      if (t.in == nullptr || !is_aligned(t.in, es))
+        return report(MSDA_ERROR_MISALIGNED, "NULL or unaligned input");
+      const int64_t* is = input_strides + 3 * i;
+      t.ib = is[0]; t.iq = is[1]; t.ih = is[2];
+      for (int64_t s : {t.ib, t.iq, t.ih}) fit(s * es);
+      fit(static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.in) % 16));
+    }
+  }
+  const int64_t rest = in_place ? 0 : channels - 2 * num_pairs;
+  fit(rest * es);
+  const int64_t n = vb / es;
+  a.heads0 = static_cast<int32_t>(heads[0]);
+  a.heads = static_cast<int32_t>(all_heads);
+  a.P = static_cast<int32_t>(num_pairs);
+  a.turned = static_cast<int32_t>(num_pairs / n);
+  a.units = a.turned + static_cast<int32_t>(rest / n);
+  a.total = static_cast<int32_t>(batch * num_tokens);
+  if (a.units == 0 && grad_positions == nullptr) return report_ok();
+  const int64_t per_token = std::max<int64_t>(1, all_heads * a.units);
+  a.tokens = static_cast<int32_t>(std::max<int64_t>(
+      1, std::min(kRotUnits / per_token, kRotPairs / std::max<int64_t>(num_pairs, 1))));
+  a.dq = divider(static_cast<uint32_t>(num_tokens));
+  a.dunit = divider(static_cast<uint32_t>(a.units));
+  a.dhead = divider(static_cast<uint32_t>(per_token));
+  a.dpair = divider(static_cast<uint32_t>(num_pairs));
+  a.pos = positions;
+  a.pos_batch = position_batch;
+  a.pos_dtype = position_dtype;
+  a.axes = static_cast<int32_t>(num_axes);
+  a.inv_freq = inv_freq;
+  a.axis = axis_index;
+  a.sign = inverse ? -1.f : 1.f;
+  a.gpos = grad_positions;
+  cudaError_t err;
+  if (dtype == MSDA_FLOAT32) err = rotary_dispatch<float>(a, static_cast<int>(vb), interleaved, st);
+  else if (dtype == MSDA_FLOAT16)
+    err = rotary_dispatch<__half>(a, static_cast<int>(vb), interleaved, st);
+  else err = rotary_dispatch<__nv_bfloat16>(a, static_cast<int>(vb), interleaved, st);
+  return report_cuda(err, "rotary launch");
+}

@@ -141,3 +141,118 @@ def _fused_backward(ctx, grad_output):
 msda_fused_forward.register_autograd(_fused_backward, setup_context=_fused_setup_context)
 
 __all__ += ["msda_fused_forward", "msda_fused_backward"]
+
+
+# ---------------------------------------------------------------- pyramid group norm
+@torch.library.custom_op("msda_b200::group_norm_forward", mutates_args=())
+def group_norm_forward(x: list[Tensor], maps: bool, spatial_shapes: Tensor | None,
+                       num_groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
+                       activation: str) -> tuple[Tensor, Tensor]:
+    """(y, statistics) of pyramid_group_norm; x holds the levels (maps) or the flattened pyramid."""
+    from msda_triton_b200 import norm
+
+    maps, xs, rows = norm._check(x if maps else x[0], spatial_shapes, num_groups, weight, bias,
+                                 activation)
+    return norm.norm_forward(maps, xs, rows, num_groups, weight, bias, eps, activation)
+
+
+@group_norm_forward.register_fake
+def _group_norm_forward_fake(x, maps, spatial_shapes, num_groups, weight, bias, eps, activation):
+    first = x[0]
+    keys = sum(t.shape[1:-1].numel() for t in x)
+    levels = len(x) if maps else spatial_shapes.shape[0]
+    return (first.new_empty((first.shape[0], keys, first.shape[-1])),
+            first.new_empty((first.shape[0], levels, num_groups, 2), dtype=torch.float32))
+
+
+@torch.library.custom_op("msda_b200::group_norm_backward", mutates_args=())
+def group_norm_backward(grad_y: Tensor, stats: Tensor, x: list[Tensor], maps: bool,
+                        spatial_shapes: Tensor | None, num_groups: int, weight: Tensor | None,
+                        bias: Tensor | None, activation: str) -> list[Tensor]:
+    """Gradients of x, then of weight and bias where they are given."""
+    from msda_triton_b200 import norm
+
+    maps, xs, rows = norm._check(x if maps else x[0], spatial_shapes, num_groups, weight, bias,
+                                 activation)
+    gxs, gw, gb = norm.norm_backward(maps, xs, rows, num_groups, weight, bias, activation, stats,
+                                     grad_y)
+    return gxs + [g for g in (gw, gb) if g is not None]
+
+
+@group_norm_backward.register_fake
+def _group_norm_backward_fake(grad_y, stats, x, maps, spatial_shapes, num_groups, weight, bias,
+                              activation):
+    return [torch.empty_like(t, memory_format=torch.contiguous_format)
+            for t in (*x, weight, bias) if t is not None]
+
+
+def _group_norm_setup(ctx, inputs, output):
+    x, maps, spatial_shapes, num_groups, weight, bias, _, activation = inputs
+    ctx.save_for_backward(output[1], spatial_shapes, weight, bias, *x)
+    ctx.meta = maps, num_groups, activation
+
+
+def _group_norm_backward(ctx, grad_y, grad_stats):
+    stats, spatial_shapes, weight, bias, *x = ctx.saved_tensors
+    maps, num_groups, activation = ctx.meta
+    grads = group_norm_backward(grad_y.contiguous(), stats, x, maps, spatial_shapes, num_groups,
+                                weight, bias, activation)
+    gxs, rest = grads[:len(x)], iter(grads[len(x):])
+    return (gxs, None, None, None, None if weight is None else next(rest),
+            None if bias is None else next(rest), None, None)
+
+
+group_norm_forward.register_autograd(_group_norm_backward, setup_context=_group_norm_setup)
+
+
+# ---------------------------------------------------------------- rotary positions
+@torch.library.custom_op("msda_b200::rotary_forward", mutates_args=())
+def rotary_forward(xs: list[Tensor], positions: Tensor, inv_freq: Tensor, axis_index: Tensor,
+                   interleaved: bool) -> list[Tensor]:
+    """One or two tensors of heads turned by their positions (1 or B, Q, A)."""
+    from msda_triton_b200 import positions as rotary_ops
+
+    positions = rotary_ops._check(xs, positions, inv_freq, axis_index)
+    return rotary_ops.rotary_forward(positions, inv_freq, axis_index, interleaved, xs)
+
+
+@rotary_forward.register_fake
+def _rotary_forward_fake(xs, positions, inv_freq, axis_index, interleaved):
+    return [torch.empty_like(x, memory_format=torch.contiguous_format) for x in xs]
+
+
+@torch.library.custom_op("msda_b200::rotary_backward", mutates_args=())
+def rotary_backward(grads: list[Tensor], inputs: list[Tensor], positions: Tensor,
+                    inv_freq: Tensor, axis_index: Tensor, interleaved: bool) -> list[Tensor]:
+    """Gradients of the tensors and, where `inputs` are given, of the positions."""
+    from msda_triton_b200 import positions as rotary_ops
+
+    gxs, gpos = rotary_ops.rotary_backward(positions, inv_freq, axis_index, interleaved, grads,
+                                       inputs or None)
+    return gxs + ([] if gpos is None else [gpos])
+
+
+@rotary_backward.register_fake
+def _rotary_backward_fake(grads, inputs, positions, inv_freq, axis_index, interleaved):
+    return [torch.empty_like(t, memory_format=torch.contiguous_format)
+            for t in (*grads, *([positions] if inputs else []))]
+
+
+def _rotary_setup(ctx, inputs, output):
+    xs, positions, inv_freq, axis_index, interleaved = inputs
+    ctx.count, ctx.interleaved = len(xs), interleaved
+    ctx.save_for_backward(positions, inv_freq, axis_index,
+                          *(xs if positions.requires_grad else ()))
+
+
+def _rotary_backward(ctx, grads):
+    positions, inv_freq, axis_index, *inputs = ctx.saved_tensors
+    got = rotary_backward([g.contiguous() for g in grads], inputs, positions, inv_freq,
+                          axis_index, ctx.interleaved)
+    gpos = got[ctx.count] if inputs else None
+    return got[:ctx.count], gpos, None, None, None
+
+
+rotary_forward.register_autograd(_rotary_backward, setup_context=_rotary_setup)
+
+__all__ += ["group_norm_forward", "group_norm_backward", "rotary_forward", "rotary_backward"]
