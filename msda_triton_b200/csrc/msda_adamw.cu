@@ -74,37 +74,49 @@ template <int N> struct AdamTable {
 
 constexpr uint32_t kMaxFinite = 0x7f7fffffu;
 
-template <int TOP, bool SIGNED>
-__device__ __forceinline__ float adam_decode(uint32_t code, uint32_t e) {
-  constexpr uint32_t kTopCode = SIGNED ? 127u : 255u;
-  const uint32_t size = SIGNED ? code & 127u : code;
-  uint32_t bits = (size + ((e - TOP) << 3)) << 20;
-  if (size == 0u) bits = 0u;
+// Byte i of a word of codes as a value; `shift` is 8 (E - top) << 20.
+template <bool SIGNED>
+__device__ __forceinline__ float adam_decode(uint32_t word, int i, uint32_t shift) {
+  constexpr uint32_t kTopCode = (SIGNED ? 127u : 255u) << 20;
+  const int up = 20 - 8 * i;
+  const uint32_t size = (up >= 0 ? word << up : word >> -up) & kTopCode;
+  uint32_t bits = size == 0u ? 0u : size + shift;
   if (size == kTopCode) bits = 0x7fc00000u;
-  if (SIGNED) bits |= (code & 128u) << 24;
+  if (SIGNED) bits |= word << (24 - 8 * i) & 0x80000000u;
   return __uint_as_float(bits);
 }
+__device__ __forceinline__ uint32_t adam_shift(uint32_t e, uint32_t top) { return (e - top) << 23; }
 
 // The codes of four values per lane; `r` holds 20 random bits each.
-template <int TOP, bool SIGNED>
+template <uint32_t TOP, bool SIGNED>
 __device__ __forceinline__ uint32_t adam_encode(const float* x, const uint32_t* r, uint32_t& e) {
   constexpr uint32_t kTopCode = SIGNED ? 127u : 255u;
   uint32_t b[4], most = 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    b[i] = __float_as_uint(x[i]) & 0x7fffffffu;
-    most = max(most, b[i] > kMaxFinite ? 0u : b[i]);
+    b[i] = __float_as_uint(x[i]);
+    if (SIGNED) b[i] &= 0x7fffffffu;
+    most = max(most, b[i]);
   }
   most = __reduce_max_sync(~0u, most);
-  e = max((most + 0x1fffffu) >> 23, static_cast<uint32_t>(TOP));
+  const bool odd = most > kMaxFinite - 0xfffffu;  // something is not finite, or rounds to it
+  if (odd) {
+    most = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (b[i] <= kMaxFinite) most = max(most, b[i]);
+    most = __reduce_max_sync(~0u, most);
+  }
+  e = max((most + 0x1fffffu) >> 23, TOP);
+  const int base = static_cast<int>(e - TOP) << 3;
   uint32_t word = 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    int code = static_cast<int>(min(b[i] + r[i], kMaxFinite) >> 20) -
-               (static_cast<int>(e - TOP) << 3);
-    code = max(code, !SIGNED && b[i] != 0u ? 1 : 0);
-    uint32_t c = b[i] > kMaxFinite ? kTopCode : static_cast<uint32_t>(code);
-    if (SIGNED && code > 0) c |= (__float_as_uint(x[i]) >> 31) << 7;
+    uint32_t c = b[i] + r[i];
+    if (odd) c = min(c, kMaxFinite);
+    c = static_cast<uint32_t>(max(static_cast<int>(c >> 20) - base, SIGNED ? 0 : min(static_cast<int>(b[i]), 1)));
+    if (odd && b[i] > kMaxFinite) c = kTopCode;
+    if (SIGNED) c |= __float_as_uint(x[i]) >> 24 & 128u;
     word |= c << (8 * i);
   }
   return word;
@@ -117,26 +129,25 @@ __device__ __forceinline__ uint32_t adam_random(uint32_t index, uint32_t key) {
   return x ^ (x >> 16);
 }
 
-// Up to four elements of the tensor at p, the rest zeros.
+// Four elements; those of index `valid` and up are not there.
 template <typename T>
-__device__ __forceinline__ void adam_load(const T* p, int valid, bool vec, float* f) {
+__device__ __forceinline__ Raw<4 * sizeof(T)> adam_load(const T* p, int valid, bool vec) {
+  Raw<4 * sizeof(T)> w;
   if (vec && valid == 4) {
-    const Raw<4 * sizeof(T)> r = [&] {
-      Raw<4 * sizeof(T)> w;
-      if constexpr (sizeof(T) == 4) {
-        const uint4 q = *reinterpret_cast<const uint4*>(p);
-        w.w[0] = q.x; w.w[1] = q.y; w.w[2] = q.z; w.w[3] = q.w;
-      } else {
-        const uint2 q = *reinterpret_cast<const uint2*>(p);
-        w.w[0] = q.x; w.w[1] = q.y;
-      }
-      return w;
-    }();
-    Chunk<T, 4 * sizeof(T)>::unpack(r, f);
+    if constexpr (sizeof(T) == 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(p);
+      w.w[0] = q.x; w.w[1] = q.y; w.w[2] = q.z; w.w[3] = q.w;
+    } else {
+      const uint2 q = *reinterpret_cast<const uint2*>(p);
+      w.w[0] = q.x; w.w[1] = q.y;
+    }
   } else {
+    float f[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = i < valid ? Elem<T>::to_f(p[i]) : 0.f;
+    w = Chunk<T, 4 * sizeof(T)>::pack(f);
   }
+  return w;
 }
 template <typename T>
 __device__ __forceinline__ void adam_store(T* p, int valid, bool vec, const float* f) {
@@ -149,9 +160,16 @@ __device__ __forceinline__ void adam_store(T* p, int valid, bool vec, const floa
   }
 }
 
+__device__ __forceinline__ float adam_sqrt(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <typename T, bool SMALL, bool MASTER, int N>
 __global__ void __launch_bounds__(kAdamThreads)
 adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
+  constexpr int U = kAdamUnroll;
   const AdamArgs& a = tab.a;
   int lo = 0, hi = a.tensors;  // the last tensor whose first CTA is not after this one
   while (hi - lo > 1) {
@@ -162,65 +180,95 @@ adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
   const AdamTensor& t = tab.t[lo];
   const int lane = threadIdx.x & 31;
   const int64_t first = static_cast<int64_t>(blockIdx.x - t.chunk0) * kChunk +
-                        (threadIdx.x >> 5) * (kBlock * kAdamUnroll) + lane * 4;
-  T* p = static_cast<T*>(t.p);
-  const T* g = static_cast<const T*>(t.g);
+                        (threadIdx.x >> 5) * (kBlock * U) + lane * 4;
+  // elements from this lane's first one to the tensor's end
+  const int left = static_cast<int>(max(min(t.n - first, static_cast<int64_t>(kChunk)),
+                                        -static_cast<int64_t>(kChunk)));
+  T* p = static_cast<T*>(t.p) + first;
+  const T* g = static_cast<const T*>(t.g) + first;
   const bool vec = (reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) %
                        (4 * sizeof(T)) == 0;
+  const int64_t s0 = t.offset + first;
+  float* const master = a.master + s0;
+  uint8_t *const m8 = static_cast<uint8_t*>(a.m) + s0, *const v8 = static_cast<uint8_t*>(a.v) + s0;
+  uint8_t *const me = a.me + s0 / kBlock, *const ve = a.ve + s0 / kBlock;
+  float *const m32 = static_cast<float*>(a.m) + s0, *const v32 = static_cast<float*>(a.v) + s0;
   const float scale = a.grad_scale == nullptr ? 1.f : __ldg(a.grad_scale);
 
+  // everything is on its way before the first use
+  Raw<4 * sizeof(T)> rg[U], rp[U];
+  Raw<16> rx[U], rm[U], rv[U];
+  uint32_t cm[U], cv[U], em[U], ev[U];
 #pragma unroll
-  for (int u = 0; u < kAdamUnroll; ++u) {
-    const int64_t e0 = first + u * kBlock;
-    if (e0 - lane * 4 >= t.n) break;  // the whole warp: a block that does not exist
-    const int valid = static_cast<int>(min(max(t.n - e0, int64_t{0}), int64_t{4}));
-    const int64_t s0 = t.offset + e0;
-    float x[4], d[4], m[4], v[4];
-    adam_load(g + e0, valid, vec, d);
-    if (MASTER) adam_load(a.master + s0, 4, true, x);
-    else adam_load(p + e0, valid, vec, x);
+  for (int u = 0; u < U; ++u) {
+    const int valid = left - u * kBlock;
+    if (valid + lane * 4 <= 0) continue;  // the whole warp: a block that is not there
+    rg[u] = adam_load(g + u * kBlock, min(valid, 4), vec);
+    if (MASTER) rx[u] = adam_load(master + u * kBlock, 4, true);
+    else rp[u] = adam_load(p + u * kBlock, min(valid, 4), vec);
     if (SMALL) {
-      const uint32_t cm = *reinterpret_cast<const uint32_t*>(static_cast<uint8_t*>(a.m) + s0);
-      const uint32_t cv = *reinterpret_cast<const uint32_t*>(static_cast<uint8_t*>(a.v) + s0);
-      const uint32_t em = a.me[s0 / kBlock], ev = a.ve[s0 / kBlock];
+      cm[u] = *reinterpret_cast<const uint32_t*>(m8 + u * kBlock);
+      cv[u] = *reinterpret_cast<const uint32_t*>(v8 + u * kBlock);
+      em[u] = me[u];
+      ev[u] = ve[u];
+    } else {
+      rm[u] = adam_load(m32 + u * kBlock, 4, true);
+      rv[u] = adam_load(v32 + u * kBlock, 4, true);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int valid = left - u * kBlock;
+    if (valid + lane * 4 <= 0) break;
+    float x[4], d[4], m[4], v[4];
+    Chunk<T, 4 * sizeof(T)>::unpack(rg[u], d);
+    if (MASTER) Chunk<float, 16>::unpack(rx[u], x);
+    else Chunk<T, 4 * sizeof(T)>::unpack(rp[u], x);
+    if (SMALL) {
+      const uint32_t sm = adam_shift(em[u], 15u), sv = adam_shift(ev[u], 31u);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        m[i] = adam_decode<15, true>(cm >> (8 * i) & 255u, em);
-        v[i] = adam_decode<31, false>(cv >> (8 * i) & 255u, ev);
+        m[i] = adam_decode<true>(cm[u], i, sm);
+        v[i] = adam_decode<false>(cv[u], i, sv);
       }
     } else {
-      adam_load(static_cast<const float*>(a.m) + s0, 4, true, m);
-      adam_load(static_cast<const float*>(a.v) + s0, 4, true, v);
+      Chunk<float, 16>::unpack(rm[u], m);
+      Chunk<float, 16>::unpack(rv[u], v);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float e = d[i] * scale;
       m[i] = a.b1 * m[i] + a.c1 * e;
       v[i] = a.b2 * v[i] + a.c2 * e * e;
-      x[i] = a.decay * x[i] - t.step_size * __fdividef(m[i], sqrtf(v[i]) * t.inv_sqrt_bc2 + a.eps);
-      if (i >= valid) m[i] = v[i] = x[i] = 0.f;  // between tensors
+      x[i] = a.decay * x[i] -
+             t.step_size * __fdividef(m[i], adam_sqrt(v[i]) * t.inv_sqrt_bc2 + a.eps);
     }
-    adam_store(p + e0, valid, vec, x);
-    if (MASTER) adam_store(a.master + s0, 4, true, x);
+    if (valid < 4) {  // between tensors
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i >= valid) m[i] = v[i] = x[i] = 0.f;
+    }
+    adam_store(p + u * kBlock, min(valid, 4), vec, x);
+    if (MASTER) adam_store(master + u * kBlock, 4, true, x);
     if (SMALL) {
-      uint32_t rm[4], rv[4], em, ev;
+      uint32_t qm[4], qv[4], nm, nv;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t r = adam_random(static_cast<uint32_t>(s0) + i, t.key);
-        rm[i] = ((r & 0xffffu) << 4) + 8u;
-        rv[i] = ((r >> 16) << 4) + 8u;
+        const uint32_t r = adam_random(static_cast<uint32_t>(s0) + u * kBlock + i, t.key);
+        qm[i] = (r << 4 & 0xffff0u) | 8u;
+        qv[i] = (r >> 12 & 0xffff0u) | 8u;
       }
-      const uint32_t cm = adam_encode<15, true>(m, rm, em);
-      const uint32_t cv = adam_encode<31, false>(v, rv, ev);
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + s0) = cm;
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + s0) = cv;
+      const uint32_t wm = adam_encode<15u, true>(m, qm, nm);
+      const uint32_t wv = adam_encode<31u, false>(v, qv, nv);
+      *reinterpret_cast<uint32_t*>(m8 + u * kBlock) = wm;
+      *reinterpret_cast<uint32_t*>(v8 + u * kBlock) = wv;
       if (lane == 0) {
-        a.me[s0 / kBlock] = static_cast<uint8_t>(em);
-        a.ve[s0 / kBlock] = static_cast<uint8_t>(ev);
+        me[u] = static_cast<uint8_t>(nm);
+        ve[u] = static_cast<uint8_t>(nv);
       }
     } else {
-      adam_store(static_cast<float*>(a.m) + s0, 4, true, m);
-      adam_store(static_cast<float*>(a.v) + s0, 4, true, v);
+      adam_store(m32 + u * kBlock, 4, true, m);
+      adam_store(v32 + u * kBlock, 4, true, v);
     }
   }
 }
@@ -234,11 +282,12 @@ adamw_values_kernel(const uint8_t* m, const uint8_t* me, const uint8_t* v, const
   const uint2 cm = __ldg(reinterpret_cast<const uint2*>(m + i));
   const uint2 cv = __ldg(reinterpret_cast<const uint2*>(v + i));
   const uint32_t em = __ldg(me + i / kBlock), ev = __ldg(ve + i / kBlock);
+  const uint32_t sm = adam_shift(em, 15u), sv = adam_shift(ev, 31u);
   float fm[8], fv[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    fm[k] = adam_decode<15, true>((k < 4 ? cm.x : cm.y) >> (8 * (k & 3)) & 255u, em);
-    fv[k] = adam_decode<31, false>((k < 4 ? cv.x : cv.y) >> (8 * (k & 3)) & 255u, ev);
+    fm[k] = adam_decode<true>(k < 4 ? cm.x : cm.y, k & 3, sm);
+    fv[k] = adam_decode<false>(k < 4 ? cv.x : cv.y, k & 3, sv);
   }
   st_chunk<16>(mo + i, Chunk<__nv_bfloat16, 16>::pack(fm));
   st_chunk<16>(vo + i, Chunk<__nv_bfloat16, 16>::pack(fv));

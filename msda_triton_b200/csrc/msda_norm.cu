@@ -8,18 +8,21 @@
 namespace msda {
 namespace {
 
-// Bytes of input per wave: what the application pass finds in L2 again.
-constexpr int64_t kWaveBytes = 40 << 20;
-// Narrowest row piece that a slab is cut to, and the input bytes of a tile.
-constexpr int64_t kSlabBytes = 64;
-constexpr int64_t kTileBytes = 64 << 10;
+// Bytes of input per wave, and of the largest unit that counts as one that L2 holds.
+constexpr int64_t kWaveBytes = int64_t{1} << 30;
+constexpr int64_t kFitBytes = 72 << 20;
+// Row pieces that a segment is cut to: as wide as this, narrower (whole lines
+// still) where a unit only then fits; and the input bytes of a tile.
+constexpr int64_t kSlabBytes = 256;
+constexpr int64_t kMinPiece = 128;
+constexpr int64_t kTileBytes = 128 << 10;
 // CTAs that a pass over everything should have at least.
 constexpr int64_t kMinTiles = 148 * 4;
 
 struct Plan {
   NormLevel lv[kMaxLevels];
   int64_t tiles;    // over all levels
-  int64_t units;
+  int64_t counters;
   int32_t partial_stride;
   int64_t partial, done, chan, coef, bytes;  // offsets into the workspace, and its size
   int64_t zero, zero_bytes;                  // the part that starts as zeros
@@ -32,38 +35,41 @@ int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 int make_plan(int dtype, int64_t B, int64_t C, int64_t G, int64_t L, const int64_t* rows,
               bool backward, Plan& p) {
   const int64_t es = elem_bytes(dtype), cg = C / G;
-  const int64_t row_bytes = C * es * (backward ? 2 : 1);
+  const int64_t streams = backward ? 2 : 1, row_bytes = C * es * streams;
   int64_t total = 0;
   for (int64_t l = 0; l < L; ++l) total += B * rows[l] * row_bytes;
-  p.tiles = p.units = 0;
+  p.tiles = p.counters = 0;
   int64_t slab_groups_max = 1;
   for (int64_t l = 0; l < L; ++l) {
     NormLevel& v = p.lv[l];
     v.rows = rows[l];
     v.block0 = p.tiles;
-    v.unit0 = static_cast<int32_t>(p.units);
-    // A segment that a wave holds keeps whole rows (of at most kNormMaxSlab
-    // channels); a longer one is cut into slabs that a wave holds, if pieces
-    // of kSlabBytes do.
-    int64_t sg = std::min(G, std::max<int64_t>(1, kNormMaxSlab / cg));
-    if (rows[l] * row_bytes > kWaveBytes) {
-      const int64_t fit = kWaveBytes * C / (rows[l] * row_bytes);  // channels
-      const int64_t least = ceil_div(kSlabBytes, cg * es);         // groups
-      if (fit >= least * cg) sg = std::min(sg, fit / cg);
-      else if (2 * fit >= least * cg) sg = std::min(sg, least);
+    v.done0 = static_cast<int32_t>(p.counters);
+    // Slabs of whole lines; narrower ones where a wave only then holds a slab.
+    int64_t piece_bytes = kSlabBytes, sg = 1;
+    for (;; piece_bytes /= 2) {
+      sg = std::min(G, std::max<int64_t>(1, std::min(ceil_div(piece_bytes, cg * es), kNormMaxSlab / cg)));
+      if (rows[l] * sg * cg * es * streams <= kFitBytes || piece_bytes <= kMinPiece) break;
+    }
+    const int64_t unit = std::max<int64_t>(1, rows[l] * sg * cg * es * streams);
+    const int64_t slabs = ceil_div(G, sg);
+    v.run = static_cast<int32_t>(unit > kFitBytes ? slabs : std::min(slabs, std::max<int64_t>(1, kWaveBytes / unit)));
+    if (unit > kFitBytes) {  // no residency
+      sg = std::min(G, std::max<int64_t>(1, std::min(ceil_div(kSlabBytes, cg * es), kNormMaxSlab / cg)));
+      v.run = static_cast<int32_t>(ceil_div(G, sg));
     }
     v.slab_groups = static_cast<int32_t>(sg);
     v.slabs = static_cast<int32_t>(ceil_div(G, sg));
     slab_groups_max = std::max(slab_groups_max, sg);
     const int64_t piece = sg * cg * es * (backward ? 2 : 1);
-    const int64_t tile = std::min(kTileBytes, std::max<int64_t>(total / kMinTiles, 4096));
+    const int64_t tile = std::min(kTileBytes, std::max<int64_t>(total / kMinTiles, 16384));
     v.tile_rows = static_cast<int32_t>(std::max<int64_t>(
         1, std::min<int64_t>({rows[l], tile / piece, int64_t{1} << 30})));
     v.tiles = static_cast<int32_t>(ceil_div(rows[l], v.tile_rows));
     const int64_t units = rows[l] > 0 ? B * v.slabs : 0;
-    p.units += units;
+    p.counters += units * (1 + ceil_div(v.tiles, kNormFan));
     p.tiles += units * v.tiles;
-    if (rows[l] > (int64_t{1} << 30) || p.units > (int64_t{1} << 30))
+    if (rows[l] > (int64_t{1} << 30) || p.counters > (int64_t{1} << 30))
       return report(MSDA_ERROR_INT32_OVERFLOW, "level %lld: too many rows",
                     static_cast<long long>(l));
   }
@@ -74,7 +80,7 @@ int make_plan(int dtype, int64_t B, int64_t C, int64_t G, int64_t L, const int64
   p.coef = at;
   at += backward ? round_up(B * L * G * 8, 256) : 0;
   p.zero = p.done = at;
-  at += round_up(p.units * 4, 256);
+  at += round_up(p.counters * 4, 256);
   p.chan = at;
   at += backward ? round_up(B * L * C * 8, 256) : 0;
   p.zero_bytes = at - p.zero;
@@ -124,34 +130,32 @@ int vector_bytes(const Plan& p, int64_t L, int64_t cg, int64_t es, bool backward
 // Waves of whole units, each of kWaveBytes of input if units are that small.
 cudaError_t launch_waves(const NormArgs& a, const Plan& p, int64_t B, int dtype, int vb, int act,
                          bool backward, cudaStream_t st) {
-  NormWave w{0, 0, 0, 0};
+  NormWave w{0, 0, 0, 0, (int)envi("X_ORDER", 1)};
   const int64_t es = elem_bytes(dtype) * (backward ? 2 : 1);
   int64_t in_wave = 0;
   auto flush = [&]() {
     const cudaError_t err = norm_wave(a, w, dtype, vb, act, backward, st);
-    w = NormWave{w.stats0, w.stats0 + w.stats, w.stats, 0};
+    w = NormWave{w.stats0, w.stats0 + w.stats, w.stats, 0, w.order};
     in_wave = 0;
     return err;
   };
   for (int l = 0; l < a.L; ++l) {
     const NormLevel& v = a.lv[l];
-    int64_t left = v.rows > 0 ? B * v.slabs : 0;
-    const int64_t unit = v.rows * std::min<int64_t>(v.slab_groups * a.cg, a.C) * es;
-    while (left > 0) {
-      int64_t take = std::min(left, (kWaveBytes - in_wave) / unit);
-      if (take == 0 && in_wave == 0) take = 1;
-      if (take > 0) {
+    if (v.rows == 0) continue;
+    for (int64_t b = 0; b < B; ++b)
+      for (int32_t s0 = 0; s0 < v.slabs; s0 += v.run) {
+        const int32_t width = std::min(v.run, v.slabs - s0);
+        const int64_t bytes = v.rows * es *
+                              (std::min<int64_t>((s0 + width) * v.slab_groups * a.cg, a.C) -
+                               static_cast<int64_t>(s0) * v.slab_groups * a.cg);
         // a launch's tiles are counted in 32 bits
-        take = std::max<int64_t>(1, std::min<int64_t>(take, (1 << 28) / v.tiles));
-        w.stats += static_cast<int32_t>(take * v.tiles);
-        in_wave += take * unit;
-        left -= take;
+        if (w.stats > 0 && (in_wave + bytes > kWaveBytes || w.stats > (1 << 28))) {
+          const cudaError_t err = flush();
+          if (err != cudaSuccess) return err;
+        }
+        w.stats += width * v.tiles;
+        in_wave += bytes;
       }
-      if (left > 0) {
-        const cudaError_t err = flush();
-        if (err != cudaSuccess) return err;
-      }
-    }
   }
   cudaError_t err = flush();
   if (err == cudaSuccess && w.applies > 0) err = flush();

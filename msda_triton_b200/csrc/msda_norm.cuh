@@ -35,6 +35,7 @@ namespace msda {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormMaxSlab = 256;  // channels of a slab of several groups
+constexpr int kNormFan = 32;       // tiles whose results are joined at a time
 
 struct NormLevel {
   const char* x;       // first row of batch entry 0
@@ -43,11 +44,12 @@ struct NormLevel {
   int64_t x_batch, x_row, out_batch, out_row, gy_batch, gy_row;  // strides in elements
   int64_t rows;
   int64_t block0;      // first tile of the level, counted over all levels
-  int32_t unit0;       // first unit
+  int32_t done0;       // first of the level's counters: per unit one, and one per kNormFan tiles
   int32_t tiles;       // tiles per unit
   int32_t tile_rows;
   int32_t slabs;       // slabs per segment
   int32_t slab_groups; // groups per slab; the last may have fewer
+  int32_t run;         // slabs of a segment that go together, tile by tile
 };
 
 struct NormArgs {
@@ -61,7 +63,7 @@ struct NormArgs {
   float2* partial;     // per tile: per group of the slab (mean, sum of squared deviations);
                        // backward: per channel of the slab (s1, s2)
   int32_t partial_stride;
-  unsigned int* done;  // per unit: tiles whose statistics are written
+  unsigned int* done;  // counters of partial results that are written
   float2* chan;        // backward, (B, L, C): s1, s2
   float2* coef;        // backward, (B, L, G): a, q
 };
@@ -70,6 +72,7 @@ struct NormArgs {
 struct NormWave {
   int64_t apply0, stats0;
   int32_t applies, stats;
+  int32_t order;
 };
 
 struct NormParamGrad {

@@ -16,8 +16,9 @@ libmsda_b200.so (msda_group_norm_fwd / _bwd); there is no CPU fallback.
 
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
+from array import array
 from collections.abc import Sequence
 
 import torch
@@ -47,21 +48,20 @@ def _check(x, spatial_shapes, num_groups, weight, bias, activation):
     if not xs:
         raise ValueError("pyramid_group_norm needs at least one level")
     first = xs[0]
+    device, dtype, shape = first.device, first.dtype, first.shape
+    if not first.is_cuda:
+        raise ValueError("pyramid_group_norm requires CUDA tensors. Got CPU tensors instead.")
+    if dtype not in _core._DTYPE_CODE:
+        raise NotImplementedError("pyramid_group_norm only supports fp32, fp16, and bf16. "
+                                  f"Got {dtype}.")
     for t in xs:
-        if not t.is_cuda:
-            raise ValueError("pyramid_group_norm requires CUDA tensors. "
-                             "Got CPU tensors instead.")
-        if t.dtype not in _core._DTYPE_CODE:
-            raise NotImplementedError("pyramid_group_norm only supports fp32, fp16, and bf16. "
-                                      f"Got {t.dtype}.")
         if t.dim() < 3 or (not maps and t.dim() != 3):
             raise ValueError("x must be (B, K, C), or levels of (B, *spatial, C); "
                              f"got {tuple(t.shape)}")
-        if (t.device != first.device or t.dtype != first.dtype or t.shape[0] != first.shape[0]
-                or t.shape[-1] != first.shape[-1]):
+        if t is not first and (t.device != device or t.dtype != dtype
+                               or t.shape[0] != shape[0] or t.shape[-1] != shape[-1]):
             raise ValueError("levels must share their device, dtype, batch and channels; got "
-                             f"{tuple(t.shape)} {t.dtype} beside {tuple(first.shape)} "
-                             f"{first.dtype}")
+                             f"{tuple(t.shape)} {t.dtype} beside {tuple(shape)} {dtype}")
     if maps:
         if spatial_shapes is not None:
             sizes = [list(s) for s in _sizes(spatial_shapes)]
@@ -73,12 +73,12 @@ def _check(x, spatial_shapes, num_groups, weight, bias, activation):
         if spatial_shapes is None:
             raise ValueError("spatial_shapes is required for a flattened pyramid")
         sizes = _sizes(spatial_shapes)
-        if any(n < 0 for s in sizes for n in s):
-            raise ValueError(f"negative spatial shape: {sizes}")
         rows = [math.prod(s) for s in sizes]
-        if sum(rows) != x.shape[1]:
-            raise ValueError(f"K={x.shape[1]} does not match sum of spatial shapes {sum(rows)}")
-    channels = first.shape[-1]
+        if any(min(s, default=0) < 0 for s in sizes):
+            raise ValueError(f"negative spatial shape: {sizes}")
+        if sum(rows) != shape[1]:
+            raise ValueError(f"K={shape[1]} does not match sum of spatial shapes {sum(rows)}")
+    channels = shape[-1]
     if num_groups < 1 or channels < 1 or channels % num_groups:
         raise ValueError(f"channels ({channels}) must be a positive multiple of num_groups "
                          f"({num_groups})")
@@ -87,11 +87,11 @@ def _check(x, spatial_shapes, num_groups, weight, bias, activation):
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
-        if t.device != first.device:
-            raise ValueError(f"{name} must be on {first.device}, got {t.device}")
+        if t.device != device:
+            raise ValueError(f"{name} must be on {device}, got {t.device}")
         if t.dtype not in _core._DTYPE_CODE:
             raise NotImplementedError(f"{name} must be fp32, fp16, or bf16. Got {t.dtype}.")
-        if tuple(t.shape) not in ((channels,), (len(rows), channels)):
+        if t.shape not in ((channels,), (len(rows), channels)):
             raise ValueError(f"{name} must be ({channels},) or ({len(rows)}, {channels}), "
                              f"got {tuple(t.shape)}")
     if weight is not None and bias is not None and weight.shape != bias.shape:
@@ -119,35 +119,38 @@ def _dense_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.numel() == 0 or _row_stride(t) is not None else t.contiguous()
 
 
-def _i64s(values) -> ctypes.Array:
-    return (ctypes.c_int64 * len(values))(*values)
+def _table(values) -> tuple[array, int]:
+    """A host table of 64-bit values (to be kept alive), and where it lies."""
+    table = array("q", values)
+    return table, table.buffer_info()[0]
 
 
-def _tables(maps, xs, rows):
+def _levels(maps, xs, rows):
     """Host tables of the levels' addresses and (batch, row) strides."""
     if maps:
         ptrs = [t.data_ptr() for t in xs]
         strides = [s for t in xs for s in (t.stride(0), _row_stride(t) or 0)]
     else:
         (x,) = xs
-        step = x.stride(1) * x.element_size()
-        ptrs, at = [], x.data_ptr()
+        batch, step, _ = x.stride()
+        ptrs, at, size = [], x.data_ptr(), x.element_size() * step
         for n in rows:
             ptrs.append(at)
-            at += n * step
-        strides = [x.stride(0), x.stride(1)] * len(rows)
-    return (ctypes.c_void_p * len(ptrs))(*ptrs), _i64s(strides)
+            at += n * size
+        strides = [batch, step] * len(rows)
+    return _table(ptrs), _table(strides)
 
 
 def _affine(weight, bias):
     """(weight, bias, dtype code, per_level) as the kernels take them."""
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        weight, bias = weight.float(), bias.float()
-    weight = None if weight is None else weight.detach().contiguous()
-    bias = None if bias is None else bias.detach().contiguous()
     one = weight if weight is not None else bias
     if one is None:
         return None, None, _lib.FLOAT32, 0
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        weight, bias = weight.float(), bias.float()
+        one = weight
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
     return weight, bias, _core._DTYPE_CODE[one.dtype], int(one.dim() == 2)
 
 
@@ -155,35 +158,40 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(dtype, batch, channels, groups, rows, backward, device):
-    n = _lib.lib().msda_group_norm_workspace_bytes(dtype, batch, channels, groups, len(rows),
-                                                   rows, int(backward))
-    return torch.empty((n,), device=device, dtype=torch.uint8), n
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(dtype, batch, channels, groups, rows, backward):
+    """A function of sizes alone."""
+    table = _table(rows)
+    return _lib.lib().msda_group_norm_workspace_bytes(dtype, batch, channels, groups, len(rows),
+                                                      table[1], backward)
 
 
 def norm_forward(maps, xs, rows, groups, weight, bias, eps, activation):
     """(y, statistics) of checked arguments."""
-    xs = [_dense_rows(t.detach()) for t in xs]
+    xs = [_dense_rows(t) for t in xs]
     first = xs[0]
     batch, channels, code = first.shape[0], first.shape[-1], _core._DTYPE_CODE[first.dtype]
     y = torch.empty((batch, sum(rows), channels), device=first.device, dtype=first.dtype)
-    stats = torch.empty((batch, len(rows), groups, 2), device=first.device, dtype=torch.float32)
+    # the statistics, and behind them (on a boundary of 256 bytes) the workspace
+    n_stats = -(-batch * len(rows) * groups * 2 // 64) * 64
+    ws_bytes = _workspace_bytes(code, batch, channels, groups, tuple(rows), 0)
+    stats = torch.empty((n_stats + ws_bytes // 4,), device=first.device, dtype=torch.float32)
     w, b, affine, per_level = _affine(weight, bias)
-    c_rows = _i64s(rows)
-    ptrs, strides = _tables(maps, xs, rows)
-    ws, ws_bytes = _workspace(code, batch, channels, groups, c_rows, False, first.device)
-    with torch.cuda.device(first.device):
-        _core.check_status(_lib.lib().msda_group_norm_fwd(
-            code, batch, channels, groups, len(rows), c_rows, ptrs, strides, _ptr(w), _ptr(b),
-            affine, per_level, eps, ACTIVATIONS[activation], y.data_ptr(), stats.data_ptr(),
-            ws.data_ptr(), ws_bytes, _core._stream_ptr(first.device)))
+    c_rows = _table(rows)
+    ptrs, strides = _levels(maps, xs, rows)
+    at = stats.data_ptr()
+    _core.launch(
+        _lib.lib().msda_group_norm_fwd, first.get_device(),
+        code, batch, channels, groups, len(rows), c_rows[1], ptrs[1], strides[1], _ptr(w), _ptr(b),
+        affine, per_level, eps, ACTIVATIONS[activation], y.data_ptr(), at, at + 4 * n_stats,
+        ws_bytes)
     return y, stats
 
 
 def norm_backward(maps, xs, rows, groups, weight, bias, activation, stats, grad_y):
     """(gradients of xs, of weight, of bias); the last two None where the input is."""
     shapes = [t.shape for t in xs]
-    xs = [_dense_rows(t.detach()) for t in xs]
+    xs = [_dense_rows(t) for t in xs]
     first = xs[0]
     batch, channels, code = first.shape[0], first.shape[-1], _core._DTYPE_CODE[first.dtype]
     grad_y = grad_y.to(first.dtype).contiguous()
@@ -191,16 +199,16 @@ def norm_backward(maps, xs, rows, groups, weight, bias, activation, stats, grad_
     w, b, affine, per_level = _affine(weight, bias)
     gw = None if w is None else torch.empty_like(w)
     gb = None if b is None else torch.empty_like(b)
-    c_rows = _i64s(rows)
-    ptrs, strides = _tables(maps, xs, rows)
-    gptrs, gstrides = _tables(maps, gxs, rows)
-    ws, ws_bytes = _workspace(code, batch, channels, groups, c_rows, True, first.device)
-    with torch.cuda.device(first.device):
-        _core.check_status(_lib.lib().msda_group_norm_bwd(
-            code, batch, channels, groups, len(rows), c_rows, ptrs, strides, _ptr(w), _ptr(b),
-            affine, per_level, ACTIVATIONS[activation], stats.data_ptr(), grad_y.data_ptr(),
-            gptrs, gstrides, _ptr(gw), _ptr(gb), ws.data_ptr(), ws_bytes,
-            _core._stream_ptr(first.device)))
+    c_rows = _table(rows)
+    ptrs, strides = _levels(maps, xs, rows)
+    gptrs, gstrides = _levels(maps, gxs, rows)
+    ws_bytes = _workspace_bytes(code, batch, channels, groups, tuple(rows), 1)
+    ws = torch.empty((ws_bytes,), device=first.device, dtype=torch.uint8)
+    _core.launch(
+        _lib.lib().msda_group_norm_bwd, first.get_device(),
+        code, batch, channels, groups, len(rows), c_rows[1], ptrs[1], strides[1], _ptr(w), _ptr(b),
+        affine, per_level, ACTIVATIONS[activation], stats.data_ptr(), grad_y.data_ptr(),
+        gptrs[1], gstrides[1], _ptr(gw), _ptr(gb), ws.data_ptr(), ws_bytes)
     return (gxs, None if gw is None else gw.to(weight.dtype),
             None if gb is None else gb.to(bias.dtype))
 
@@ -262,8 +270,11 @@ def pyramid_group_norm(x: torch.Tensor | Sequence[torch.Tensor],
                                       weight, bias, eps, activation)
         return y
     maps, xs, rows = _check(x, spatial_shapes, num_groups, weight, bias, activation)
-    return PyramidGroupNormFn.apply(maps, rows, num_groups, float(eps), activation, weight, bias,
-                                    *xs)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (weight, bias, *xs)):
+        return PyramidGroupNormFn.apply(maps, rows, num_groups, float(eps), activation, weight,
+                                        bias, *xs)
+    return norm_forward(maps, xs, rows, num_groups, weight, bias, float(eps), activation)[0]
 
 
 class PyramidGroupNorm(nn.Module):

@@ -153,7 +153,8 @@ def group_norm_forward(x: list[Tensor], maps: bool, spatial_shapes: Tensor | Non
 
     maps, xs, rows = norm._check(x if maps else x[0], spatial_shapes, num_groups, weight, bias,
                                  activation)
-    return norm.norm_forward(maps, xs, rows, num_groups, weight, bias, eps, activation)
+    y, stats = norm.norm_forward(maps, xs, rows, num_groups, weight, bias, eps, activation)
+    return y, stats[:y.shape[0] * len(rows) * num_groups * 2]
 
 
 @group_norm_forward.register_fake
@@ -162,7 +163,7 @@ def _group_norm_forward_fake(x, maps, spatial_shapes, num_groups, weight, bias, 
     keys = sum(t.shape[1:-1].numel() for t in x)
     levels = len(x) if maps else spatial_shapes.shape[0]
     return (first.new_empty((first.shape[0], keys, first.shape[-1])),
-            first.new_empty((first.shape[0], levels, num_groups, 2), dtype=torch.float32))
+            first.new_empty((first.shape[0] * levels * num_groups * 2,), dtype=torch.float32))
 
 
 @torch.library.custom_op("msda_b200::group_norm_backward", mutates_args=())

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 from array import array
 from collections.abc import Sequence
+from operator import attrgetter, eq
 
 import torch
 from torch import Tensor
@@ -63,15 +64,18 @@ def _flat(t: Tensor, at: int, p: Tensor) -> Tensor:
     return t.as_strided(p.shape, p.stride(), at)
 
 
+_dtype_of, _shape_of = attrgetter("dtype"), attrgetter("shape")
+
+
 def _one_kind(params: Sequence[Tensor]) -> None:
     if not params:
         return
-    dtype, device = params[0].dtype, params[0].device
+    dtype = params[0].dtype
     if not params[0].is_cuda:
         raise ValueError("AdamW requires CUDA tensors. Got CPU tensors instead.")
     if dtype not in _core._DTYPE_CODE:
         raise NotImplementedError(f"AdamW only supports fp32, fp16, and bf16. Got {dtype}.")
-    if any(p.dtype != dtype for p in params) or any(p.device != device for p in params):
+    if len(set(map(_dtype_of, params))) > 1 or len(set(map(Tensor.get_device, params))) > 1:
         raise ValueError("the tensors of a step must share their dtype and device")
 
 
@@ -160,45 +164,47 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor | None],
         return
     _one_kind(params)
     first = params[0]
-    dtype, device = first.dtype, first.device
+    dtype, device, index = first.dtype, first.device, first.get_device()
     bits, elements = _state_tensors(state, dtype, device)
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("adamw_step cannot be captured in a CUDA graph: the step's bias "
                            "corrections are computed on the host")
-    live = [p for p, g in zip(params, grads) if g is not None]
-    given = [g for g in grads if g is not None] if len(live) < n else grads
-    if any(g.dtype != dtype for g in given) or any(g.device != device for g in given):
+    given, live = grads, params
+    if any(g is None for g in grads):
+        given = [g for g in grads if g is not None]
+        live = [p for p, g in zip(params, grads) if g is not None]
+        if not live:
+            return
+    if set(map(_dtype_of, given)) != {dtype} or set(map(Tensor.get_device, given)) != {index}:
         raise ValueError(f"gradients must be {dtype} on {device}, as the tensors")
     # the usual case, dense tensors of the same shape, is checked without a loop in Python
-    if not (all(map(Tensor.is_contiguous, live)) and all(map(Tensor.is_contiguous, given))
-            and [p.shape for p in live] == [g.shape for g in given]):
+    if not (all(map(Tensor.is_contiguous, params)) and all(map(Tensor.is_contiguous, given))
+            and all(map(eq, map(_shape_of, live), map(_shape_of, given)))):
         given = [_laid_out(p, g) for p, g in zip(live, given)]
-    if len(live) == n:
-        grad_ptrs = [g.data_ptr() for g in given]
-    else:
-        rest = iter(given)
-        grad_ptrs = [0 if g is None else next(rest).data_ptr() for g in grads]
+    g_ptr = array("q", map(Tensor.data_ptr, given))
+    if live is not params:
+        rest = iter(g_ptr)
+        g_ptr = array("q", [0 if g is None else next(rest) for g in grads])
     if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1
                                    or grad_scale.device != device):
         raise ValueError(f"grad_scale must be one fp32 value on {device}")
-    steps = [int(step)] * n if not isinstance(step, Sequence) else [int(s) for s in step]
-    if len(steps) != n:
-        raise ValueError(f"{n} tensors and {len(steps)} steps")
-    p_ptr = array("Q", [p.data_ptr() for p in params])
-    g_ptr = array("Q", grad_ptrs)
-    counts = array("q", [p.numel() for p in params])
-    t = array("q", steps)
+    if isinstance(step, int):
+        steps = array("q", [step]) * n
+    else:
+        steps = array("q", map(int, step))
+        if len(steps) != n:
+            raise ValueError(f"{n} tensors and {len(steps)} steps")
+    p_ptr = array("q", map(Tensor.data_ptr, params))
+    counts = array("q", map(Tensor.numel, params))
     address = lambda a: a.buffer_info()[0]  # noqa: E731
     ptr = lambda name: state[name].data_ptr() if name in state else None  # noqa: E731
-    with torch.cuda.device(device):
-        code = _lib.lib().msda_adamw_step(
-            _core._DTYPE_CODE[dtype], bits, n, address(p_ptr), address(g_ptr), address(counts),
-            address(t), float(lr), float(betas[0]), float(betas[1]), float(eps),
-            float(weight_decay), int(seed) & 0xFFFFFFFF,
-            None if grad_scale is None else grad_scale.data_ptr(), ptr("exp_avg"),
-            ptr("exp_avg_sq"), ptr("exp_avg_exponent"), ptr("exp_avg_sq_exponent"),
-            ptr("master"), elements, _core._stream_ptr(device))
-    _core.check_status(code)
+    _core.launch(
+        _lib.lib().msda_adamw_step, index,
+        _core._DTYPE_CODE[dtype], bits, n, address(p_ptr), address(g_ptr), address(counts),
+        address(steps), lr, betas[0], betas[1], eps, weight_decay, int(seed) & 0xFFFFFFFF,
+        None if grad_scale is None else grad_scale.data_ptr(), ptr("exp_avg"),
+        ptr("exp_avg_sq"), ptr("exp_avg_exponent"), ptr("exp_avg_sq_exponent"),
+        ptr("master"), elements)
     torch.autograd.graph.increment_version(live)
     torch.autograd.graph.increment_version(state.values())
 
@@ -214,11 +220,10 @@ def adamw_state_values(state: dict[str, Tensor]) -> tuple[Tensor, Tensor]:
     if bits == 32:
         return m, v
     out = [torch.empty(n, device=m.device, dtype=torch.bfloat16) for _ in range(2)]
-    with torch.cuda.device(m.device):
-        _core.check_status(_lib.lib().msda_adamw_values(
-            m.data_ptr(), state["exp_avg_exponent"].data_ptr(), v.data_ptr(),
-            state["exp_avg_sq_exponent"].data_ptr(), n, out[0].data_ptr(), out[1].data_ptr(),
-            _core._stream_ptr(m.device)))
+    _core.launch(_lib.lib().msda_adamw_values, m.get_device(),
+                 m.data_ptr(), state["exp_avg_exponent"].data_ptr(), v.data_ptr(),
+                 state["exp_avg_sq_exponent"].data_ptr(), n, out[0].data_ptr(),
+                 out[1].data_ptr())
     return out[0], out[1]
 
 

@@ -12,7 +12,7 @@ fallback.
 
 from __future__ import annotations
 
-import ctypes
+from array import array
 from collections.abc import Sequence
 
 import torch
@@ -73,85 +73,92 @@ def _check(xs, positions, inv_freq, axis_index):
     first = xs[0]
     if not first.is_cuda:
         raise ValueError("rotary requires CUDA tensors. Got CPU tensors instead.")
-    for x in xs:
-        if x.dtype not in _core._DTYPE_CODE:
-            raise NotImplementedError("rotary only supports fp32, fp16, and bf16. "
-                                      f"Got {x.dtype}.")
-        if x.dim() != 4:
-            raise ValueError(f"expected (B, Q, H, C), got {tuple(x.shape)}")
-        if (x.device != first.device or x.dtype != first.dtype or x.shape[:2] != first.shape[:2]
-                or x.shape[3] != first.shape[3]):
+    dtype, device, shape = first.dtype, first.device, first.shape
+    if dtype not in _core._DTYPE_CODE:
+        raise NotImplementedError(f"rotary only supports fp32, fp16, and bf16. Got {dtype}.")
+    if len(shape) != 4:
+        raise ValueError(f"expected (B, Q, H, C), got {tuple(shape)}")
+    B, Q, _, C = shape
+    for x in xs[1:]:
+        other = x.shape
+        if (x.device != device or x.dtype != dtype or len(other) != 4 or other[0] != B
+                or other[1] != Q or other[3] != C):
             raise ValueError("queries and keys must share their device, dtype, batch, tokens and "
-                             f"channels; got {tuple(x.shape)} {x.dtype} beside "
-                             f"{tuple(first.shape)} {first.dtype}")
+                             f"channels; got {tuple(other)} {x.dtype} beside {tuple(shape)} "
+                             f"{dtype}")
     if positions.dim() == 2:
         positions = positions[None]
-    B, Q, _, C = first.shape
-    if positions.dim() != 3 or positions.shape[0] not in (1, B) or positions.shape[1] != Q:
+    where = positions.shape
+    if len(where) != 3 or where[0] not in (1, B) or where[1] != Q:
         raise ValueError(f"positions must be (Q, A) or (1 or B, Q, A) with B={B}, Q={Q}; "
-                         f"got {tuple(positions.shape)}")
-    if not 1 <= positions.shape[2] <= MAX_AXES:
-        raise ValueError(f"positions must have 1 to {MAX_AXES} axes, got {positions.shape[2]}")
+                         f"got {tuple(where)}")
+    if not 1 <= where[2] <= MAX_AXES:
+        raise ValueError(f"positions must have 1 to {MAX_AXES} axes, got {where[2]}")
     if positions.dtype == torch.bool or positions.is_complex():
         raise ValueError(f"positions must be numbers, got {positions.dtype}")
-    if (inv_freq.dim() != 1 or inv_freq.dtype != torch.float32
-            or axis_index.shape != inv_freq.shape or axis_index.dtype != torch.int32):
+    pairs = inv_freq.shape
+    if (len(pairs) != 1 or inv_freq.dtype != torch.float32 or axis_index.shape != pairs
+            or axis_index.dtype != torch.int32):
         raise ValueError("inv_freq must be (pairs,) fp32 and axis_index (pairs,) int32, got "
-                         f"{tuple(inv_freq.shape)} {inv_freq.dtype} and "
+                         f"{tuple(pairs)} {inv_freq.dtype} and "
                          f"{tuple(axis_index.shape)} {axis_index.dtype}")
-    pairs = inv_freq.shape[0]
-    if 2 * pairs > C or pairs > MAX_PAIRS:
-        raise ValueError(f"{pairs} pairs do not fit {C} channels (and at most {MAX_PAIRS})")
-    for name, t in (("positions", positions), ("inv_freq", inv_freq), ("axis_index", axis_index)):
-        if t.device != first.device:
-            raise ValueError(f"{name} must be on {first.device}, got {t.device}")
+    if 2 * pairs[0] > C or pairs[0] > MAX_PAIRS:
+        raise ValueError(f"{pairs[0]} pairs do not fit {C} channels (and at most {MAX_PAIRS})")
+    if positions.device != device or inv_freq.device != device or axis_index.device != device:
+        raise ValueError(f"positions, inv_freq and axis_index must be on {device}, got "
+                         f"{positions.device}, {inv_freq.device} and {axis_index.device}")
     return positions
 
 
 def _positions(positions):
     """In a dtype and layout that the kernel reads."""
-    p = positions.detach()
-    if p.dtype not in _POSITION_CODE:
-        p = p.float() if p.dtype.is_floating_point else p.long()
-    return p.contiguous()
+    if positions.dtype not in _POSITION_CODE:
+        p = positions.detach()
+        positions = p.float() if p.dtype.is_floating_point else p.long()
+    return positions if positions.is_contiguous() else positions.detach().contiguous()
 
 
 def _dense_channels(x):
-    x = x.detach()
-    return x if x.stride(3) == 1 or x.shape[3] <= 1 else x.contiguous()
+    return x if x.stride(3) == 1 or x.shape[3] <= 1 else x.detach().contiguous()
 
 
-def _ptrs(ts):
-    return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
+def _address(values) -> tuple[array, int]:
+    """A host table of 64-bit values (to be kept alive), and where it lies."""
+    table = array("q", values)
+    return table, table.buffer_info()[0]
 
 
-def _strides(ts):
-    return (ctypes.c_int64 * (3 * len(ts)))(*[s for t in ts for s in t.stride()[:3]])
+def _tables(ts):
+    """Host tables of the tensors' addresses and of their (batch, token, head) strides."""
+    strides = []
+    for t in ts:
+        strides += t.stride()[:3]
+    return _address([t.data_ptr() for t in ts]), _address(strides)
 
 
 def turn(xs, ys, positions, inv_freq, axis_index, interleaved, inverse, inputs=None, gpos=None):
     """Launch on prepared tensors: ys are the xs turned (or turned back)."""
     first = xs[0]
     B, Q, _, C = first.shape
-    shared = positions.shape[0] == 1
-    heads = (ctypes.c_int64 * len(xs))(*[x.shape[2] for x in xs])
-    with torch.cuda.device(first.device):
-        _core.check_status(_lib.lib().msda_rotary(
-            _core._DTYPE_CODE[first.dtype], B, Q, C, len(xs), heads, _ptrs(xs), _strides(xs),
-            _ptrs(ys), _strides(ys), positions.data_ptr(), _POSITION_CODE[positions.dtype],
-            0 if shared else Q * positions.shape[2], positions.shape[2], inv_freq.data_ptr(),
-            axis_index.data_ptr(), inv_freq.shape[0], int(interleaved), int(inverse),
-            None if inputs is None else _ptrs(inputs),
-            None if inputs is None else _strides(inputs),
-            None if gpos is None else gpos.data_ptr(), _core._stream_ptr(first.device)))
+    batch, _, axes = positions.shape
+    heads = _address([x.shape[2] for x in xs])
+    (px, sx), (py, sy) = _tables(xs), _tables(ys)
+    pi, si = _tables(inputs) if inputs is not None else ((None, None), (None, None))
+    _core.launch(
+        _lib.lib().msda_rotary, first.get_device(),
+        _core._DTYPE_CODE[first.dtype], B, Q, C, len(xs), heads[1], px[1], sx[1], py[1], sy[1],
+        positions.data_ptr(), _POSITION_CODE[positions.dtype], 0 if batch == 1 else Q * axes, axes,
+        inv_freq.data_ptr(), axis_index.data_ptr(), inv_freq.shape[0], interleaved, inverse,
+        pi[1], si[1], None if gpos is None else gpos.data_ptr())
 
 
-def _new(xs):
-    return [torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in xs]
+def _new(x):
+    return (torch.empty_like(x) if x.is_contiguous()
+            else torch.empty(x.shape, device=x.device, dtype=x.dtype))
 
 
 def rotary_forward(positions, inv_freq, axis_index, interleaved, xs):
-    ys = _new(xs)
+    ys = [_new(x) for x in xs]
     turn([_dense_channels(x) for x in xs], ys, _positions(positions), inv_freq.contiguous(),
          axis_index.contiguous(), interleaved, False)
     return ys
@@ -160,7 +167,7 @@ def rotary_forward(positions, inv_freq, axis_index, interleaved, xs):
 def rotary_backward(positions, inv_freq, axis_index, interleaved, grads, inputs=None):
     """(gradients of the inputs, of the positions or None without `inputs`)."""
     grads = [_dense_channels(g) for g in grads]
-    gxs, pos, gpos = _new(grads), _positions(positions), None
+    gxs, pos, gpos = [_new(g) for g in grads], _positions(positions), None
     if inputs is not None:
         B, Q = grads[0].shape[:2]
         gpos = torch.empty((B, Q, pos.shape[2]), device=pos.device, dtype=torch.float32)
@@ -202,7 +209,9 @@ def _apply(xs, positions, inv_freq, axis_index, interleaved):
             positions = positions[None]
         return tuple(ops.rotary_forward(list(xs), positions, inv_freq, axis_index, interleaved))
     positions = _check(xs, positions, inv_freq, axis_index)
-    return RotaryFn.apply(positions, inv_freq, axis_index, bool(interleaved), *xs)
+    if torch.is_grad_enabled() and (positions.requires_grad or any(x.requires_grad for x in xs)):
+        return RotaryFn.apply(positions, inv_freq, axis_index, bool(interleaved), *xs)
+    return tuple(rotary_forward(positions, inv_freq, axis_index, bool(interleaved), xs))
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -249,9 +258,8 @@ def rotary_qk_(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fr
             raise ValueError("rotary_qk_ needs dense channels")
         if any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
             raise ValueError("rotary_qk_ cannot write to an expanded tensor")
-    xs = [q.detach(), k.detach()]
-    turn(xs, xs, _positions(positions), inv_freq.contiguous(), axis_index.contiguous(),
-         interleaved, False)
+    turn((q, k), (q, k), _positions(positions), inv_freq.contiguous(), axis_index.contiguous(),
+         bool(interleaved), False)
     torch.autograd.graph.increment_version((q, k))
     return q, k
 
