@@ -130,7 +130,7 @@ int vector_bytes(const Plan& p, int64_t L, int64_t cg, int64_t es, bool backward
 // Waves of whole units, each of kWaveBytes of input if units are that small.
 cudaError_t launch_waves(const NormArgs& a, const Plan& p, int64_t B, int dtype, int vb, int act,
                          bool backward, cudaStream_t st) {
-  NormWave w{0, 0, 0, 0, (int)envi("X_ORDER", 1)};
+  NormWave w{0, 0, 0, 0, 1};
   const int64_t es = elem_bytes(dtype) * (backward ? 2 : 1);
   int64_t in_wave = 0;
   auto flush = [&]() {
