@@ -152,17 +152,6 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def launch(fn, device_index: int, *args) -> None:
-    """fn(*args, stream): a C entry on the device's current stream, with that device current."""
-    if torch.cuda.current_device() == device_index:
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(device_index))
-    else:
-        with torch.cuda.device(device_index):
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(device_index))
-    if code != _lib.SUCCESS:
-        check_status(code)
-
-
 def _common_args(value, shapes, on_dev, loc, attn):
     B, K, H, C = value.shape
     _, Q, _, L, P, _ = loc.shape

@@ -9,11 +9,13 @@ selects another build of the same ABI (e.g. the bounds-checked one).
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
 LIB_PATH = os.environ.get("MSDA_B200_LIB") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), "_lib", "libmsda_b200.so")
+BINDING_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_binding.so")
 
 # Status codes (msda_status in include/msda_b200.h).
 SUCCESS = 0
@@ -65,8 +67,21 @@ EXPORTED_SYMBOLS = (
     "msda_abi_version",
 )
 
+# Functions that binding.cpp calls, in the order of its table.
+BINDING_SYMBOLS = (
+    "msda_status_string",
+    "msda_last_error",
+    "msda_group_norm_workspace_bytes",
+    "msda_group_norm_fwd",
+    "msda_group_norm_bwd",
+    "msda_rotary",
+    "msda_adamw_step",
+    "msda_adamw_values",
+)
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_binding = None
 
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
@@ -213,6 +228,31 @@ def lib() -> ctypes.CDLL:
                 )
             _lib = handle
     return _lib
+
+
+def binding():
+    """Load (once) and return the torch side of the operators in csrc/binding.cpp, which calls
+    the functions of lib()."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    handle = lib()
+    with _lock:
+        if _binding is None:
+            if not os.path.exists(BINDING_PATH):
+                raise RuntimeError(
+                    f"msda_triton_b200: binding not found at {BINDING_PATH}; build it with "
+                    "`python -m msda_triton_b200.build` (there is no CPU fallback)"
+                )
+            import torch  # noqa: F401  (its libraries are the binding's)
+
+            spec = importlib.util.spec_from_file_location("_binding", BINDING_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            module.bind([ctypes.cast(getattr(handle, name), _vp).value
+                         for name in BINDING_SYMBOLS])
+            _binding = module
+    return _binding
 
 
 def last_error() -> str:

@@ -6,7 +6,9 @@
 Every .cu file in csrc/ is compiled by nvcc in parallel with
 `-gencode arch=compute_100a,code=sm_100a` and linked into
 msda_triton_b200/_lib/libmsda_b200.so (statically linked CUDA runtime, so
-the library depends on nothing but the driver).
+the library depends on nothing but the driver).  csrc/binding.cpp, the torch
+side of some operators, is compiled against the installed torch into
+msda_triton_b200/_lib/_binding.so.
 
     python -m msda_triton_b200.build --checked
 
@@ -24,6 +26,7 @@ import glob
 import os
 import shutil
 import subprocess
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -32,6 +35,8 @@ INCLUDE = os.path.join(ROOT, "include")
 OBJ_DIR = os.path.join(PKG, "_build")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(LIB_DIR, "libmsda_b200.so")
+BINDING_SRC = os.path.join(CSRC, "binding.cpp")
+BINDING = os.path.join(LIB_DIR, "_binding.so")
 CHECKED_OBJ_DIR = os.path.join(PKG, "_build_checked")
 CHECKED_LIB = os.path.join(PKG, "_lib_checked", "libmsda_b200.so")
 
@@ -49,7 +54,7 @@ def _nvcc() -> str:
 
 
 def _deps_mtime() -> float:
-    files = glob.glob(os.path.join(CSRC, "*")) + glob.glob(os.path.join(INCLUDE, "*.h"))
+    files = glob.glob(os.path.join(CSRC, "*.cu*")) + glob.glob(os.path.join(INCLUDE, "*.h"))
     return max(os.path.getmtime(f) for f in files)
 
 
@@ -62,9 +67,37 @@ def _compile(src: str, extra: list[str], obj_dir: str) -> str:
     return obj
 
 
+def build_binding(force: bool = False) -> str:
+    """Compile csrc/binding.cpp against the installed torch; returns the module's path."""
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(
+            os.path.getmtime(f) for f in [BINDING_SRC, *glob.glob(os.path.join(INCLUDE, "*.h"))]):
+        return BINDING
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc())) or "/usr/local/cuda"
+    dirs = [os.path.join(root, "include"),
+            os.path.join(root, "include", "torch", "csrc", "api", "include"),
+            os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    os.makedirs(LIB_DIR, exist_ok=True)
+    tmp = BINDING + ".tmp"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[a for d in dirs for a in ("-isystem", d)], BINDING_SRC, "-o", tmp,
+           "-L" + os.path.join(root, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
+           "-lc10_cuda", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {BINDING_SRC}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(force: bool = False, verbose_ptxas: bool = False, checked: bool = False) -> str:
     """Compile every CUDA source and link the shared library; returns its path.
     checked=True builds the bounds-checked variant (-DMSDA_CHECKED)."""
+    if not checked:
+        build_binding(force)
     lib_path = CHECKED_LIB if checked else LIB
     obj_dir = CHECKED_OBJ_DIR if checked else OBJ_DIR
     if not force and os.path.exists(lib_path) and os.path.getmtime(lib_path) >= _deps_mtime():

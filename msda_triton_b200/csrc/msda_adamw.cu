@@ -5,8 +5,11 @@
 //   p  = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // in fp32, the parameter rounded once to its type (from an fp32 master copy,
-// if there is one).  Bound by memory: 28 bytes a parameter in fp32, 10 with
-// bf16 parameters and 8-bit moments.
+// if there is one).  With fp32 moments it is bound by memory: 28 bytes a
+// parameter in fp32 (22 in bf16), 335 M of them in 1.35 ms (1.07 ms), 6.9 TB/s.
+// With 8-bit moments and bf16 parameters, 10 bytes a parameter, the coding is:
+// about 75 instructions a parameter, 0.90 ms for 335 M (3.8 TB/s; fp32
+// parameters 0.98 ms, 5.5 TB/s).
 //
 // States of all tensors lie in one array each; tensor i's elements start at
 // the sum of the earlier tensors' sizes, each rounded up to kBlock.
@@ -17,7 +20,8 @@
 // second moment takes 5 exponent bits (top = 31, a range of 2^31), the first
 // its sign and 4 (top = 15).  E is the largest magnitude's exponent after it
 // is rounded up by one code more than it can be, so the highest code is never
-// reached by rounding; it stands for a value that is not finite.
+// reached by rounding; it stands for a value that is not finite, in a block
+// whose exponent byte is 255 for that (and counts as 254).
 //
 // Moments are rounded at random, up with the probability of the part cut off:
 // a change of 0.1 % a step (b2 = 0.999) is far below the spacing of 12.5 %, and
@@ -52,19 +56,25 @@ struct AdamTensor {
   void* p;
   const void* g;
   int64_t n;
-  int64_t offset;  // of its states
   float step_size, inv_sqrt_bc2;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
   uint32_t key;
-  uint32_t chunk0;  // first CTA of the launch
+  uint32_t offset;  // of its states, in blocks
+  uint32_t cta0;    // first CTA of the launch
+  uint32_t ctas;
 };
 
 struct AdamArgs {
-  float b1, c1, b2, c2, eps, decay;  // c = 1 - b, decay = 1 - lr wd
+  // m = k m + c (g - l m): with l = k = 1 (b >= 1/2), only c's share of the
+  // rounding of c and of the difference reaches m; with a small b that share is
+  // most of m, and l = 0, k = b
+  float c1, k1, l1, c2, k2, l2;  // c = 1 - b; l negated
+  float eps, decay;              // decay = 1 - lr wd
   const float* grad_scale;
   void *m, *v;
   uint8_t *me, *ve;
   float* master;
   int32_t tensors;
+  int32_t rounds;  // of kChunk elements per CTA
 };
 
 template <int N> struct AdamTable {
@@ -73,24 +83,63 @@ template <int N> struct AdamTable {
 };
 
 constexpr uint32_t kMaxFinite = 0x7f7fffffu;
+constexpr uint32_t kOdd = 255u;  // exponent byte of a block with something not finite
 
-// Byte i of a word of codes as a value; `shift` is 8 (E - top) << 20.
+// Byte i of a word of codes as a value; `shift` is 8 (E - top).
 template <bool SIGNED>
 __device__ __forceinline__ float adam_decode(uint32_t word, int i, uint32_t shift) {
-  constexpr uint32_t kTopCode = (SIGNED ? 127u : 255u) << 20;
+  constexpr uint32_t kCode = (SIGNED ? 127u : 255u) << 20;
   const int up = 20 - 8 * i;
-  const uint32_t size = (up >= 0 ? word << up : word >> -up) & kTopCode;
-  uint32_t bits = size == 0u ? 0u : size + shift;
-  if (size == kTopCode) bits = 0x7fc00000u;
+  const uint32_t size = (up >= 0 ? word << up : word >> -up) & kCode;
+  uint32_t bits = min(size, 1u << 20) * shift + size;  // zero stays zero
   if (SIGNED) bits |= word << (24 - 8 * i) & 0x80000000u;
   return __uint_as_float(bits);
 }
-__device__ __forceinline__ uint32_t adam_shift(uint32_t e, uint32_t top) { return (e - top) << 23; }
+__device__ __forceinline__ uint32_t adam_shift(uint32_t e, uint32_t top) {
+  return (min(e, kOdd - 1u) - top) << 3;
+}
+// The highest code of a block with E = kOdd: not finite.
+template <bool SIGNED>
+__device__ __forceinline__ void adam_decode_odd(uint32_t word, float* f) {
+  constexpr uint32_t kTopCode = SIGNED ? 127u : 255u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if ((word >> (8 * i) & kTopCode) == kTopCode) f[i] = __uint_as_float(0x7fc00000u);
+}
+
+// Four values as codes where some are not finite, or at the end of the range.
+template <uint32_t TOP, bool SIGNED>
+__device__ __noinline__ uint32_t adam_encode_odd(float4 x, uint4 r, uint32_t& e) {
+  constexpr uint32_t kTopCode = SIGNED ? 127u : 255u;
+  const float f[4] = {x.x, x.y, x.z, x.w};
+  const uint32_t rnd[4] = {r.x, r.y, r.z, r.w};
+  uint32_t most = 0u;
+  bool lost = false;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = __float_as_uint(f[i]) & 0x7fffffffu;
+    if (b <= kMaxFinite) most = max(most, b);
+    else lost = true;
+  }
+  most = __reduce_max_sync(~0u, most);
+  lost = __any_sync(~0u, lost);
+  e = min(max((most + 0x1fffffu) >> 23, TOP), kOdd - 1u);
+  const int base = static_cast<int>(e - TOP) << 3;
+  uint32_t word = 0u;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = __float_as_uint(f[i]) & 0x7fffffffu;
+    int c = static_cast<int>(min(b + rnd[i], kMaxFinite) >> 20) - base;
+    c = min(max(c, !SIGNED && b != 0u ? 1 : 0), static_cast<int>(kTopCode) - 1);
+    if (b > kMaxFinite) c = kTopCode;
+    if (SIGNED) c |= __float_as_uint(f[i]) >> 24 & 128u;
+    word |= static_cast<uint32_t>(c) << (8 * i);
+  }
+  if (lost) e = kOdd;
+  return word;
+}
 
 // The codes of four values per lane; `r` holds 20 random bits each.
 template <uint32_t TOP, bool SIGNED>
 __device__ __forceinline__ uint32_t adam_encode(const float* x, const uint32_t* r, uint32_t& e) {
-  constexpr uint32_t kTopCode = SIGNED ? 127u : 255u;
   uint32_t b[4], most = 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -99,25 +148,22 @@ __device__ __forceinline__ uint32_t adam_encode(const float* x, const uint32_t* 
     most = max(most, b[i]);
   }
   most = __reduce_max_sync(~0u, most);
-  const bool odd = most > kMaxFinite - 0xfffffu;  // something is not finite, or rounds to it
-  if (odd) {
-    most = 0u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (b[i] <= kMaxFinite) most = max(most, b[i]);
-    most = __reduce_max_sync(~0u, most);
-  }
+  if (most > kMaxFinite - 0x1fffffu)
+    return adam_encode_odd<TOP, SIGNED>(make_float4(x[0], x[1], x[2], x[3]),
+                                        make_uint4(r[0], r[1], r[2], r[3]), e);
   e = max((most + 0x1fffffu) >> 23, TOP);
   const int base = static_cast<int>(e - TOP) << 3;
   uint32_t word = 0u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t c = b[i] + r[i];
-    if (odd) c = min(c, kMaxFinite);
-    c = static_cast<uint32_t>(max(static_cast<int>(c >> 20) - base, SIGNED ? 0 : min(static_cast<int>(b[i]), 1)));
-    if (odd && b[i] > kMaxFinite) c = kTopCode;
-    if (SIGNED) c |= __float_as_uint(x[i]) >> 24 & 128u;
-    word |= c << (8 * i);
+  for (int i = 3; i >= 0; --i) {
+    int c = static_cast<int>((b[i] + r[i]) >> 20) - base;
+    c = max(c, SIGNED ? 0 : min(static_cast<int>(b[i]), 1));
+    word = word * 256u + c;
+  }
+  if (SIGNED) {  // the top bytes side by side
+    const uint32_t s01 = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x73);
+    const uint32_t s23 = __byte_perm(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x73);
+    word |= __byte_perm(s01, s23, 0x5410) & 0x80808080u;
   }
   return word;
 }
@@ -160,10 +206,39 @@ __device__ __forceinline__ void adam_store(T* p, int valid, bool vec, const floa
   }
 }
 
+// The root of at least the smallest normal number (below it the unit's result
+// would be zero), and a NaN's.
 __device__ __forceinline__ float adam_sqrt(float x) {
   float y;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("{\n .reg .f32 t;\n max.NaN.f32 t, %1, 0f00800000;\n sqrt.approx.ftz.f32 %0, t;\n}"
+      : "=f"(y) : "f"(x));
   return y;
+}
+// x is no less than such a root times a factor above 1/2: never subnormal.
+__device__ __forceinline__ float adam_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 template <typename T, bool SMALL, bool MASTER, int N>
@@ -174,101 +249,122 @@ adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
   int lo = 0, hi = a.tensors;  // the last tensor whose first CTA is not after this one
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (tab.t[mid].chunk0 <= blockIdx.x) lo = mid;
+    if (tab.t[mid].cta0 <= blockIdx.x) lo = mid;
     else hi = mid;
   }
   const AdamTensor& t = tab.t[lo];
   const int lane = threadIdx.x & 31;
-  const int64_t first = static_cast<int64_t>(blockIdx.x - t.chunk0) * kChunk +
-                        (threadIdx.x >> 5) * (kBlock * U) + lane * 4;
-  // elements from this lane's first one to the tensor's end
-  const int left = static_cast<int>(max(min(t.n - first, static_cast<int64_t>(kChunk)),
-                                        -static_cast<int64_t>(kChunk)));
-  T* p = static_cast<T*>(t.p) + first;
-  const T* g = static_cast<const T*>(t.g) + first;
-  const bool vec = (reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) %
-                       (4 * sizeof(T)) == 0;
-  const int64_t s0 = t.offset + first;
-  float* const master = a.master + s0;
-  uint8_t *const m8 = static_cast<uint8_t*>(a.m) + s0, *const v8 = static_cast<uint8_t*>(a.v) + s0;
-  uint8_t *const me = a.me + s0 / kBlock, *const ve = a.ve + s0 / kBlock;
-  float *const m32 = static_cast<float*>(a.m) + s0, *const v32 = static_cast<float*>(a.v) + s0;
   const float scale = a.grad_scale == nullptr ? 1.f : __ldg(a.grad_scale);
+  const uint64_t gs = pair(scale, scale), c1 = pair(a.c1, a.c1), k1 = pair(a.k1, a.k1),
+                 l1 = pair(a.l1, a.l1), c2 = pair(a.c2, a.c2), k2 = pair(a.k2, a.k2),
+                 l2 = pair(a.l2, a.l2), bc = pair(t.inv_sqrt_bc2, t.inv_sqrt_bc2),
+                 eps = pair(a.eps, a.eps), decay = pair(a.decay, a.decay),
+                 size = pair(-t.step_size, -t.step_size);
+  const bool vec = (reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g)) %
+                       (4 * sizeof(T)) == 0;
 
-  // everything is on its way before the first use
-  Raw<4 * sizeof(T)> rg[U], rp[U];
-  Raw<16> rx[U], rm[U], rv[U];
-  uint32_t cm[U], cv[U], em[U], ev[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int valid = left - u * kBlock;
-    if (valid + lane * 4 <= 0) continue;  // the whole warp: a block that is not there
-    rg[u] = adam_load(g + u * kBlock, min(valid, 4), vec);
-    if (MASTER) rx[u] = adam_load(master + u * kBlock, 4, true);
-    else rp[u] = adam_load(p + u * kBlock, min(valid, 4), vec);
-    if (SMALL) {
-      cm[u] = *reinterpret_cast<const uint32_t*>(m8 + u * kBlock);
-      cv[u] = *reinterpret_cast<const uint32_t*>(v8 + u * kBlock);
-      em[u] = me[u];
-      ev[u] = ve[u];
-    } else {
-      rm[u] = adam_load(m32 + u * kBlock, 4, true);
-      rv[u] = adam_load(v32 + u * kBlock, 4, true);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int valid = left - u * kBlock;
-    if (valid + lane * 4 <= 0) break;
-    float x[4], d[4], m[4], v[4];
-    Chunk<T, 4 * sizeof(T)>::unpack(rg[u], d);
-    if (MASTER) Chunk<float, 16>::unpack(rx[u], x);
-    else Chunk<T, 4 * sizeof(T)>::unpack(rp[u], x);
-    if (SMALL) {
-      const uint32_t sm = adam_shift(em[u], 15u), sv = adam_shift(ev[u], 31u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        m[i] = adam_decode<true>(cm[u], i, sm);
-        v[i] = adam_decode<false>(cv[u], i, sv);
+  // rounds of neighbouring CTAs lie side by side: with a CTA's own rounds next
+  // to one another, all CTAs at once touch every other 4 KB of the codes, and
+  // half of the memory channels (1726 us)
+  for (int round = 0; round < a.rounds; ++round) {
+    const int64_t first =
+        static_cast<int64_t>(blockIdx.x - t.cta0 + round * t.ctas) * kChunk +
+        (threadIdx.x >> 5) * (kBlock * U) + lane * 4;
+    // elements from this lane's first one to the tensor's end
+    const int left = static_cast<int>(max(min(t.n - first, static_cast<int64_t>(kChunk)),
+                                          -static_cast<int64_t>(kChunk)));
+    if (left + lane * 4 <= 0) return;  // the whole warp
+    T* p = static_cast<T*>(t.p) + first;
+    const T* g = static_cast<const T*>(t.g) + first;
+    const int64_t s0 = static_cast<int64_t>(t.offset) * kBlock + first;
+    float* const master = a.master + s0;
+    uint8_t *const m8 = static_cast<uint8_t*>(a.m) + s0, *const v8 = static_cast<uint8_t*>(a.v) + s0;
+    uint8_t *const me = a.me + s0 / kBlock, *const ve = a.ve + s0 / kBlock;
+    float *const m32 = static_cast<float*>(a.m) + s0, *const v32 = static_cast<float*>(a.v) + s0;
+
+    // everything is on its way before the first use
+    Raw<4 * sizeof(T)> rg[U], rp[U];
+    Raw<16> rx[U], rm[U], rv[U];
+    uint32_t cm[U], cv[U], em[U], ev[U];
+  #pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int valid = left - u * kBlock;
+      if (valid + lane * 4 <= 0) continue;  // the whole warp: a block that is not there
+      rg[u] = adam_load(g + u * kBlock, min(valid, 4), vec);
+      if (MASTER) rx[u] = adam_load(master + u * kBlock, 4, true);
+      else rp[u] = adam_load(p + u * kBlock, min(valid, 4), vec);
+      if (SMALL) {
+        cm[u] = *reinterpret_cast<const uint32_t*>(m8 + u * kBlock);
+        cv[u] = *reinterpret_cast<const uint32_t*>(v8 + u * kBlock);
+        em[u] = me[u];
+        ev[u] = ve[u];
+      } else {
+        rm[u] = adam_load(m32 + u * kBlock, 4, true);
+        rv[u] = adam_load(v32 + u * kBlock, 4, true);
       }
-    } else {
-      Chunk<float, 16>::unpack(rm[u], m);
-      Chunk<float, 16>::unpack(rv[u], v);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float e = d[i] * scale;
-      m[i] = a.b1 * m[i] + a.c1 * e;
-      v[i] = a.b2 * v[i] + a.c2 * e * e;
-      x[i] = a.decay * x[i] -
-             t.step_size * __fdividef(m[i], adam_sqrt(v[i]) * t.inv_sqrt_bc2 + a.eps);
-    }
-    if (valid < 4) {  // between tensors
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i >= valid) m[i] = v[i] = x[i] = 0.f;
-    }
-    adam_store(p + u * kBlock, min(valid, 4), vec, x);
-    if (MASTER) adam_store(master + u * kBlock, 4, true, x);
-    if (SMALL) {
-      uint32_t qm[4], qv[4], nm, nv;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t r = adam_random(static_cast<uint32_t>(s0) + u * kBlock + i, t.key);
-        qm[i] = (r << 4 & 0xffff0u) | 8u;
-        qv[i] = (r >> 12 & 0xffff0u) | 8u;
+  #pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int valid = left - u * kBlock;
+      if (valid + lane * 4 <= 0) return;
+      float x[4], d[4], m[4], v[4];
+      Chunk<T, 4 * sizeof(T)>::unpack(rg[u], d);
+      if (MASTER) Chunk<float, 16>::unpack(rx[u], x);
+      else Chunk<T, 4 * sizeof(T)>::unpack(rp[u], x);
+      if (SMALL) {
+        const uint32_t sm = adam_shift(em[u], 15u), sv = adam_shift(ev[u], 31u);
+  #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          m[i] = adam_decode<true>(cm[u], i, sm);
+          v[i] = adam_decode<false>(cv[u], i, sv);
+        }
+        if (em[u] == kOdd) adam_decode_odd<true>(cm[u], m);
+        if (ev[u] == kOdd) adam_decode_odd<false>(cv[u], v);
+      } else {
+        Chunk<float, 16>::unpack(rm[u], m);
+        Chunk<float, 16>::unpack(rv[u], v);
       }
-      const uint32_t wm = adam_encode<15u, true>(m, qm, nm);
-      const uint32_t wv = adam_encode<31u, false>(v, qv, nv);
-      *reinterpret_cast<uint32_t*>(m8 + u * kBlock) = wm;
-      *reinterpret_cast<uint32_t*>(v8 + u * kBlock) = wv;
-      if (lane == 0) {
-        me[u] = static_cast<uint8_t>(nm);
-        ve[u] = static_cast<uint8_t>(nv);
+  #pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        uint64_t e = mul2(pair(d[i], d[i + 1]), gs);
+        uint64_t mm = pair(m[i], m[i + 1]), vv = pair(v[i], v[i + 1]);
+        mm = fma2(c1, fma2(l1, mm, e), mul2(k1, mm));
+        e = mul2(e, e);
+        vv = fma2(c2, fma2(l2, vv, e), mul2(k2, vv));
+        unpair(mm, m[i], m[i + 1]);
+        unpair(vv, v[i], v[i + 1]);
+        float den[2];
+        unpair(fma2(pair(adam_sqrt(v[i]), adam_sqrt(v[i + 1])), bc, eps), den[0], den[1]);
+        const uint64_t q = mul2(mm, pair(adam_rcp(den[0]), adam_rcp(den[1])));
+        unpair(fma2(size, q, mul2(decay, pair(x[i], x[i + 1]))), x[i], x[i + 1]);
       }
-    } else {
-      adam_store(m32 + u * kBlock, 4, true, m);
-      adam_store(v32 + u * kBlock, 4, true, v);
+      if (valid < 4) {  // between tensors
+  #pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i >= valid) m[i] = v[i] = x[i] = 0.f;
+      }
+      adam_store(p + u * kBlock, min(valid, 4), vec, x);
+      if (MASTER) adam_store(master + u * kBlock, 4, true, x);
+      if (SMALL) {
+        uint32_t qm[4], qv[4], nm, nv;
+  #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t r = adam_random(static_cast<uint32_t>(s0) + u * kBlock + i, t.key);
+          qm[i] = (r << 4 & 0xffff0u) | 8u;
+          qv[i] = (r >> 12 & 0xffff0u) | 8u;
+        }
+        const uint32_t wm = adam_encode<15u, true>(m, qm, nm);
+        const uint32_t wv = adam_encode<31u, false>(v, qv, nv);
+        *reinterpret_cast<uint32_t*>(m8 + u * kBlock) = wm;
+        *reinterpret_cast<uint32_t*>(v8 + u * kBlock) = wv;
+        if (lane == 0) {
+          me[u] = static_cast<uint8_t>(nm);
+          ve[u] = static_cast<uint8_t>(nv);
+        }
+      } else {
+        adam_store(m32 + u * kBlock, 4, true, m);
+        adam_store(v32 + u * kBlock, 4, true, v);
+      }
     }
   }
 }
@@ -288,6 +384,14 @@ adamw_values_kernel(const uint8_t* m, const uint8_t* me, const uint8_t* v, const
   for (int k = 0; k < 8; ++k) {
     fm[k] = adam_decode<true>(k < 4 ? cm.x : cm.y, k & 3, sm);
     fv[k] = adam_decode<false>(k < 4 ? cv.x : cv.y, k & 3, sv);
+  }
+  if (em == kOdd) {
+    adam_decode_odd<true>(cm.x, fm);
+    adam_decode_odd<true>(cm.y, fm + 4);
+  }
+  if (ev == kOdd) {
+    adam_decode_odd<false>(cv.x, fv);
+    adam_decode_odd<false>(cv.y, fv + 4);
   }
   st_chunk<16>(mo + i, Chunk<__nv_bfloat16, 16>::pack(fm));
   st_chunk<16>(vo + i, Chunk<__nv_bfloat16, 16>::pack(fv));
@@ -321,6 +425,7 @@ struct Step {
 template <int N> cudaError_t adamw_all(const Step& s, const AdamArgs& args, cudaStream_t st) {
   AdamTable<N> tab;
   tab.a = args;
+  const int64_t per_cta = static_cast<int64_t>(kChunk) * args.rounds;
   int used = 0;
   int64_t chunks = 0, offset = 0, known = -1;
   float step_size = 0.f, inv_sqrt_bc2 = 0.f;
@@ -344,14 +449,15 @@ template <int N> cudaError_t adamw_all(const Step& s, const AdamArgs& args, cuda
       step_size = static_cast<float>(s.lr / (1.0 - std::pow(s.b1, t)));
       inv_sqrt_bc2 = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(s.b2, t)));
     }
-    const int64_t own = (n + kChunk - 1) / kChunk;
+    const int64_t own = (n + per_cta - 1) / per_cta;
     if (used == N || chunks + own > 0x7fffffff) {
       const cudaError_t err = flush();
       if (err != cudaSuccess) return err;
     }
-    tab.t[used++] = AdamTensor{s.params[i], s.grads[i], n, at, step_size, inv_sqrt_bc2,
+    tab.t[used++] = AdamTensor{s.params[i], s.grads[i], n, step_size, inv_sqrt_bc2,
                                s.seed + static_cast<uint32_t>(known) * 0x632be5abu,
-                               static_cast<uint32_t>(chunks)};
+                               static_cast<uint32_t>(at / kBlock), static_cast<uint32_t>(chunks),
+                               static_cast<uint32_t>(own)};
     chunks += own;
   }
   return flush();
@@ -403,10 +509,12 @@ int msda_adamw_step(int dtype, int state_bits, int64_t num_tensors, void* const*
       (small && (exp_avg_exponent == nullptr || exp_avg_sq_exponent == nullptr)))
     return report(MSDA_ERROR_MISALIGNED, "NULL or unaligned state");
   AdamArgs a{};
-  a.b1 = static_cast<float>(beta1);
   a.c1 = static_cast<float>(1.0 - beta1);
-  a.b2 = static_cast<float>(beta2);
+  a.k1 = beta1 < 0.5 ? static_cast<float>(beta1) : 1.f;
+  a.l1 = beta1 < 0.5 ? 0.f : -1.f;
   a.c2 = static_cast<float>(1.0 - beta2);
+  a.k2 = beta2 < 0.5 ? static_cast<float>(beta2) : 1.f;
+  a.l2 = beta2 < 0.5 ? 0.f : -1.f;
   a.eps = static_cast<float>(eps);
   a.decay = static_cast<float>(1.0 - lr * weight_decay);
   a.grad_scale = grad_scale;
@@ -415,6 +523,11 @@ int msda_adamw_step(int dtype, int state_bits, int64_t num_tensors, void* const*
   a.me = exp_avg_exponent;
   a.ve = exp_avg_sq_exponent;
   a.master = master;
+  // Two rounds a CTA for 8-bit states, whose kernel is bound by instructions
+  // (finding the tensor costs seven an element in one round: 930 us against
+  // 895 for 335 M bf16 parameters), where each SM still gets many CTAs; one
+  // where memory is the bound (fp32 states: 1070 us against 1082).
+  a.rounds = small && total >= int64_t{148} * 64 * kChunk ? 2 : 1;
   const Step s{dtype, small, num_tensors, params, grads, counts, steps, lr, beta1, beta2, seed};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // a launch copies its parameters: the short table where it is enough

@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from msda_triton_b200 import _core
+from msda_triton_b200 import _core, _lib
 
 
 @torch.library.custom_op("msda_b200::msda_forward", mutates_args=())
@@ -149,12 +149,8 @@ def group_norm_forward(x: list[Tensor], maps: bool, spatial_shapes: Tensor | Non
                        num_groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
                        activation: str) -> tuple[Tensor, Tensor]:
     """(y, statistics) of pyramid_group_norm; x holds the levels (maps) or the flattened pyramid."""
-    from msda_triton_b200 import norm
-
-    maps, xs, rows = norm._check(x if maps else x[0], spatial_shapes, num_groups, weight, bias,
-                                 activation)
-    y, stats = norm.norm_forward(maps, xs, rows, num_groups, weight, bias, eps, activation)
-    return y, stats[:y.shape[0] * len(rows) * num_groups * 2]
+    return _lib.binding().pyramid_group_norm_forward(x, maps, spatial_shapes, num_groups, weight,
+                                                     bias, eps, activation)
 
 
 @group_norm_forward.register_fake
@@ -171,13 +167,9 @@ def group_norm_backward(grad_y: Tensor, stats: Tensor, x: list[Tensor], maps: bo
                         spatial_shapes: Tensor | None, num_groups: int, weight: Tensor | None,
                         bias: Tensor | None, activation: str) -> list[Tensor]:
     """Gradients of x, then of weight and bias where they are given."""
-    from msda_triton_b200 import norm
-
-    maps, xs, rows = norm._check(x if maps else x[0], spatial_shapes, num_groups, weight, bias,
-                                 activation)
-    gxs, gw, gb = norm.norm_backward(maps, xs, rows, num_groups, weight, bias, activation, stats,
-                                     grad_y)
-    return gxs + [g for g in (gw, gb) if g is not None]
+    grads = _lib.binding().pyramid_group_norm_backward(grad_y, stats, x, maps, spatial_shapes,
+                                                       num_groups, weight, bias, activation)
+    return [g for g in grads if g is not None]
 
 
 @group_norm_backward.register_fake
@@ -211,10 +203,7 @@ group_norm_forward.register_autograd(_group_norm_backward, setup_context=_group_
 def rotary_forward(xs: list[Tensor], positions: Tensor, inv_freq: Tensor, axis_index: Tensor,
                    interleaved: bool) -> list[Tensor]:
     """One or two tensors of heads turned by their positions (1 or B, Q, A)."""
-    from msda_triton_b200 import positions as rotary_ops
-
-    positions = rotary_ops._check(xs, positions, inv_freq, axis_index)
-    return rotary_ops.rotary_forward(positions, inv_freq, axis_index, interleaved, xs)
+    return _lib.binding().rotary_forward(xs, positions, inv_freq, axis_index, interleaved)
 
 
 @rotary_forward.register_fake
@@ -226,11 +215,8 @@ def _rotary_forward_fake(xs, positions, inv_freq, axis_index, interleaved):
 def rotary_backward(grads: list[Tensor], inputs: list[Tensor], positions: Tensor,
                     inv_freq: Tensor, axis_index: Tensor, interleaved: bool) -> list[Tensor]:
     """Gradients of the tensors and, where `inputs` are given, of the positions."""
-    from msda_triton_b200 import positions as rotary_ops
-
-    gxs, gpos = rotary_ops.rotary_backward(positions, inv_freq, axis_index, interleaved, grads,
-                                       inputs or None)
-    return gxs + ([] if gpos is None else [gpos])
+    return _lib.binding().rotary_backward(grads, inputs, positions, inv_freq, axis_index,
+                                          interleaved)
 
 
 @rotary_backward.register_fake

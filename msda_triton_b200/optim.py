@@ -10,9 +10,7 @@ CPU fallback.
 
 from __future__ import annotations
 
-from array import array
 from collections.abc import Sequence
-from operator import attrgetter, eq
 
 import torch
 from torch import Tensor
@@ -64,9 +62,6 @@ def _flat(t: Tensor, at: int, p: Tensor) -> Tensor:
     return t.as_strided(p.shape, p.stride(), at)
 
 
-_dtype_of, _shape_of = attrgetter("dtype"), attrgetter("shape")
-
-
 def _one_kind(params: Sequence[Tensor]) -> None:
     if not params:
         return
@@ -75,7 +70,7 @@ def _one_kind(params: Sequence[Tensor]) -> None:
         raise ValueError("AdamW requires CUDA tensors. Got CPU tensors instead.")
     if dtype not in _core._DTYPE_CODE:
         raise NotImplementedError(f"AdamW only supports fp32, fp16, and bf16. Got {dtype}.")
-    if len(set(map(_dtype_of, params))) > 1 or len(set(map(Tensor.get_device, params))) > 1:
+    if any(p.dtype != dtype or p.device != params[0].device for p in params):
         raise ValueError("the tensors of a step must share their dtype and device")
 
 
@@ -89,47 +84,9 @@ def _is_dense(p: Tensor) -> bool:
     return True
 
 
-def _laid_out(p: Tensor, g: Tensor) -> Tensor:
-    """g in p's memory order."""
-    if g.layout != torch.strided:
-        raise ValueError(f"gradients must be dense, got {g.layout}")
-    if g.shape != p.shape:
-        raise ValueError(f"gradient {tuple(g.shape)} for a tensor {tuple(p.shape)}")
-    if not _is_dense(p):
-        raise ValueError("a parameter's elements must fill one range of memory, got strides "
-                         f"{p.stride()} for {tuple(p.shape)}")
-    if all(a == b for a, b, n in zip(g.stride(), p.stride(), p.shape) if n > 1):
-        return g
-    return torch.empty_like(p).copy_(g)
-
-
+# Elements of a parameter for each element of a state.
 _SIZES = {"exp_avg": 1, "exp_avg_sq": 1, "exp_avg_exponent": BLOCK, "exp_avg_sq_exponent": BLOCK,
           "master": 1}
-
-
-def _state_tensors(state: dict[str, Tensor], dtype: torch.dtype, device) -> tuple[int, int]:
-    """(bits, elements) of a checked state."""
-    for name in ("exp_avg", "exp_avg_sq"):
-        if name not in state:
-            raise ValueError(f"the state has no {name!r}")
-    m = state["exp_avg"]
-    bits = {torch.float32: 32, torch.uint8: 8}.get(m.dtype)
-    if bits is None:
-        raise ValueError(f"states must be fp32 or uint8 codes, got {m.dtype}")
-    wanted = {"exp_avg", "exp_avg_sq"} | ({"exp_avg_exponent", "exp_avg_sq_exponent"}
-                                         if bits == 8 else set())
-    if dtype in (torch.float16, torch.bfloat16):
-        wanted |= {"master"} & state.keys()
-    if state.keys() != wanted:
-        raise ValueError(f"a state of {bits} bits holds {sorted(wanted)}, got {sorted(state)}")
-    n = m.numel()
-    for name, t in state.items():
-        dt = torch.float32 if name == "master" else m.dtype
-        if (t.dtype != dt or t.dim() != 1 or t.numel() * _SIZES[name] != n or t.device != device
-                or not t.is_contiguous()):
-            raise ValueError(f"state {name!r} must be dense {dt} of {n // _SIZES[name]} elements "
-                             f"on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return bits, n
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor | None],
@@ -157,74 +114,14 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor | None],
         NotImplementedError: dtype other than fp32/fp16/bf16.
         RuntimeError: under CUDA graph capture, where `step` would be frozen.
     """
-    n = len(params)
-    if len(grads) != n:
-        raise ValueError(f"{n} tensors and {len(grads)} gradients")
-    if n == 0:
-        return
-    _one_kind(params)
-    first = params[0]
-    dtype, device, index = first.dtype, first.device, first.get_device()
-    bits, elements = _state_tensors(state, dtype, device)
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("adamw_step cannot be captured in a CUDA graph: the step's bias "
-                           "corrections are computed on the host")
-    given, live = grads, params
-    if any(g is None for g in grads):
-        given = [g for g in grads if g is not None]
-        live = [p for p, g in zip(params, grads) if g is not None]
-        if not live:
-            return
-    if set(map(_dtype_of, given)) != {dtype} or set(map(Tensor.get_device, given)) != {index}:
-        raise ValueError(f"gradients must be {dtype} on {device}, as the tensors")
-    # the usual case, dense tensors of the same shape, is checked without a loop in Python
-    if not (all(map(Tensor.is_contiguous, params)) and all(map(Tensor.is_contiguous, given))
-            and all(map(eq, map(_shape_of, live), map(_shape_of, given)))):
-        given = [_laid_out(p, g) for p, g in zip(live, given)]
-    g_ptr = array("q", map(Tensor.data_ptr, given))
-    if live is not params:
-        rest = iter(g_ptr)
-        g_ptr = array("q", [0 if g is None else next(rest) for g in grads])
-    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1
-                                   or grad_scale.device != device):
-        raise ValueError(f"grad_scale must be one fp32 value on {device}")
-    if isinstance(step, int):
-        steps = array("q", [step]) * n
-    else:
-        steps = array("q", map(int, step))
-        if len(steps) != n:
-            raise ValueError(f"{n} tensors and {len(steps)} steps")
-    p_ptr = array("q", map(Tensor.data_ptr, params))
-    counts = array("q", map(Tensor.numel, params))
-    address = lambda a: a.buffer_info()[0]  # noqa: E731
-    ptr = lambda name: state[name].data_ptr() if name in state else None  # noqa: E731
-    _core.launch(
-        _lib.lib().msda_adamw_step, index,
-        _core._DTYPE_CODE[dtype], bits, n, address(p_ptr), address(g_ptr), address(counts),
-        address(steps), lr, betas[0], betas[1], eps, weight_decay, int(seed) & 0xFFFFFFFF,
-        None if grad_scale is None else grad_scale.data_ptr(), ptr("exp_avg"),
-        ptr("exp_avg_sq"), ptr("exp_avg_exponent"), ptr("exp_avg_sq_exponent"),
-        ptr("master"), elements)
-    torch.autograd.graph.increment_version(live)
-    torch.autograd.graph.increment_version(state.values())
+    _lib.binding().adamw_step(params, grads, state, step, lr, betas[0], betas[1], eps,
+                              weight_decay, seed & 0xFFFFFFFF, grad_scale)
 
 
 def adamw_state_values(state: dict[str, Tensor]) -> tuple[Tensor, Tensor]:
     """(exp_avg, exp_avg_sq) that a state stands for, flat as the state is.
     8-bit moments come as bf16, which holds them exactly; fp32 ones as they are."""
-    m, v = state["exp_avg"], state["exp_avg_sq"]
-    if not m.is_cuda:
-        raise ValueError("AdamW requires CUDA tensors. Got CPU tensors instead.")
-    bits, n = _state_tensors({k: t for k, t in state.items() if k != "master"}, torch.float32,
-                             m.device)
-    if bits == 32:
-        return m, v
-    out = [torch.empty(n, device=m.device, dtype=torch.bfloat16) for _ in range(2)]
-    _core.launch(_lib.lib().msda_adamw_values, m.get_device(),
-                 m.data_ptr(), state["exp_avg_exponent"].data_ptr(), v.data_ptr(),
-                 state["exp_avg_sq_exponent"].data_ptr(), n, out[0].data_ptr(),
-                 out[1].data_ptr())
-    return out[0], out[1]
+    return _lib.binding().adamw_values(state)
 
 
 class _Part:

@@ -12,17 +12,14 @@ fallback.
 
 from __future__ import annotations
 
-from array import array
 from collections.abc import Sequence
 
 import torch
 from torch import nn
 
-from msda_triton_b200 import _core, _lib
+from msda_triton_b200 import _lib
 
-_POSITION_CODE = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 MAX_AXES = 4
-MAX_PAIRS = 2048
 
 
 def axial_frequencies(rotated: int, num_axes: int, theta: float = 100.0,
@@ -68,150 +65,13 @@ def pyramid_positions(spatial_shapes, device=None) -> torch.Tensor:
     return torch.cat(levels)[None]
 
 
-def _check(xs, positions, inv_freq, axis_index):
-    """positions as (1 or B, Q, A)."""
-    first = xs[0]
-    if not first.is_cuda:
-        raise ValueError("rotary requires CUDA tensors. Got CPU tensors instead.")
-    dtype, device, shape = first.dtype, first.device, first.shape
-    if dtype not in _core._DTYPE_CODE:
-        raise NotImplementedError(f"rotary only supports fp32, fp16, and bf16. Got {dtype}.")
-    if len(shape) != 4:
-        raise ValueError(f"expected (B, Q, H, C), got {tuple(shape)}")
-    B, Q, _, C = shape
-    for x in xs[1:]:
-        other = x.shape
-        if (x.device != device or x.dtype != dtype or len(other) != 4 or other[0] != B
-                or other[1] != Q or other[3] != C):
-            raise ValueError("queries and keys must share their device, dtype, batch, tokens and "
-                             f"channels; got {tuple(other)} {x.dtype} beside {tuple(shape)} "
-                             f"{dtype}")
+def _traced(xs, positions, inv_freq, axis_index, interleaved):
+    """As one opaque op (msda_b200::rotary_forward) under torch.compile."""
+    from msda_triton_b200 import ops
+
     if positions.dim() == 2:
         positions = positions[None]
-    where = positions.shape
-    if len(where) != 3 or where[0] not in (1, B) or where[1] != Q:
-        raise ValueError(f"positions must be (Q, A) or (1 or B, Q, A) with B={B}, Q={Q}; "
-                         f"got {tuple(where)}")
-    if not 1 <= where[2] <= MAX_AXES:
-        raise ValueError(f"positions must have 1 to {MAX_AXES} axes, got {where[2]}")
-    if positions.dtype == torch.bool or positions.is_complex():
-        raise ValueError(f"positions must be numbers, got {positions.dtype}")
-    pairs = inv_freq.shape
-    if (len(pairs) != 1 or inv_freq.dtype != torch.float32 or axis_index.shape != pairs
-            or axis_index.dtype != torch.int32):
-        raise ValueError("inv_freq must be (pairs,) fp32 and axis_index (pairs,) int32, got "
-                         f"{tuple(pairs)} {inv_freq.dtype} and "
-                         f"{tuple(axis_index.shape)} {axis_index.dtype}")
-    if 2 * pairs[0] > C or pairs[0] > MAX_PAIRS:
-        raise ValueError(f"{pairs[0]} pairs do not fit {C} channels (and at most {MAX_PAIRS})")
-    if positions.device != device or inv_freq.device != device or axis_index.device != device:
-        raise ValueError(f"positions, inv_freq and axis_index must be on {device}, got "
-                         f"{positions.device}, {inv_freq.device} and {axis_index.device}")
-    return positions
-
-
-def _positions(positions):
-    """In a dtype and layout that the kernel reads."""
-    if positions.dtype not in _POSITION_CODE:
-        p = positions.detach()
-        positions = p.float() if p.dtype.is_floating_point else p.long()
-    return positions if positions.is_contiguous() else positions.detach().contiguous()
-
-
-def _dense_channels(x):
-    return x if x.stride(3) == 1 or x.shape[3] <= 1 else x.detach().contiguous()
-
-
-def _address(values) -> tuple[array, int]:
-    """A host table of 64-bit values (to be kept alive), and where it lies."""
-    table = array("q", values)
-    return table, table.buffer_info()[0]
-
-
-def _tables(ts):
-    """Host tables of the tensors' addresses and of their (batch, token, head) strides."""
-    strides = []
-    for t in ts:
-        strides += t.stride()[:3]
-    return _address([t.data_ptr() for t in ts]), _address(strides)
-
-
-def turn(xs, ys, positions, inv_freq, axis_index, interleaved, inverse, inputs=None, gpos=None):
-    """Launch on prepared tensors: ys are the xs turned (or turned back)."""
-    first = xs[0]
-    B, Q, _, C = first.shape
-    batch, _, axes = positions.shape
-    heads = _address([x.shape[2] for x in xs])
-    (px, sx), (py, sy) = _tables(xs), _tables(ys)
-    pi, si = _tables(inputs) if inputs is not None else ((None, None), (None, None))
-    _core.launch(
-        _lib.lib().msda_rotary, first.get_device(),
-        _core._DTYPE_CODE[first.dtype], B, Q, C, len(xs), heads[1], px[1], sx[1], py[1], sy[1],
-        positions.data_ptr(), _POSITION_CODE[positions.dtype], 0 if batch == 1 else Q * axes, axes,
-        inv_freq.data_ptr(), axis_index.data_ptr(), inv_freq.shape[0], interleaved, inverse,
-        pi[1], si[1], None if gpos is None else gpos.data_ptr())
-
-
-def _new(x):
-    return (torch.empty_like(x) if x.is_contiguous()
-            else torch.empty(x.shape, device=x.device, dtype=x.dtype))
-
-
-def rotary_forward(positions, inv_freq, axis_index, interleaved, xs):
-    ys = [_new(x) for x in xs]
-    turn([_dense_channels(x) for x in xs], ys, _positions(positions), inv_freq.contiguous(),
-         axis_index.contiguous(), interleaved, False)
-    return ys
-
-
-def rotary_backward(positions, inv_freq, axis_index, interleaved, grads, inputs=None):
-    """(gradients of the inputs, of the positions or None without `inputs`)."""
-    grads = [_dense_channels(g) for g in grads]
-    gxs, pos, gpos = [_new(g) for g in grads], _positions(positions), None
-    if inputs is not None:
-        B, Q = grads[0].shape[:2]
-        gpos = torch.empty((B, Q, pos.shape[2]), device=pos.device, dtype=torch.float32)
-        inputs = [_dense_channels(x) for x in inputs]
-    turn(grads, gxs, pos, inv_freq.contiguous(), axis_index.contiguous(), interleaved, True,
-         inputs, gpos)
-    if gpos is not None:
-        if pos.shape[0] != gpos.shape[0]:  # one set of positions for the whole batch
-            gpos = gpos.sum(0, keepdim=True)
-        gpos = gpos.to(positions.dtype)
-    return gxs, gpos
-
-
-class RotaryFn(torch.autograd.Function):
-    """Autograd Function of rotary / rotary_qk; gradients flow to the tensors and, where they
-    require one, to the positions."""
-
-    @staticmethod
-    def forward(ctx, positions, inv_freq, axis_index, interleaved, *xs):
-        ys = rotary_forward(positions, inv_freq, axis_index, interleaved, xs)
-        ctx.interleaved = interleaved
-        ctx.save_for_backward(positions, inv_freq, axis_index,
-                              *(xs if ctx.needs_input_grad[0] else ()))
-        return tuple(ys)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        positions, inv_freq, axis_index, *inputs = ctx.saved_tensors
-        gxs, gpos = rotary_backward(positions, inv_freq, axis_index, ctx.interleaved, grads,
-                                    inputs or None)
-        return (gpos, None, None, None, *gxs)
-
-
-def _apply(xs, positions, inv_freq, axis_index, interleaved):
-    if torch.compiler.is_compiling():
-        from msda_triton_b200 import ops
-
-        if positions.dim() == 2:
-            positions = positions[None]
-        return tuple(ops.rotary_forward(list(xs), positions, inv_freq, axis_index, interleaved))
-    positions = _check(xs, positions, inv_freq, axis_index)
-    if torch.is_grad_enabled() and (positions.requires_grad or any(x.requires_grad for x in xs)):
-        return RotaryFn.apply(positions, inv_freq, axis_index, bool(interleaved), *xs)
-    return tuple(rotary_forward(positions, inv_freq, axis_index, bool(interleaved), xs))
+    return tuple(ops.rotary_forward(list(xs), positions, inv_freq, axis_index, interleaved))
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -234,7 +94,9 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
         ValueError: CPU tensors, shapes that do not fit.
         NotImplementedError: dtype other than fp32/fp16/bf16.
     """
-    return _apply((x,), positions, inv_freq, axis_index, interleaved)[0]
+    if torch.compiler.is_compiling():
+        return _traced((x,), positions, inv_freq, axis_index, interleaved)[0]
+    return _lib.binding().rotary(x, positions, inv_freq, axis_index, interleaved)
 
 
 def rotary_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -242,25 +104,16 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
               ) -> tuple[torch.Tensor, torch.Tensor]:
     """rotary of queries and keys of the same tokens in one launch; they may
     differ in their number of heads."""
-    return _apply((q, k), positions, inv_freq, axis_index, interleaved)
+    if torch.compiler.is_compiling():
+        return _traced((q, k), positions, inv_freq, axis_index, interleaved)
+    return _lib.binding().rotary_qk(q, k, positions, inv_freq, axis_index, interleaved)
 
 
 def rotary_qk_(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                axis_index: torch.Tensor, interleaved: bool = False
                ) -> tuple[torch.Tensor, torch.Tensor]:
     """rotary_qk in place, for inference: q and k are overwritten and returned."""
-    positions = _check((q, k), positions, inv_freq, axis_index)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
-                                    or positions.requires_grad):
-        raise RuntimeError("rotary_qk_ has no gradient: use rotary_qk, or torch.no_grad()")
-    for x in (q, k):
-        if x.stride(3) != 1 and x.shape[3] > 1:
-            raise ValueError("rotary_qk_ needs dense channels")
-        if any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
-            raise ValueError("rotary_qk_ cannot write to an expanded tensor")
-    turn((q, k), (q, k), _positions(positions), inv_freq.contiguous(), axis_index.contiguous(),
-         bool(interleaved), False)
-    torch.autograd.graph.increment_version((q, k))
+    _lib.binding().rotary_in_place([q, k], positions, inv_freq, axis_index, interleaved)
     return q, k
 
 
@@ -298,5 +151,5 @@ class AxialRotary(nn.Module):
         return self
 
 
-__all__ = ["rotary", "rotary_qk", "rotary_qk_", "AxialRotary", "RotaryFn", "axial_frequencies",
+__all__ = ["rotary", "rotary_qk", "rotary_qk_", "AxialRotary", "axial_frequencies",
            "pyramid_positions"]
