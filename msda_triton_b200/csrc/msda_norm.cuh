@@ -11,19 +11,20 @@
 //   gx = r (dz w_c - a - h q),  a = sum_c w_c s1_c / n,  q = sum_c w_c s2_c / n
 //   gw_c = sum_b s2_c,  gd_c = sum_b s1_c.
 //
-// Work is cut into units: a segment, or a slab of whole groups of it, in tiles
-// of rows, a CTA each.  A statistics pass and an application pass run over
-// each unit; the CTA that finishes a unit's statistics last joins its tiles'
-// partial results, in tile order whichever CTA it is, so results do not
-// depend on the schedule.  Both passes are limited by memory (about 6 flops a
-// byte in 16 bits), so units go in waves that fit in L2, and one launch holds
-// the application of a wave and the statistics of the next: the application
-// reads the rows that the statistics brought in.
+// Work is cut into units, slabs of whole groups of a segment, and units into
+// tiles of rows, a CTA each.  A first launch takes the tiles' statistics, a
+// second applies them, from the last tile back: what the first read last is
+// then still in L2.
 //
-// Statistics are carried in fp32 as (count, mean, sum of squared deviations):
-// each thread takes the mean and deviations of a chunk of rows in registers,
-// and chunks, threads and tiles are joined pairwise (Chan, Golub, LeVeque), so
-// a mean far from zero costs no digits.
+// Tiles leave partial results.  Where a unit has few tiles, each CTA of the
+// second launch joins those of its groups itself ("direct"): that costs 1 us at
+// its start, and neither counters nor a wait.  Else the CTA that finishes a
+// group of kNormFan tiles last joins them, and the last of those groups the
+// unit's.  Both go in tile order whichever CTA is last, so results
+// do not depend on the schedule.  Statistics are carried in fp32 as (count,
+// mean, sum of squared deviations): each thread takes the mean and deviations
+// of a chunk of rows in registers, and chunks, threads and tiles are joined
+// pairwise (Chan, Golub, LeVeque), so a mean far from zero costs no digits.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -43,13 +44,12 @@ struct NormLevel {
   const char* gy;      // backward only
   int64_t x_batch, x_row, out_batch, out_row, gy_batch, gy_row;  // strides in elements
   int64_t rows;
-  int64_t block0;      // first tile of the level, counted over all levels
+  int32_t tile0;       // first tile of the level, counted over all levels
   int32_t done0;       // first of the level's counters: per unit one, and one per kNormFan tiles
   int32_t tiles;       // tiles per unit
   int32_t tile_rows;
   int32_t slabs;       // slabs per segment
   int32_t slab_groups; // groups per slab; the last may have fewer
-  int32_t run;         // slabs of a segment that go together, tile by tile
 };
 
 struct NormArgs {
@@ -63,34 +63,22 @@ struct NormArgs {
   float2* partial;     // per tile: per group of the slab (mean, sum of squared deviations);
                        // backward: per channel of the slab (s1, s2)
   int32_t partial_stride;
-  unsigned int* done;  // counters of partial results that are written
-  float2* chan;        // backward, (B, L, C): s1, s2
-  float2* coef;        // backward, (B, L, G): a, q
-};
-
-// Tiles [apply0, apply0 + applies) of one wave, [stats0, stats0 + stats) of the next.
-struct NormWave {
-  int64_t apply0, stats0;
-  int32_t applies, stats;
-  int32_t order;
-};
-
-struct NormParamGrad {
-  const float2* chan;
-  int32_t B, L, C;
-  int32_t per_level;
-  int32_t dtype;
-  void* gweight;  // (C) or (L, C), or nullptr
+  int32_t direct;
+  unsigned int* done;  // counters of partial results that are written (not direct)
+  float2* chan;        // backward, (B, L, C): s1, s2 (not direct)
+  float2* coef;        // backward, (B, L, G): a, q (not direct)
+  float2* weighted;    // backward, per tile and group of the slab: sum w s1, sum w s2 (direct)
+  int32_t tiles;
+  // gradients of the affine map, by the second launch's first CTAs
+  int32_t B, param_ctas;
+  void* gweight;       // as weight, or nullptr
   void* gbias;
 };
 
-cudaError_t norm_wave(const NormArgs& a, const NormWave& w, int dtype, int vb, int act,
-                      bool backward, cudaStream_t st);
-cudaError_t norm_param_grad(const NormParamGrad& p, cudaStream_t st);
+constexpr int kNormParamChannels = 8;  // of a CTA that sums gradients of the affine map
 
-// One instance per dtype (msda_norm_{f32,f16,bf16}.cu).
+// Both launches; one instance per dtype (msda_norm_{f32,f16,bf16}.cu).
 template <typename T>
-cudaError_t norm_wave_t(const NormArgs& a, const NormWave& w, int vb, int act, bool backward,
-                        cudaStream_t st);
+cudaError_t norm_launch(const NormArgs& a, int vb, int act, bool backward, cudaStream_t st);
 
 }  // namespace msda

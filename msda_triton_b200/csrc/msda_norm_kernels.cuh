@@ -1,41 +1,118 @@
-// msda_norm_kernels.cuh -- device code of msda_norm.cuh's passes.
+// msda_norm_kernels.cuh -- device code of msda_norm.cuh's items.
 #pragma once
 
 #include "msda_b200.h"
+#include "msda_f32x2.cuh"
 #include "msda_norm.cuh"
 
+// Loads that leave L1 alone, and stores that L2 lets go of first: the forward
+// reads each row twice from L2 or DRAM and never its output (647 -> 582 us for
+// the 1.23 GB of two 3D xl pyramids).  The backward is slower with such stores
+// (1130 -> 1210 us).
 namespace msda {
+
+template <int VB> __device__ __forceinline__ Raw<VB> norm_ld(const void* p) {
+  if constexpr (VB == 16) {
+    Raw<16> r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "l"(p));
+    return r;
+  } else {
+    return ld_chunk<VB>(p);
+  }
+}
+template <int VB> __device__ __forceinline__ void norm_st(void* p, const Raw<VB>& r) {
+  if constexpr (VB == 16)
+    __stcs(static_cast<uint4*>(p), make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]));
+  else
+    st_chunk<VB>(p, r);
+}
 
 template <int K> struct Count { static constexpr int value = K; };
 
-__device__ __forceinline__ float norm_param(const void* p, int dtype, int64_t i, float none) {
-  if (p == nullptr) return none;
-  if (dtype == MSDA_FLOAT32) return __ldg(static_cast<const float*>(p) + i);
-  if (dtype == MSDA_FLOAT16) return __half2float(__ldg(static_cast<const __half*>(p) + i));
-  return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + i));
+// EPV parameters from element i on.
+template <int EPV>
+__device__ __forceinline__ void norm_params(const void* p, int dtype, int64_t i, float none,
+                                            float* f) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int k = 0; k < EPV; ++k) f[k] = none;
+  } else if (dtype == MSDA_FLOAT32) {
+    const float* q = static_cast<const float*>(p) + i;
+    if (EPV % 4 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0) {
+#pragma unroll
+      for (int k = 0; k + 3 < EPV; k += 4) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(q + k));
+        f[k] = v.x; f[k + 1] = v.y; f[k + 2] = v.z; f[k + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < EPV; ++k) f[k] = __ldg(q + k);
+    }
+  } else if (dtype == MSDA_FLOAT16) {
+#pragma unroll
+    for (int k = 0; k < EPV; ++k) f[k] = __half2float(__ldg(static_cast<const __half*>(p) + i + k));
+  } else {
+#pragma unroll
+    for (int k = 0; k < EPV; ++k)
+      f[k] = __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + i + k));
+  }
 }
 
-// 1 / (1 + exp(-z)): 0 where the exponential overflows.
-__device__ __forceinline__ float norm_sigmoid(float z) {
-  return __fdividef(1.f, 1.f + __expf(-z));
+// A vector as pairs of fp32; one of a single element has a second one of 0.
+template <typename T, int VB> struct Pairs {
+  static constexpr int EPV = Chunk<T, VB>::EPV, N = (EPV + 1) / 2;
+  static __device__ __forceinline__ void unpack(const Raw<VB>& r, uint64_t* p) {
+    float f[2 * N];
+    f[2 * N - 1] = 0.f;
+    Chunk<T, VB>::unpack(r, f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = pair(f[2 * i], f[2 * i + 1]);
+  }
+  static __device__ __forceinline__ Raw<VB> pack(const uint64_t* p) {
+    float f[2 * N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) unpair(p[i], f[2 * i], f[2 * i + 1]);
+    return Chunk<T, VB>::pack(f);
+  }
+  static __device__ __forceinline__ void of(const float* f, uint64_t* p) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = pair(f[2 * i], 2 * i + 1 < EPV ? f[2 * i + 1] : 0.f);
+  }
+};
+
+// 1 / (1 + exp(-z)); 0 where the exponential overflows.
+__device__ __forceinline__ uint64_t norm_sigmoid(uint64_t z) {
+  float a, b;
+  unpair(mul2(z, pair(-1.4426950409f, -1.4426950409f)), a, b);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+  unpair(add2(pair(a, b), pair(1.f, 1.f)), a, b);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+  return pair(a, b);
 }
+__device__ __forceinline__ float norm_cdf(float z) { return 0.5f * (1.f + erff(z * 0.70710678f)); }
 
 // act(z); dact: act'(z).  A NaN stays one.
-template <int ACT> __device__ __forceinline__ float norm_act(float z) {
-  if (ACT == MSDA_ACT_RELU) return z < 0.f ? 0.f : z;
-  if (ACT == MSDA_ACT_SILU) return z * norm_sigmoid(z);
-  if (ACT == MSDA_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
-  return z;
+template <int ACT> __device__ __forceinline__ uint64_t norm_act(uint64_t z) {
+  if (ACT == MSDA_ACT_NONE) return z;
+  if (ACT == MSDA_ACT_SILU) return mul2(z, norm_sigmoid(z));
+  float a, b;
+  unpair(z, a, b);
+  if (ACT == MSDA_ACT_RELU) return pair(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b);
+  return pair(a * norm_cdf(a), b * norm_cdf(b));
 }
-template <int ACT> __device__ __forceinline__ float norm_dact(float z) {
-  if (ACT == MSDA_ACT_RELU) return z <= 0.f ? 0.f : 1.f;
-  if (ACT == MSDA_ACT_SILU) {
-    const float s = norm_sigmoid(z);
-    return s * (1.f + z * (1.f - s));
+template <int ACT> __device__ __forceinline__ uint64_t norm_dact(uint64_t z) {
+  if (ACT == MSDA_ACT_SILU) {  // s (1 + z (1 - s))
+    const uint64_t s = norm_sigmoid(z), zs = mul2(z, s);
+    return fma2(s, fma2(zs, pair(-1.f, -1.f), z), s);
   }
-  if (ACT == MSDA_ACT_GELU)
-    return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
-  return 1.f;
+  float a, b;
+  unpair(z, a, b);
+  if (ACT == MSDA_ACT_RELU) return pair(a <= 0.f ? 0.f : 1.f, b <= 0.f ? 0.f : 1.f);
+  return pair(norm_cdf(a) + a * 0.39894228f * __expf(-0.5f * a * a),
+              norm_cdf(b) + b * 0.39894228f * __expf(-0.5f * b * b));
 }
 
 // (n, mean, m2) joined with another set's.
@@ -54,40 +131,62 @@ __device__ __forceinline__ void norm_join(float& n, float& mean, float& m2, floa
   n = nn;
 }
 
-// Where a tile lies, and which of its vectors a thread takes: column tc (then
-// tc + tcols, ... where one group is wider than the CTA), rows tr, tr + trows, ...
-template <int EPV> struct NormTile {
-  int l, counter, tile, step, groups, nvc, tcols, trows, tc, tr, rows, g0;  // step: blocks to the unit's next tile
-  int64_t b, row0;
-  __device__ __forceinline__ NormTile(const NormArgs& a, int64_t block) {
-    l = a.L - 1;
-    while (block < a.lv[l].block0) --l;
-    const NormLevel& v = a.lv[l];
-    const int64_t rel = block - v.block0;
-    const int64_t seg = static_cast<int64_t>(v.slabs) * v.tiles;
-    b = rel / seg;
-    int64_t r = rel - b * seg;
-    const int64_t together = static_cast<int64_t>(v.run) * v.tiles;
-    const int s0 = static_cast<int>(r / together) * v.run;
-    r -= static_cast<int64_t>(s0) * v.tiles;
-    const int width = min(v.run, v.slabs - s0);
-    tile = static_cast<int>(r / width);
-    const int slab = s0 + static_cast<int>(r - static_cast<int64_t>(tile) * width);
-    step = width;
-    counter = v.done0 + (static_cast<int>(b) * v.slabs + slab) * (1 + (v.tiles + kNormFan - 1) / kNormFan);
-    g0 = slab * v.slab_groups;
-    groups = min(v.slab_groups, a.G - g0);
-    row0 = static_cast<int64_t>(tile) * v.tile_rows;
-    rows = static_cast<int>(min(static_cast<int64_t>(v.tile_rows), v.rows - row0));
-    nvc = groups * a.cg / EPV;
-    tcols = min(nvc, kNormThreads);
-    trows = kNormThreads / tcols;
-    tr = threadIdx.x / tcols;
-    tc = threadIdx.x - tr * tcols;
-    if (tr >= trows) tr = rows;  // no rows
-  }
-  __device__ __forceinline__ int64_t segment(const NormArgs& a) const { return b * a.L + l; }
+// ------------------------------------------------------------------ tiles
+struct NormTile {
+  int l, b, counter;
+  int block, tile, step;  // step: blocks to the unit's next tile
+  int groups, g0, rows, nvc, tcols, trows;
+  int64_t row0;
 };
+
+// A segment's slabs go side by side, tile by tile: neighbouring CTAs read
+// neighbouring pieces of the same rows.
+template <int EPV>
+__host__ __device__ __forceinline__ NormTile norm_tile(const NormArgs& a, int block) {
+  NormTile t;
+  t.block = block;
+  t.l = a.L - 1;
+  while (block < a.lv[t.l].tile0) --t.l;
+  const NormLevel& v = a.lv[t.l];
+  const int rel = block - v.tile0, seg = v.slabs * v.tiles;
+  t.b = rel / seg;
+  const int r = rel - t.b * seg;
+  t.tile = r / v.slabs;
+  t.step = v.slabs;
+  const int slab = r - t.tile * v.slabs;
+  t.counter = v.done0 + (t.b * v.slabs + slab) * (1 + (v.tiles + kNormFan - 1) / kNormFan);
+  t.g0 = slab * v.slab_groups;
+  t.groups = min(v.slab_groups, a.G - t.g0);
+  t.row0 = static_cast<int64_t>(t.tile) * v.tile_rows;
+  t.rows = static_cast<int>(min(static_cast<int64_t>(v.tile_rows), v.rows - t.row0));
+  t.nvc = t.groups * a.cg / EPV;
+  t.tcols = min(t.nvc, kNormThreads);
+  t.trows = kNormThreads / t.tcols;
+  return t;
+}
+
+// A thread's vectors of a tile: column tc (then tc + tcols, ... where one
+// group is wider than the CTA), rows tr, tr + trows, ...
+struct NormThread {
+  int tc, tr;
+  int64_t segment, seg_group, seg_chan;
+  __device__ __forceinline__ NormThread(const NormArgs& a, const NormTile& t) {
+    tr = threadIdx.x / t.tcols;
+    tc = threadIdx.x - tr * t.tcols;
+    if (tr >= t.trows) tr = t.rows;  // no rows
+    segment = static_cast<int64_t>(t.b) * a.L + t.l;
+    seg_group = segment * a.G + t.g0;
+    seg_chan = segment * a.C + static_cast<int64_t>(t.g0) * a.cg;
+  }
+};
+
+// Calls chunk(Count<U>) while U rows are left, then chunk(Count<1>).
+template <int U, typename Chunk>
+__device__ __forceinline__ void norm_rows(const NormTile& t, int tr, Chunk chunk) {
+  int r = tr;
+  for (; r + (U - 1) * t.trows < t.rows; r += U * t.trows) chunk(Count<U>{});
+  for (; r < t.rows; r += t.trows) chunk(Count<1>{});
+}
 
 // Whether this CTA is the last of `count`: what the others wrote is then visible.
 __device__ __forceinline__ bool norm_last(unsigned int* done, int count) {
@@ -106,20 +205,19 @@ __device__ __forceinline__ bool norm_last(unsigned int* done, int count) {
 // `full` rows (the last of `tail`), into tile `slot`'s or, with `final`, into
 // the unit's.
 template <typename Join>
-__device__ __forceinline__ void norm_join_tiles(const NormArgs& a, const NormLevel& v, int counter,
-                                                int tile, Join join) {
-  const int group = tile / kNormFan, groups = (v.tiles + kNormFan - 1) / kNormFan;
+__device__ __forceinline__ void norm_join_tiles(const NormArgs& a, const NormTile& t, Join join) {
+  const NormLevel& v = a.lv[t.l];
+  const int group = t.tile / kNormFan, groups = (v.tiles + kNormFan - 1) / kNormFan;
   const int first = group * kNormFan, count = min(kNormFan, v.tiles - first);
   const int64_t full = v.tile_rows, last = v.rows - (v.tiles - 1) * full;
-  if (!norm_last(a.done + counter + 1 + group, count)) return;
+  if (!norm_last(a.done + t.counter + 1 + group, count)) return;
   join(first, 1, count, full, group + 1 < groups ? full : last, groups == 1);
   if (groups == 1) return;
-  if (!norm_last(a.done + counter, groups)) return;
+  if (!norm_last(a.done + t.counter, groups)) return;
   join(0, kNormFan, groups, full * kNormFan, v.rows - (groups - 1) * full * kNormFan, true);
 }
 
-// A launch may start before the one ahead of it has ended: its statistics need
-// nothing of that one, its applications wait for it.
+// The second launch may start before the first has ended, and waits for it.
 __device__ __forceinline__ void norm_let_next_start() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
@@ -127,72 +225,56 @@ __device__ __forceinline__ void norm_wait_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Whether this CTA applies, and its tile.
-__device__ __forceinline__ bool norm_applies(const NormWave& w, int64_t& block) {
-  const int i = blockIdx.x;
-  if (w.order == 0) {  // apply first
-    if (i < w.applies) { block = w.apply0 + i; return true; }
-    block = w.stats0 + (i - w.applies);
-    return false;
-  }
-  if (w.order == 1) {
-    if (i < w.stats) { block = w.stats0 + i; return false; }
-    block = w.apply0 + (i - w.stats);
-    return true;
-  }
-  const int both = min(w.applies, w.stats);
-  if (i < 2 * both) {
-    block = (i & 1) ? w.apply0 + (i >> 1) : w.stats0 + (i >> 1);
-    return i & 1;
-  }
-  if (w.applies > both) { block = w.apply0 + (i - both); return true; }
-  block = w.stats0 + (i - both);
-  return false;
-}
-
-template <typename T, int VB, int U>
-__device__ void norm_stats(const NormArgs& a, int64_t block) {
-  constexpr int EPV = Chunk<T, VB>::EPV;
+// ------------------------------------------------------------------ forward
+template <typename T, int VB, bool DIRECT, int U>
+__device__ void norm_stats(const NormArgs& a, const NormTile& t) {
+  using P = Pairs<T, VB>;
+  constexpr int EPV = P::EPV;
   __shared__ float3 part[kNormThreads];
-  const NormTile<EPV> t(a, block);
   const NormLevel& v = a.lv[t.l];
-  const T* x = reinterpret_cast<const T*>(v.x) + t.b * v.x_batch + t.row0 * v.x_row +
+  const NormThread me(a, t);
+  const T* x = reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row +
                static_cast<int64_t>(t.g0) * a.cg;
+  const int64_t hop = t.trows * v.x_row;
   float n = 0.f, mean = 0.f, m2 = 0.f;
-  for (int col = t.tc; col < t.nvc; col += t.tcols) {
-    const T* p = x + col * EPV + t.tr * v.x_row;
-    const int64_t hop = t.trows * v.x_row;
-    auto chunk = [&](auto count) {
+  for (int col = me.tc; col < t.nvc; col += t.tcols) {
+    const T* p = x + col * EPV;
+    norm_rows<U>(t, me.tr, [&](auto count) {
       constexpr int K = decltype(count)::value;
       Raw<VB> w[K];
 #pragma unroll
-      for (int u = 0; u < K; ++u) w[u] = ld_chunk<VB>(p + u * hop);
+      for (int u = 0; u < K; ++u) w[u] = norm_ld<VB>(p + u * hop);
       p += K * hop;
-      float s = 0.f, q = 0.f;
+      uint64_t s = 0, q = 0;  // two zeros
 #pragma unroll
       for (int u = 0; u < K; ++u) {
-        float f[EPV];
-        Chunk<T, VB>::unpack(w[u], f);
+        uint64_t f[P::N];
+        P::unpack(w[u], f);
 #pragma unroll
-        for (int i = 0; i < EPV; ++i) s += f[i];
+        for (int i = 0; i < P::N; ++i) s = add2(s, f[i]);
       }
-      const float cm = s * (1.f / (K * EPV));
+      float sa, sb;
+      unpair(s, sa, sb);
+      const float cm = (sa + sb) * (1.f / (K * EPV));
+      // a single element's second half is no element
+      const uint64_t minus = pair(-cm, EPV == 1 ? 0.f : -cm);
 #pragma unroll
       for (int u = 0; u < K; ++u) {
-        float f[EPV];
-        Chunk<T, VB>::unpack(w[u], f);
+        uint64_t f[P::N];
+        P::unpack(w[u], f);
 #pragma unroll
-        for (int i = 0; i < EPV; ++i) q += (f[i] - cm) * (f[i] - cm);
+        for (int i = 0; i < P::N; ++i) {
+          const uint64_t d = add2(f[i], minus);
+          q = fma2(d, d, q);
+        }
       }
-      norm_join(n, mean, m2, K * EPV, cm, q);
-    };
-    int r = t.tr;
-    for (; r + (U - 1) * t.trows < t.rows; r += U * t.trows) chunk(Count<U>{});
-    for (; r < t.rows; r += t.trows) chunk(Count<1>{});
+      unpair(q, sa, sb);
+      norm_join(n, mean, m2, K * EPV, cm, sa + sb);
+    });
   }
   part[threadIdx.x] = make_float3(n, mean, m2);
   __syncthreads();
-  // lanes j of a group's `lanes` threads join its threads' results
+  // `lanes` threads of a group join its threads' results
   int lanes = 32;
   while (lanes * t.groups > kNormThreads) lanes >>= 1;
   const int g = threadIdx.x / lanes, j = threadIdx.x & (lanes - 1);
@@ -210,125 +292,166 @@ __device__ void norm_stats(const NormArgs& a, int64_t block) {
     norm_join(n, mean, m2, nb, mb, sb);
   }
   auto finish = [&](float mu, float var) {
-    if (on && j == 0)
-      a.stats[t.segment(a) * a.G + t.g0 + g] = make_float2(mu, rsqrtf(var + a.eps));
+    if (on && j == 0) a.stats[me.seg_group + g] = make_float2(mu, rsqrtf(var + a.eps));
   };
-  if (v.tiles == 1) {
-    finish(mean, m2 / n);
-    return;
-  }
-  float2* const mine = a.partial + (block - static_cast<int64_t>(t.tile) * t.step) * a.partial_stride + g;
-  const int64_t hop = static_cast<int64_t>(t.step) * a.partial_stride;
-  if (on && j == 0) mine[t.tile * hop] = make_float2(mean, m2);
-  norm_join_tiles(a, v, t.counter, t.tile, [&](int slot, int next, int count, int64_t full,
-                                               int64_t tail, bool final) {
+  float2* const mine =
+      a.partial + (t.block - static_cast<int64_t>(t.tile) * t.step) * a.partial_stride + g;
+  const int64_t next_tile = static_cast<int64_t>(t.step) * a.partial_stride;
+  if (on && j == 0) mine[t.tile * next_tile] = make_float2(mean, m2);
+  if (DIRECT) return;
+  norm_join_tiles(a, t, [&](int slot, int next, int count, int64_t full, int64_t tail,
+                            bool final) {
     // the mean of the means, then the deviations from it
     const float nf = static_cast<float>(full) * a.cg, nt = static_cast<float>(tail) * a.cg;
     const float all = nf * (count - 1) + nt;
-    const float2* q = mine + slot * hop;
+    const float2* q = mine + slot * next_tile;
     float mu = 0.f, dev = 0.f;
     if (on)
       for (int k = j; k < count; k += lanes)
-        mu += __ldcg(&q[k * next * hop].x) * ((k + 1 < count ? nf : nt) / all);
+        mu += __ldcg(&q[k * next * next_tile].x) * ((k + 1 < count ? nf : nt) / all);
     for (int d = 1; d < lanes; d <<= 1) mu += __shfl_xor_sync(~0u, mu, d);
     if (on)
       for (int k = j; k < count; k += lanes) {
-        const float2 o = __ldcg(q + k * next * hop);
+        const float2 o = __ldcg(q + k * next * next_tile);
         dev += o.y + (o.x - mu) * (o.x - mu) * (k + 1 < count ? nf : nt);
       }
     for (int d = 1; d < lanes; d <<= 1) dev += __shfl_xor_sync(~0u, dev, d);
     if (final) finish(mu, dev / all);
-    else if (on && j == 0) mine[slot * hop] = make_float2(mu, dev);
+    else if (on && j == 0) mine[slot * next_tile] = make_float2(mu, dev);
   });
 }
 
-template <typename T, int VB, int ACT, int U>
-__device__ void norm_apply(const NormArgs& a, int64_t block) {
-  constexpr int EPV = Chunk<T, VB>::EPV;
-  const NormTile<EPV> t(a, block);
+// h = x * scale + shift of one group, as pairs.  16-bit x has no digits that
+// the mean's product could lose; fp32 x is centred first (shift: -mean).
+template <typename T> struct NormCentre {
+  uint64_t shift, scale;
+  __device__ __forceinline__ NormCentre(float2 st) {
+    const float s = sizeof(T) == 2 ? -st.x * st.y : -st.x;
+    shift = pair(s, s);
+    scale = pair(st.y, st.y);
+  }
+  __device__ __forceinline__ uint64_t operator()(uint64_t x) const {
+    return sizeof(T) == 2 ? fma2(x, scale, shift) : mul2(add2(x, shift), scale);
+  }
+};
+
+// The statistics of a tile's groups from its unit's partial results (direct):
+// the mean of the means, then the deviations from it.
+__device__ __forceinline__ void norm_join_here(const NormArgs& a, const NormTile& t,
+                                               const NormThread& me, float2* st) {
   const NormLevel& v = a.lv[t.l];
-  for (int col = t.tc; col < t.nvc; col += t.tcols) {
-    const int c0 = t.g0 * a.cg + col * EPV;
-    const float2 st = __ldcg(a.stats + t.segment(a) * a.G + c0 / a.cg);
-    float w[EPV], d[EPV];
-#pragma unroll
-    for (int i = 0; i < EPV; ++i) {
-      const int64_t at = static_cast<int64_t>(t.l) * a.affine_level + c0 + i;
-      w[i] = norm_param(a.weight, a.affine_dtype, at, 1.f) * st.y;
-      d[i] = norm_param(a.bias, a.affine_dtype, at, 0.f);
-      // 16-bit x has no digits that the mean's product could lose: one step less
-      if (sizeof(T) == 2) d[i] -= st.x * w[i];
+  int lanes = 32;
+  while (lanes * t.groups > kNormThreads) lanes >>= 1;
+  const int g = threadIdx.x / lanes, j = threadIdx.x & (lanes - 1);
+  const bool on = g < t.groups;
+  const float2* q = a.partial + (t.block - static_cast<int64_t>(t.tile) * t.step) * a.partial_stride + g;
+  const int64_t next = static_cast<int64_t>(t.step) * a.partial_stride;
+  const float full = static_cast<float>(v.tile_rows) * a.cg;
+  const float tail = static_cast<float>(v.rows - static_cast<int64_t>(v.tiles - 1) * v.tile_rows) * a.cg;
+  const float all = static_cast<float>(v.rows) * a.cg;
+  float mu = 0.f, dev = 0.f;
+  if (on) {
+#pragma unroll 4
+    for (int k = j; k < v.tiles; k += lanes)
+      mu += __ldcg(&q[k * next].x) * ((k + 1 < v.tiles ? full : tail) / all);
+  }
+  for (int d = 1; d < lanes; d <<= 1) mu += __shfl_xor_sync(~0u, mu, d);
+  if (on) {
+#pragma unroll 4
+    for (int k = j; k < v.tiles; k += lanes) {
+      const float2 o = __ldcg(q + k * next);
+      dev += o.y + (o.x - mu) * (o.x - mu) * (k + 1 < v.tiles ? full : tail);
     }
-    const T* p = reinterpret_cast<const T*>(v.x) + t.b * v.x_batch + (t.row0 + t.tr) * v.x_row + c0;
-    T* y = reinterpret_cast<T*>(v.out) + t.b * v.out_batch + (t.row0 + t.tr) * v.out_row + c0;
-    const int64_t hop = t.trows * v.x_row, yhop = t.trows * v.out_row;
-    auto chunk = [&](auto count) {
+  }
+  for (int d = 1; d < lanes; d <<= 1) dev += __shfl_xor_sync(~0u, dev, d);
+  if (on && j == 0) {
+    st[g] = make_float2(mu, rsqrtf(dev / all + a.eps));
+    if (t.tile == 0) a.stats[me.seg_group + g] = st[g];  // for the backward
+  }
+  __syncthreads();
+}
+
+template <typename T, int VB, int ACT, bool DIRECT, int U>
+__device__ void norm_apply(const NormArgs& a, const NormTile& t) {
+  using P = Pairs<T, VB>;
+  constexpr int EPV = P::EPV;
+  __shared__ float2 joined[DIRECT ? kNormMaxSlab : 1];
+  const NormLevel& v = a.lv[t.l];
+  const NormThread me(a, t);
+  if (DIRECT) norm_join_here(a, t, me, joined);
+  const int64_t hop = t.trows * v.x_row, yhop = t.trows * v.out_row;
+  for (int col = me.tc; col < t.nvc; col += t.tcols) {
+    const int c0 = t.g0 * a.cg + col * EPV;
+    const float2 st = DIRECT ? joined[c0 / a.cg - t.g0]
+                               : __ldcg(a.stats + me.segment * a.G + c0 / a.cg);
+    float f[EPV];
+    uint64_t w[P::N], d[P::N];
+    const int64_t at = static_cast<int64_t>(t.l) * a.affine_level + c0;
+    norm_params<EPV>(a.weight, a.affine_dtype, at, 1.f, f);
+    P::of(f, w);
+    norm_params<EPV>(a.bias, a.affine_dtype, at, 0.f, f);
+    P::of(f, d);
+    const uint64_t minus = pair(-st.x, -st.x), r2 = pair(st.y, st.y);
+#pragma unroll
+    for (int i = 0; i < P::N; ++i) {
+      w[i] = mul2(w[i], r2);
+      if (sizeof(T) == 2) d[i] = fma2(w[i], minus, d[i]);  // as NormCentre
+    }
+    const T* p = reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row + c0;
+    T* y = reinterpret_cast<T*>(v.out) + v.out_batch * t.b + (t.row0 + me.tr) * v.out_row + c0;
+    norm_rows<U>(t, me.tr, [&](auto count) {
       constexpr int K = decltype(count)::value;
       Raw<VB> raw[K];
 #pragma unroll
-      for (int u = 0; u < K; ++u) raw[u] = ld_chunk<VB>(p + u * hop);
+      for (int u = 0; u < K; ++u) raw[u] = norm_ld<VB>(p + u * hop);
       p += K * hop;
 #pragma unroll
       for (int u = 0; u < K; ++u) {
-        float f[EPV];
-        Chunk<T, VB>::unpack(raw[u], f);
+        uint64_t e[P::N];
+        P::unpack(raw[u], e);
 #pragma unroll
-        for (int i = 0; i < EPV; ++i)
-          f[i] = norm_act<ACT>((sizeof(T) == 2 ? f[i] : f[i] - st.x) * w[i] + d[i]);
-        st_chunk<VB>(y + u * yhop, Chunk<T, VB>::pack(f));
+        for (int i = 0; i < P::N; ++i)
+          e[i] = norm_act<ACT>(fma2(sizeof(T) == 2 ? e[i] : add2(e[i], minus), w[i], d[i]));
+        norm_st<VB>(y + u * yhop, P::pack(e));
       }
       y += K * yhop;
-    };
-    int r = t.tr;
-    for (; r + (U - 1) * t.trows < t.rows; r += U * t.trows) chunk(Count<U>{});
-    for (; r < t.rows; r += t.trows) chunk(Count<1>{});
-  }
-}
-
-template <typename T, int VB, int ACT, int U>
-__global__ void __launch_bounds__(kNormThreads, 4)
-norm_fwd_kernel(const __grid_constant__ NormArgs a, const NormWave w) {
-  norm_let_next_start();
-  int64_t block;
-  if (norm_applies(w, block)) {
-    norm_wait_previous();
-    norm_apply<T, VB, ACT, U>(a, block);
-  } else {
-    norm_stats<T, VB, U>(a, block);
+    });
   }
 }
 
 // ------------------------------------------------------------------ backward
-// Sums s1, s2 per channel of one tile; the unit's last CTA joins the tiles and
-// forms the groups' coefficients a, q.
-template <typename T, int VB, int ACT, int U>
-__device__ void norm_grad_stats(const NormArgs& a, int64_t block) {
-  constexpr int EPV = Chunk<T, VB>::EPV;
-  __shared__ float2 part[kNormThreads][EPV];
-  const NormTile<EPV> t(a, block);
+// Sums s1, s2 per channel of one tile, and the groups' coefficients a, q of the unit.
+template <typename T, int VB, int ACT, bool DIRECT, int U>
+__device__ void norm_grad_stats(const NormArgs& a, const NormTile& t) {
+  using P = Pairs<T, VB>;
+  constexpr int EPV = P::EPV;
+  __shared__ float2 part[kNormThreads * EPV];
   const NormLevel& v = a.lv[t.l];
-  float2* mine = a.partial + block * a.partial_stride;
+  const NormThread me(a, t);
+  const int64_t hop = t.trows * v.x_row, ghop = t.trows * v.gy_row;
+  float2* const mine = a.partial + static_cast<int64_t>(t.block) * a.partial_stride;
   for (int col0 = 0; col0 < t.nvc; col0 += t.tcols) {
-    const int col = col0 + t.tc;
-    float s1[EPV], s2[EPV];
+    const int col = col0 + me.tc;
+    uint64_t s1[P::N], s2[P::N];
 #pragma unroll
-    for (int i = 0; i < EPV; ++i) s1[i] = s2[i] = 0.f;
+    for (int i = 0; i < P::N; ++i) s1[i] = s2[i] = 0;  // two zeros
     if (col < t.nvc) {
       const int c0 = t.g0 * a.cg + col * EPV;
-      const float2 st = __ldcg(a.stats + t.segment(a) * a.G + c0 / a.cg);
-      float w[EPV], d[EPV];
+      const NormCentre<T> centre(__ldg(a.stats + me.segment * a.G + c0 / a.cg));
+      uint64_t w[P::N], d[P::N];
       if (ACT != MSDA_ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < EPV; ++i) {
-          const int64_t at = static_cast<int64_t>(t.l) * a.affine_level + c0 + i;
-          w[i] = norm_param(a.weight, a.affine_dtype, at, 1.f);
-          d[i] = norm_param(a.bias, a.affine_dtype, at, 0.f);
-        }
+        float f[EPV];
+        const int64_t at = static_cast<int64_t>(t.l) * a.affine_level + c0;
+        norm_params<EPV>(a.weight, a.affine_dtype, at, 1.f, f);
+        P::of(f, w);
+        norm_params<EPV>(a.bias, a.affine_dtype, at, 0.f, f);
+        P::of(f, d);
       }
-      const T* p = reinterpret_cast<const T*>(v.x) + t.b * v.x_batch + (t.row0 + t.tr) * v.x_row + c0;
-      const T* g = reinterpret_cast<const T*>(v.gy) + t.b * v.gy_batch + (t.row0 + t.tr) * v.gy_row + c0;
-      const int64_t hop = t.trows * v.x_row, ghop = t.trows * v.gy_row;
-      auto chunk = [&](auto count) {
+      const T* p =
+          reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row + c0;
+      const T* g =
+          reinterpret_cast<const T*>(v.gy) + v.gy_batch * t.b + (t.row0 + me.tr) * v.gy_row + c0;
+      norm_rows<U>(t, me.tr, [&](auto count) {
         constexpr int K = decltype(count)::value;
         Raw<VB> rx[K], rg[K];
 #pragma unroll
@@ -340,31 +463,35 @@ __device__ void norm_grad_stats(const NormArgs& a, int64_t block) {
         g += K * ghop;
 #pragma unroll
         for (int u = 0; u < K; ++u) {
-          float f[EPV], e[EPV];
-          Chunk<T, VB>::unpack(rx[u], f);
-          Chunk<T, VB>::unpack(rg[u], e);
+          uint64_t f[P::N], e[P::N];
+          P::unpack(rx[u], f);
+          P::unpack(rg[u], e);
 #pragma unroll
-          for (int i = 0; i < EPV; ++i) {
-            const float h = (f[i] - st.x) * st.y;
-            const float dz = ACT == MSDA_ACT_NONE ? e[i] : e[i] * norm_dact<ACT>(h * w[i] + d[i]);
-            s1[i] += dz;
-            s2[i] += dz * h;
+          for (int i = 0; i < P::N; ++i) {
+            const uint64_t h = centre(f[i]);
+            const uint64_t dz =
+                ACT == MSDA_ACT_NONE ? e[i] : mul2(e[i], norm_dact<ACT>(fma2(h, w[i], d[i])));
+            s1[i] = add2(s1[i], dz);
+            s2[i] = fma2(dz, h, s2[i]);
           }
         }
-      };
-      int r = t.tr;
-      for (; r + (U - 1) * t.trows < t.rows; r += U * t.trows) chunk(Count<U>{});
-      for (; r < t.rows; r += t.trows) chunk(Count<1>{});
+      });
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < EPV; ++i) part[threadIdx.x][i] = make_float2(s1[i], s2[i]);
+    for (int i = 0; i < P::N; ++i) {
+      float a0, a1, b0, b1;
+      unpair(s1[i], a0, a1);
+      unpair(s2[i], b0, b1);
+      part[threadIdx.x * EPV + 2 * i] = make_float2(a0, b0);
+      if (2 * i + 1 < EPV) part[threadIdx.x * EPV + 2 * i + 1] = make_float2(a1, b1);
+    }
     __syncthreads();
-    const int cols = min(t.tcols, t.nvc - col0);
+    const int cols = min(t.tcols, t.nvc - col0), row = t.tcols * EPV;
     for (int c = threadIdx.x; c < cols * EPV; c += kNormThreads) {
       float2 s = make_float2(0.f, 0.f);
       for (int k = 0; k < t.trows; ++k) {
-        const float2 o = part[k * t.tcols + c / EPV][c % EPV];
+        const float2 o = part[k * row + c];
         s.x += o.x;
         s.y += o.y;
       }
@@ -372,11 +499,31 @@ __device__ void norm_grad_stats(const NormArgs& a, int64_t block) {
     }
   }
   const int cw = t.groups * a.cg, c0 = t.g0 * a.cg;
-  float2* const first = a.partial + (block - static_cast<int64_t>(t.tile) * t.step) * a.partial_stride;
-  const int64_t hop = static_cast<int64_t>(t.step) * a.partial_stride;
-  float2* const chan = a.chan + t.segment(a) * a.C + c0;
-  norm_join_tiles(a, v, t.counter, t.tile, [&](int slot, int next, int count, int64_t, int64_t,
-                                               bool final) {
+  // sums of a group's channels, from `s`, weighted
+  auto group = [&](const float2* s, int g) {
+    float2 sum = make_float2(0.f, 0.f);
+    for (int i = 0; i < a.cg; ++i) {
+      const int c = g * a.cg + i;
+      float w;
+      norm_params<1>(a.weight, a.affine_dtype,
+                     static_cast<int64_t>(t.l) * a.affine_level + c0 + c, 1.f, &w);
+      sum.x += w * s[c].x;
+      sum.y += w * s[c].y;
+    }
+    return sum;
+  };
+  if (DIRECT) {
+    __syncthreads();  // `mine` is written
+    const int stride = a.lv[0].slab_groups;
+    for (int g = threadIdx.x; g < t.groups; g += kNormThreads)
+      a.weighted[static_cast<int64_t>(t.block) * stride + g] = group(mine, g);
+    return;
+  }
+  float2* const first =
+      a.partial + (t.block - static_cast<int64_t>(t.tile) * t.step) * a.partial_stride;
+  const int64_t next_tile = static_cast<int64_t>(t.step) * a.partial_stride;
+  float2* const chan = a.chan + me.seg_chan;
+  norm_join_tiles(a, t, [&](int slot, int next, int count, int64_t, int64_t, bool final) {
     // `lanes` threads of a channel take the tiles in turn
     int lanes = 32;
     while (lanes > 1 && lanes * cw > kNormThreads) lanes >>= 1;
@@ -387,7 +534,7 @@ __device__ void norm_grad_stats(const NormArgs& a, int64_t block) {
       if (c < cw) {
 #pragma unroll 8
         for (int k = lane; k < count; k += lanes) {
-          const float2 o = __ldcg(first + (slot + k * next) * hop + c);
+          const float2 o = __ldcg(first + (slot + k * next) * next_tile + c);
           s.x += o.x;
           s.y += o.y;
         }
@@ -396,48 +543,125 @@ __device__ void norm_grad_stats(const NormArgs& a, int64_t block) {
         s.x += __shfl_xor_sync(~0u, s.x, d);
         s.y += __shfl_xor_sync(~0u, s.y, d);
       }
-      if (c < cw && lane == 0) (final ? chan : first + slot * hop)[c] = s;
+      if (c < cw && lane == 0) (final ? chan : first + slot * next_tile)[c] = s;
     }
     if (!final) return;
     __syncthreads();
     const float n = static_cast<float>(v.rows) * a.cg;
     for (int g = threadIdx.x; g < t.groups; g += kNormThreads) {
-      float sa = 0.f, sq = 0.f;
-      for (int i = 0; i < a.cg; ++i) {
-        const int c = g * a.cg + i;
-        const float w = norm_param(a.weight, a.affine_dtype,
-                                   static_cast<int64_t>(t.l) * a.affine_level + c0 + c, 1.f);
-        const float2 s = chan[c];
-        sa += w * s.x;
-        sq += w * s.y;
-      }
-      a.coef[t.segment(a) * a.G + t.g0 + g] = make_float2(sa / n, sq / n);
+      const float2 sum = group(chan, g);
+      a.coef[me.seg_group + g] = make_float2(sum.x / n, sum.y / n);
     }
   });
 }
 
-template <typename T, int VB, int ACT, int U>
-__device__ void norm_grad_apply(const NormArgs& a, int64_t block) {
-  constexpr int EPV = Chunk<T, VB>::EPV;
-  const NormTile<EPV> t(a, block);
+// The coefficients of a tile's groups from its unit's weighted sums (direct).
+__device__ __forceinline__ void norm_grad_join_here(const NormArgs& a, const NormTile& t,
+                                                    float2* co) {
   const NormLevel& v = a.lv[t.l];
-  for (int col = t.tc; col < t.nvc; col += t.tcols) {
-    const int c0 = t.g0 * a.cg + col * EPV;
-    const float2 st = __ldcg(a.stats + t.segment(a) * a.G + c0 / a.cg);
-    const float2 co = __ldcg(a.coef + t.segment(a) * a.G + c0 / a.cg);
-    float w[EPV], d[EPV];
-#pragma unroll
-    for (int i = 0; i < EPV; ++i) {
-      const int64_t at = static_cast<int64_t>(t.l) * a.affine_level + c0 + i;
-      w[i] = norm_param(a.weight, a.affine_dtype, at, 1.f);
-      if (ACT != MSDA_ACT_NONE) d[i] = norm_param(a.bias, a.affine_dtype, at, 0.f);
+  int lanes = 32;
+  while (lanes * t.groups > kNormThreads) lanes >>= 1;
+  const int g = threadIdx.x / lanes, j = threadIdx.x & (lanes - 1);
+  const bool on = g < t.groups;
+  const int stride = a.lv[0].slab_groups;
+  const float2* q = a.weighted + (t.block - static_cast<int64_t>(t.tile) * t.step) * stride + g;
+  const int64_t next = static_cast<int64_t>(t.step) * stride;
+  float2 s = make_float2(0.f, 0.f);
+  if (on) {
+#pragma unroll 4
+    for (int k = j; k < v.tiles; k += lanes) {
+      const float2 o = __ldcg(q + k * next);
+      s.x += o.x;
+      s.y += o.y;
     }
-    const T* p = reinterpret_cast<const T*>(v.x) + t.b * v.x_batch + (t.row0 + t.tr) * v.x_row + c0;
-    const T* g = reinterpret_cast<const T*>(v.gy) + t.b * v.gy_batch + (t.row0 + t.tr) * v.gy_row + c0;
-    T* y = reinterpret_cast<T*>(v.out) + t.b * v.out_batch + (t.row0 + t.tr) * v.out_row + c0;
-    const int64_t hop = t.trows * v.x_row, ghop = t.trows * v.gy_row, yhop = t.trows * v.out_row;
-    const float ra = st.y * co.x, rq = st.y * co.y;
-    auto chunk = [&](auto count) {
+  }
+  for (int d = 1; d < lanes; d <<= 1) {
+    s.x += __shfl_xor_sync(~0u, s.x, d);
+    s.y += __shfl_xor_sync(~0u, s.y, d);
+  }
+  const float n = static_cast<float>(v.rows) * a.cg;
+  if (on && j == 0) co[g] = make_float2(s.x / n, s.y / n);
+  __syncthreads();
+}
+
+// Gradients of kNormParamChannels channels of the affine map, of one level or
+// of all: a warp's worth of lanes a channel takes the batch entries' (direct:
+// their tiles') sums in turn.
+__device__ __forceinline__ void norm_param_grad(const NormArgs& a, int cta) {
+  const int per_row = (a.C + kNormParamChannels - 1) / kNormParamChannels;
+  const int row = cta / per_row;
+  const int c = (cta - row * per_row) * kNormParamChannels + (threadIdx.x & (kNormParamChannels - 1));
+  const int lane = threadIdx.x / kNormParamChannels;
+  constexpr int kLanes = kNormThreads / kNormParamChannels;
+  __shared__ float2 sums[kNormThreads];
+  float2 s = make_float2(0.f, 0.f);
+  auto add = [&](const float2& o) {
+    s.x += o.x;
+    s.y += o.y;
+  };
+  const int l0 = a.affine_level ? row : 0, l1 = a.affine_level ? row + 1 : a.L;
+  if (c < a.C)
+    for (int l = l0; l < l1; ++l) {
+      const NormLevel& v = a.lv[l];
+      if (v.rows == 0) continue;
+      if (a.direct) {
+        const int wide = v.slab_groups * a.cg, slab = c / wide, n = a.B * v.tiles;
+        const float2* q = a.partial + static_cast<int64_t>(v.tile0 + slab) * a.partial_stride +
+                          (c - slab * wide);
+#pragma unroll 8
+        for (int k = lane; k < n; k += kLanes)
+          add(__ldcg(q + static_cast<int64_t>(k) * v.slabs * a.partial_stride));
+      } else {
+#pragma unroll 4
+        for (int b = lane; b < a.B; b += kLanes)
+          add(__ldcg(a.chan + (static_cast<int64_t>(b) * a.L + l) * a.C + c));
+      }
+    }
+  sums[threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.x >= kNormParamChannels || c >= a.C) return;
+  for (int k = 1; k < kLanes; ++k) add(sums[k * kNormParamChannels + threadIdx.x]);
+  auto put = [&](void* out, float x) {
+    const int64_t i = static_cast<int64_t>(row) * a.C + c;
+    if (out == nullptr) return;
+    if (a.affine_dtype == MSDA_FLOAT32) static_cast<float*>(out)[i] = x;
+    else if (a.affine_dtype == MSDA_FLOAT16) static_cast<__half*>(out)[i] = __float2half_rn(x);
+    else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(x);
+  };
+  put(a.gweight, s.y);
+  put(a.gbias, s.x);
+}
+
+template <typename T, int VB, int ACT, bool DIRECT, int U>
+__device__ void norm_grad_apply(const NormArgs& a, const NormTile& t) {
+  using P = Pairs<T, VB>;
+  constexpr int EPV = P::EPV;
+  __shared__ float2 joined[DIRECT ? kNormMaxSlab : 1];
+  const NormLevel& v = a.lv[t.l];
+  const NormThread me(a, t);
+  if (DIRECT) norm_grad_join_here(a, t, joined);
+  const int64_t hop = t.trows * v.x_row, ghop = t.trows * v.gy_row, yhop = t.trows * v.out_row;
+  for (int col = me.tc; col < t.nvc; col += t.tcols) {
+    const int c0 = t.g0 * a.cg + col * EPV;
+    const float2 st = __ldg(a.stats + me.segment * a.G + c0 / a.cg);
+    const float2 co = DIRECT ? joined[c0 / a.cg - t.g0]
+                               : __ldcg(a.coef + me.segment * a.G + c0 / a.cg);
+    const NormCentre<T> centre(st);
+    float f[EPV];
+    uint64_t w[P::N], d[P::N];
+    const int64_t at = static_cast<int64_t>(t.l) * a.affine_level + c0;
+    norm_params<EPV>(a.weight, a.affine_dtype, at, 1.f, f);
+    P::of(f, w);
+    if (ACT != MSDA_ACT_NONE) {
+      norm_params<EPV>(a.bias, a.affine_dtype, at, 0.f, f);
+      P::of(f, d);
+    }
+    const T* p = reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row + c0;
+    const T* g =
+        reinterpret_cast<const T*>(v.gy) + v.gy_batch * t.b + (t.row0 + me.tr) * v.gy_row + c0;
+    T* y = reinterpret_cast<T*>(v.out) + v.out_batch * t.b + (t.row0 + me.tr) * v.out_row + c0;
+    const uint64_t r2 = pair(st.y, st.y), ma = pair(-co.x, -co.x), mq = pair(-co.y, -co.y);
+    norm_rows<U>(t, me.tr, [&](auto count) {
       constexpr int K = decltype(count)::value;
       Raw<VB> rx[K], rg[K];
 #pragma unroll
@@ -449,76 +673,99 @@ __device__ void norm_grad_apply(const NormArgs& a, int64_t block) {
       g += K * ghop;
 #pragma unroll
       for (int u = 0; u < K; ++u) {
-        float f[EPV], e[EPV];
-        Chunk<T, VB>::unpack(rx[u], f);
-        Chunk<T, VB>::unpack(rg[u], e);
+        uint64_t x[P::N], e[P::N];
+        P::unpack(rx[u], x);
+        P::unpack(rg[u], e);
 #pragma unroll
-        for (int i = 0; i < EPV; ++i) {
-          const float h = (f[i] - st.x) * st.y;
-          const float dz = ACT == MSDA_ACT_NONE ? e[i] : e[i] * norm_dact<ACT>(h * w[i] + d[i]);
-          f[i] = dz * (st.y * w[i]) - ra - h * rq;
+        for (int i = 0; i < P::N; ++i) {
+          const uint64_t h = centre(x[i]);
+          const uint64_t dz =
+              ACT == MSDA_ACT_NONE ? e[i] : mul2(e[i], norm_dact<ACT>(fma2(h, w[i], d[i])));
+          x[i] = mul2(r2, fma2(dz, w[i], fma2(h, mq, ma)));
         }
-        st_chunk<VB>(y + u * yhop, Chunk<T, VB>::pack(f));
+        st_chunk<VB>(y + u * yhop, P::pack(x));
       }
       y += K * yhop;
-    };
-    int r = t.tr;
-    for (; r + (U - 1) * t.trows < t.rows; r += U * t.trows) chunk(Count<U>{});
-    for (; r < t.rows; r += t.trows) chunk(Count<1>{});
+    });
   }
 }
 
-template <typename T, int VB, int ACT, int U>
-__global__ void __launch_bounds__(kNormThreads, 3)
-norm_bwd_kernel(const __grid_constant__ NormArgs a, const NormWave w) {
+// ------------------------------------------------------------------ the launches
+// CTAs per SM and vectors in flight per thread: of the combinations that were
+// timed (3 to 6 CTAs, 2 to 8 vectors) the fastest.
+template <typename T, int VB, int ACT, bool BWD, bool DIRECT>
+__global__ void __launch_bounds__(kNormThreads, BWD ? 3 : 4)
+norm_stats_kernel(const __grid_constant__ NormArgs a) {
   norm_let_next_start();
-  int64_t block;
-  if (norm_applies(w, block)) {
-    norm_wait_previous();
-    norm_grad_apply<T, VB, ACT, U>(a, block);
-  } else {
-    norm_grad_stats<T, VB, ACT, U>(a, block);
-  }
+  const NormTile t = norm_tile<Chunk<T, VB>::EPV>(a, blockIdx.x);
+  if (BWD) norm_grad_stats<T, VB, ACT, DIRECT, 2>(a, t);
+  else norm_stats<T, VB, DIRECT, 8>(a, t);
 }
 
-// ------------------------------------------------------------------ launches
-template <typename T, int VB, int ACT>
-cudaError_t norm_launch(const NormArgs& a, const NormWave& w, bool backward, cudaStream_t st) {
-  const unsigned int grid = static_cast<unsigned int>(w.applies + w.stats);
-  if (grid == 0) return cudaSuccess;
+template <typename T, int VB, int ACT, bool BWD, bool DIRECT>
+__global__ void __launch_bounds__(kNormThreads, BWD ? 3 : 4)
+norm_apply_kernel(const __grid_constant__ NormArgs a) {
+  const int block = static_cast<int>(blockIdx.x) - a.param_ctas;
+  if (BWD && block < 0) {
+    norm_wait_previous();
+    norm_param_grad(a, blockIdx.x);
+    return;
+  }
+  const NormTile t = norm_tile<Chunk<T, VB>::EPV>(a, a.tiles - 1 - block);
+  norm_wait_previous();
+  if (BWD) norm_grad_apply<T, VB, ACT, DIRECT, 2>(a, t);
+  else norm_apply<T, VB, ACT, DIRECT, 4>(a, t);
+}
+
+template <typename T, int VB, int ACT, bool BWD, bool DIRECT>
+cudaError_t norm_launch_one(const NormArgs& a, cudaStream_t st) {
+  // the forward's statistics are the same for every activation
+  constexpr int kAct = BWD ? ACT : MSDA_ACT_NONE;
+  if (a.tiles > 0) {
+    norm_stats_kernel<T, VB, kAct, BWD, DIRECT><<<a.tiles, kNormThreads, 0, st>>>(a);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return err;
+  }
+  if (a.tiles + a.param_ctas == 0) return cudaSuccess;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = dim3(a.tiles + a.param_ctas);
   cfg.blockDim = dim3(kNormThreads);
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = w.applies > 0 ? 1 : 0;  // the first launch follows other work
-  return backward ? cudaLaunchKernelEx(&cfg, norm_bwd_kernel<T, VB, ACT, 2>, a, w)
-                  : cudaLaunchKernelEx(&cfg, norm_fwd_kernel<T, VB, ACT, 4>, a, w);
+  cfg.numAttrs = a.tiles > 0 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, norm_apply_kernel<T, VB, ACT, BWD, DIRECT>, a);
 }
 
 template <typename T, int VB>
-cudaError_t norm_launch_act(const NormArgs& a, const NormWave& w, int act, bool backward,
-                            cudaStream_t st) {
+cudaError_t norm_launch_act(const NormArgs& a, int act, bool backward, cudaStream_t st) {
   switch (act) {
-    case MSDA_ACT_RELU: return norm_launch<T, VB, MSDA_ACT_RELU>(a, w, backward, st);
-    case MSDA_ACT_SILU: return norm_launch<T, VB, MSDA_ACT_SILU>(a, w, backward, st);
-    case MSDA_ACT_GELU: return norm_launch<T, VB, MSDA_ACT_GELU>(a, w, backward, st);
-    default: return norm_launch<T, VB, MSDA_ACT_NONE>(a, w, backward, st);
+#define MSDA_NORM_ACT(ACT)                                                   \
+  case ACT:                                                                  \
+    if (a.direct)                                                            \
+      return backward ? norm_launch_one<T, VB, ACT, true, true>(a, st)       \
+                      : norm_launch_one<T, VB, ACT, false, true>(a, st);     \
+    return backward ? norm_launch_one<T, VB, ACT, true, false>(a, st)        \
+                    : norm_launch_one<T, VB, ACT, false, false>(a, st);
+    MSDA_NORM_ACT(MSDA_ACT_RELU)
+    MSDA_NORM_ACT(MSDA_ACT_SILU)
+    MSDA_NORM_ACT(MSDA_ACT_GELU)
+    MSDA_NORM_ACT(MSDA_ACT_NONE)
+#undef MSDA_NORM_ACT
   }
+  return cudaErrorInvalidValue;
 }
 
 template <typename T>
-cudaError_t norm_wave_t(const NormArgs& a, const NormWave& w, int vb, int act, bool backward,
-                        cudaStream_t st) {
+cudaError_t norm_launch(const NormArgs& a, int vb, int act, bool backward, cudaStream_t st) {
   switch (vb) {
-    case 16: return norm_launch_act<T, 16>(a, w, act, backward, st);
-    case 8: return norm_launch_act<T, 8>(a, w, act, backward, st);
-    case 4: return norm_launch_act<T, 4>(a, w, act, backward, st);
+    case 16: return norm_launch_act<T, 16>(a, act, backward, st);
+    case 8: return norm_launch_act<T, 8>(a, act, backward, st);
+    case 4: return norm_launch_act<T, 4>(a, act, backward, st);
     default:
-      if constexpr (sizeof(T) == 2) return norm_launch_act<T, 2>(a, w, act, backward, st);
+      if constexpr (sizeof(T) == 2) return norm_launch_act<T, 2>(a, act, backward, st);
       return cudaErrorInvalidValue;
   }
 }
