@@ -20,8 +20,7 @@
 // second moment takes 5 exponent bits (top = 31, a range of 2^31), the first
 // its sign and 4 (top = 15).  E is the largest magnitude's exponent after it
 // is rounded up by one code more than it can be, so the highest code is never
-// reached by rounding; it stands for a value that is not finite, in a block
-// whose exponent byte is 255 for that (and counts as 254).
+// reached by rounding; it stands for a value that is not finite.
 //
 // Moments are rounded at random, up with the probability of the part cut off:
 // a change of 0.1 % a step (b2 = 0.999) is far below the spacing of 12.5 %, and
@@ -84,7 +83,6 @@ template <int N> struct AdamTable {
 };
 
 constexpr uint32_t kMaxFinite = 0x7f7fffffu;
-constexpr uint32_t kOdd = 255u;  // exponent byte of a block with something not finite
 
 // Byte i of a word of codes as a value; `shift` is 8 (E - top).
 template <bool SIGNED>
@@ -97,12 +95,15 @@ __device__ __forceinline__ float adam_decode(uint32_t word, int i, uint32_t shif
   return __uint_as_float(bits);
 }
 __device__ __forceinline__ uint32_t adam_shift(uint32_t e, uint32_t top) {
-  return (min(e, kOdd - 1u) - top) << 3;
+  return (e - top) << 3;
 }
-// The highest code of a block with E = kOdd: not finite.
+// The highest code is no number: whether one of a word's is tested at once.
 template <bool SIGNED>
 __device__ __forceinline__ void adam_decode_odd(uint32_t word, float* f) {
   constexpr uint32_t kTopCode = SIGNED ? 127u : 255u;
+  const bool odd = SIGNED ? ((word & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u) != 0u
+                          : (~word - 0x01010101u & word & 0x80808080u) != 0u;
+  if (!odd) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if ((word >> (8 * i) & kTopCode) == kTopCode) f[i] = __uint_as_float(0x7fc00000u);
@@ -115,26 +116,22 @@ __device__ __noinline__ uint32_t adam_encode_odd(float4 x, uint4 r, uint32_t& e)
   const float f[4] = {x.x, x.y, x.z, x.w};
   const uint32_t rnd[4] = {r.x, r.y, r.z, r.w};
   uint32_t most = 0u;
-  bool lost = false;
   for (int i = 0; i < 4; ++i) {
     const uint32_t b = __float_as_uint(f[i]) & 0x7fffffffu;
     if (b <= kMaxFinite) most = max(most, b);
-    else lost = true;
   }
   most = __reduce_max_sync(~0u, most);
-  lost = __any_sync(~0u, lost);
-  e = min(max((most + 0x1fffffu) >> 23, TOP), kOdd - 1u);
+  e = max((most + 0x1fffffu) >> 23, TOP);
   const int base = static_cast<int>(e - TOP) << 3;
   uint32_t word = 0u;
   for (int i = 0; i < 4; ++i) {
     const uint32_t b = __float_as_uint(f[i]) & 0x7fffffffu;
     int c = static_cast<int>(min(b + rnd[i], kMaxFinite) >> 20) - base;
-    c = min(max(c, !SIGNED && b != 0u ? 1 : 0), static_cast<int>(kTopCode) - 1);
+    c = max(c, !SIGNED && b != 0u ? 1 : 0);
     if (b > kMaxFinite) c = kTopCode;
     if (SIGNED) c |= __float_as_uint(f[i]) >> 24 & 128u;
     word |= static_cast<uint32_t>(c) << (8 * i);
   }
-  if (lost) e = kOdd;
   return word;
 }
 
@@ -299,8 +296,8 @@ adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
           m[i] = adam_decode<true>(cm[u], i, sm);
           v[i] = adam_decode<false>(cv[u], i, sv);
         }
-        if (em[u] == kOdd) adam_decode_odd<true>(cm[u], m);
-        if (ev[u] == kOdd) adam_decode_odd<false>(cv[u], v);
+        adam_decode_odd<true>(cm[u], m);
+        adam_decode_odd<false>(cv[u], v);
       } else {
         Chunk<float, 16>::unpack(rm[u], m);
         Chunk<float, 16>::unpack(rv[u], v);
@@ -366,14 +363,10 @@ adamw_values_kernel(const uint8_t* m, const uint8_t* me, const uint8_t* v, const
     fm[k] = adam_decode<true>(k < 4 ? cm.x : cm.y, k & 3, sm);
     fv[k] = adam_decode<false>(k < 4 ? cv.x : cv.y, k & 3, sv);
   }
-  if (em == kOdd) {
-    adam_decode_odd<true>(cm.x, fm);
-    adam_decode_odd<true>(cm.y, fm + 4);
-  }
-  if (ev == kOdd) {
-    adam_decode_odd<false>(cv.x, fv);
-    adam_decode_odd<false>(cv.y, fv + 4);
-  }
+  adam_decode_odd<true>(cm.x, fm);
+  adam_decode_odd<true>(cm.y, fm + 4);
+  adam_decode_odd<false>(cv.x, fv);
+  adam_decode_odd<false>(cv.y, fv + 4);
   st_chunk<16>(mo + i, Chunk<__nv_bfloat16, 16>::pack(fm));
   st_chunk<16>(vo + i, Chunk<__nv_bfloat16, 16>::pack(fv));
 }

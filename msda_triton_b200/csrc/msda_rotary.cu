@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotPairs = 2048;  // (token, pair) angles of a CTA
-constexpr int kRotUnits = 1024;  // vectors of a CTA's pass: four a thread
+constexpr int kRotUnits = 1024;  // vectors of a CTA's tokens, unless one has more
 constexpr int kRotAxes = 4;
 
 // n / d for 0 <= n < 2^31 as a multiply and shift: with m = ceil(2^(31+l) / d)
@@ -49,7 +49,8 @@ Divider divider(uint32_t d) {
   return Divider{static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + d - 1) / d), 31 + l, d};
 }
 
-// Strides in elements: batch entry, token, head.
+// Strides in elements: token, head, and what a batch entry's first token lies
+// off the token behind the entry before.
 struct RotTensor {
   const char* x;  // what is turned: the input, or the output's gradient
   char* y;
@@ -64,6 +65,9 @@ struct RotArgs {
   int32_t turned;          // vectors per head that are turned
   int32_t tokens;          // per CTA
   int32_t total;           // B * Q
+  int32_t hop;             // tokens between a thread's vectors if those of a token divide the
+                           // CTA's threads (then head and pair stay the same), else 0
+  int32_t flat;            // no tensor has a gap between batch entries
   Divider dq, dunit, dhead, dpair;
   const void* pos;
   int64_t pos_batch;       // elements between batch entries' positions: 0 if shared
@@ -109,131 +113,186 @@ template <int VB> __device__ __forceinline__ Raw<VB> rot_load(const void* p) {
   return r;
 }
 
+// Shared memory of a CTA: the angles' (cos, sin) of its tokens, with room after
+// each vector's N pairs so that lanes with different vectors meet different
+// banks; for the positions' gradient each pair's frequency at its axis, spaced
+// likewise, and the sums of each vector's pairs per axis.
+template <int N> struct RotShared {
+  static constexpr int kPad = N >= 4 ? 2 : 0;
+  static __host__ __device__ int turns(int P) { return P + P / N * kPad; }  // per token
+  static __host__ __device__ int weights(int P) { return P + P / N; }
+  static __host__ __device__ int turn_bytes(int P, int tokens) {
+    return (turns(P) * tokens * 8 + 15) / 16 * 16;
+  }
+};
+
+// A thread has one vector (two, of both halves) in flight; six CTAs an SM (five with
+// interleaved pairs, which take more registers) were
+// faster than three with four each (759 us against 925 for 4.9 GB, 6.5 TB/s).
 template <typename T, int VB, bool PAIRS, bool GPOS>
-__global__ void __launch_bounds__(kRotThreads)
+__global__ void __launch_bounds__(kRotThreads, GPOS ? 4 : PAIRS ? 5 : 6)
 rotary_kernel(const __grid_constant__ RotArgs a) {
-  constexpr int N = Chunk<T, VB>::EPV;            // pairs per turned vector
-  constexpr int U = GPOS ? 2 : 4;                 // vectors in flight per thread
-  __shared__ __align__(16) float2 turn[kRotPairs];
-  __shared__ float sums[GPOS ? kRotUnits : 1][kRotAxes];
+  constexpr int N = Chunk<T, VB>::EPV;  // pairs per turned vector
+  using S = RotShared<N>;
+  extern __shared__ __align__(16) char shared[];
   const int token0 = blockIdx.x * a.tokens;
   const int tokens = min(a.tokens, a.total - token0);
   const int per_token = a.heads * a.units;
   const int count = tokens * per_token;
+  const int row = S::turns(a.P);
+  float2* const turn = reinterpret_cast<float2*>(shared);
+  float4* const weight = reinterpret_cast<float4*>(shared + S::turn_bytes(a.P, a.tokens));
+  float4* const sums = weight + S::weights(a.P);
 
-  Raw<VB> va[U], vb[U], ia[U], ib[U];
-  T* out[U];
-  int at[U];  // first angle in `turn`, -1 for a vector that is copied
-  auto load = [&](int base) {
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = base + i * kRotThreads + threadIdx.x;
-      if (u >= count) continue;
-      const int t = a.dhead(u), rest = u - t * per_token;
+  Raw<VB> va, vb, ia, ib;
+  T* out = nullptr;
+  int t = 0, j = 0, gap = 0;
+  bool second = false;
+  const T *px = nullptr, *pi = nullptr;
+  T* py = nullptr;
+  auto load = [&](int u) {
+    if (u >= count) return;
+    if (u < kRotThreads || a.hop == 0) {
+      t = a.dhead(u);
+      const int rest = u - t * per_token;
       int h = a.dunit(rest);
-      const int j = rest - h * a.units;
-      const uint32_t n = token0 + t, b = a.dq(n), q = n - b * a.dq.d;
-      const bool second = h >= a.heads0;
+      j = rest - h * a.units;
+      second = h >= a.heads0;
       const RotTensor& x = a.t[second];
       if (second) h -= a.heads0;
-      int c = PAIRS ? 2 * N * j : N * j, gap = PAIRS ? N : a.P;
-      at[i] = t * a.P + j * N;
+      int c = PAIRS ? 2 * N * j : N * j;
+      gap = PAIRS ? N : a.P;
       if (j >= a.turned) {
         c = 2 * a.P + (j - a.turned) * N;
         gap = 0;
-        at[i] = -1;
       }
-      const T* p = reinterpret_cast<const T*>(x.x) + b * x.xb + q * x.xq + h * x.xh + c;
-      out[i] = reinterpret_cast<T*>(x.y) + b * x.yb + q * x.yq + h * x.yh + c;
-      va[i] = rot_load<VB>(p);
-      vb[i] = rot_load<VB>(p + gap);
-      if (GPOS) {
-        const T* s = reinterpret_cast<const T*>(x.in) + b * x.ib + q * x.iq + h * x.ih + c;
-        ia[i] = rot_load<VB>(s);
-        ib[i] = rot_load<VB>(s + gap);
-      }
+      px = reinterpret_cast<const T*>(x.x) + h * x.xh + c;
+      py = reinterpret_cast<T*>(x.y) + h * x.yh + c;
+      if (GPOS) pi = reinterpret_cast<const T*>(x.in) + h * x.ih + c;
+    } else {
+      t += a.hop;
+    }
+    const RotTensor& x = a.t[second];
+    const int64_t n = token0 + t;
+    int64_t ox = n * x.xq, oy = n * x.yq, oi = GPOS ? n * x.iq : 0;
+    if (!a.flat) {
+      const int64_t b = a.dq(static_cast<uint32_t>(n));
+      ox += b * x.xb;
+      oy += b * x.yb;
+      if (GPOS) oi += b * x.ib;
+    }
+    va = rot_load<VB>(px + ox);
+    vb = rot_load<VB>(px + ox + gap);
+    out = py + oy;
+    if (GPOS) {
+      ia = rot_load<VB>(pi + oi);
+      ib = rot_load<VB>(pi + oi + gap);
     }
   };
 
-  load(0);
+  load(threadIdx.x);
   for (int i = threadIdx.x; i < tokens * a.P; i += kRotThreads) {
-    const int t = a.dpair(i), j = i - t * a.P;
-    const uint32_t n = token0 + t, b = a.dq(n), q = n - b * a.dq.d;
-    const float p = rot_position(a, b * a.pos_batch + static_cast<int64_t>(q) * a.axes +
-                                        __ldg(a.axis + j));
-    turn[i] = rot_angle(p, __ldg(a.inv_freq + j), a.sign);
+    const int k = a.dpair(i), p = i - k * a.P;
+    const uint32_t n = token0 + k, b = a.dq(n), q = n - b * a.dq.d;
+    const float x = rot_position(a, b * a.pos_batch + static_cast<int64_t>(q) * a.axes +
+                                        __ldg(a.axis + p));
+    turn[k * row + p + p / N * S::kPad] = rot_angle(x, __ldg(a.inv_freq + p), a.sign);
   }
+  if (GPOS)
+    for (int p = threadIdx.x; p < a.P; p += kRotThreads) {
+      const float f = __ldg(a.inv_freq + p);
+      const int on = __ldg(a.axis + p);
+      weight[p + p / N] = make_float4(on == 0 ? f : 0.f, on == 1 ? f : 0.f, on == 2 ? f : 0.f,
+                                      on == 3 ? f : 0.f);
+    }
   __syncthreads();
 
-  for (int base = 0; base < count; base += U * kRotThreads) {
-    if (base > 0) load(base);
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = base + i * kRotThreads + threadIdx.x;
-      if (u >= count) continue;
-      float ax[kRotAxes] = {0.f, 0.f, 0.f, 0.f};
-      if (at[i] < 0) {
-        st_chunk<VB>(out[i], va[i]);
-      } else {
-        float f[2 * N], s[2 * N];
-        Chunk<T, VB>::unpack(va[i], f);
-        Chunk<T, VB>::unpack(vb[i], f + N);
-        if (GPOS) {
-          Chunk<T, VB>::unpack(ia[i], s);
-          Chunk<T, VB>::unpack(ib[i], s + N);
-        }
-        const int j0 = GPOS ? at[i] - static_cast<int>(a.dpair(at[i])) * a.P : 0;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const float2 cs = turn[at[i] + k];
-          const int x1 = PAIRS ? 2 * k : k, x2 = PAIRS ? 2 * k + 1 : k + N;
-          const float y1 = f[x1] * cs.x - f[x2] * cs.y, y2 = f[x2] * cs.x + f[x1] * cs.y;
-          f[x1] = y1;
-          f[x2] = y2;
-          if (GPOS) {
-            const float g = __ldg(a.inv_freq + j0 + k) * (s[x1] * y2 - s[x2] * y1);
-            const int on = __ldg(a.axis + j0 + k);
-#pragma unroll
-            for (int d = 0; d < kRotAxes; ++d) ax[d] += on == d ? g : 0.f;
-          }
-        }
-        st_chunk<VB>(out[i], Chunk<T, VB>::pack(f));
-        st_chunk<VB>(out[i] + (PAIRS ? N : a.P), Chunk<T, VB>::pack(f + N));
-      }
+  for (int u = threadIdx.x; u < count; u += kRotThreads) {
+    if (u >= kRotThreads) load(u);
+    float4 ax = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (j >= a.turned) {
+      st_chunk<VB>(out, va);
+    } else {
+      const float2* const angle = turn + t * row + j * (N + S::kPad);
+      float f[2 * N], s[2 * N];
+      Chunk<T, VB>::unpack(va, f);
+      Chunk<T, VB>::unpack(vb, f + N);
       if (GPOS) {
-        // one token's vectors may take several passes over the same slots
-        const int slot = u & (kRotUnits - 1);
-#pragma unroll
-        for (int d = 0; d < kRotAxes; ++d)
-          sums[slot][d] = u < kRotUnits ? ax[d] : sums[slot][d] + ax[d];
+        Chunk<T, VB>::unpack(ia, s);
+        Chunk<T, VB>::unpack(ib, s + N);
       }
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float2 cs = angle[k];
+        const int x1 = PAIRS ? 2 * k : k, x2 = PAIRS ? 2 * k + 1 : k + N;
+        const float y1 = f[x1] * cs.x - f[x2] * cs.y, y2 = f[x2] * cs.x + f[x1] * cs.y;
+        f[x1] = y1;
+        f[x2] = y2;
+        if (GPOS) {
+          const float g = s[x1] * y2 - s[x2] * y1;
+          const float4 w = weight[j * (N + 1) + k];
+          ax.x += g * w.x;
+          ax.y += g * w.y;
+          ax.z += g * w.z;
+          ax.w += g * w.w;
+        }
+      }
+      st_chunk<VB>(out, Chunk<T, VB>::pack(f));
+      st_chunk<VB>(out + (PAIRS ? N : a.P), Chunk<T, VB>::pack(f + N));
+    }
+    if (GPOS) {
+      // one token's vectors may take several passes over the same slots
+      float4& slot = sums[u & (kRotUnits - 1)];
+      if (u >= kRotUnits) {
+        const float4 o = slot;
+        ax = make_float4(ax.x + o.x, ax.y + o.y, ax.z + o.z, ax.w + o.w);
+      }
+      slot = ax;
     }
   }
   if (GPOS) {
     __syncthreads();
-    // a warp per (token, axis), in the same order every time
+    // a warp per token, in the same order every time
     const int slots = min(per_token, kRotUnits);
-    for (int i = threadIdx.x >> 5; i < tokens * a.axes; i += kRotThreads / 32) {
-      const int t = i / a.axes, d = i - t * a.axes;
-      float g = 0.f;
-      for (int k = threadIdx.x & 31; k < slots; k += 32) g += sums[t * slots + k][d];
+    for (int k = threadIdx.x >> 5; k < tokens; k += kRotThreads / 32) {
+      float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = threadIdx.x & 31; i < slots; i += 32) {
+        const float4 o = sums[k * slots + i];
+        g = make_float4(g.x + o.x, g.y + o.y, g.z + o.z, g.w + o.w);
+      }
 #pragma unroll
-      for (int s = 16; s > 0; s >>= 1) g += __shfl_xor_sync(~0u, g, s);
-      if ((threadIdx.x & 31) == 0)
-        a.gpos[static_cast<int64_t>(token0 + t) * a.axes + d] = g;
+      for (int s = 16; s > 0; s >>= 1) {
+        g.x += __shfl_xor_sync(~0u, g.x, s);
+        g.y += __shfl_xor_sync(~0u, g.y, s);
+        g.z += __shfl_xor_sync(~0u, g.z, s);
+        g.w += __shfl_xor_sync(~0u, g.w, s);
+      }
+      const int d = threadIdx.x & 31;
+      if (d < a.axes)
+        a.gpos[static_cast<int64_t>(token0 + k) * a.axes + d] =
+            d == 0 ? g.x : d == 1 ? g.y : d == 2 ? g.z : g.w;
     }
   }
 }
 
 template <typename T, int VB>
 cudaError_t rotary_launch(const RotArgs& a, bool pairs, cudaStream_t st) {
+  using S = RotShared<Chunk<T, VB>::EPV>;
   const unsigned int grid = (a.total + a.tokens - 1) / a.tokens;
+  int bytes = S::turn_bytes(a.P, a.tokens);
   if (a.gpos != nullptr) {
-    if (pairs) rotary_kernel<T, VB, true, true><<<grid, kRotThreads, 0, st>>>(a);
-    else rotary_kernel<T, VB, false, true><<<grid, kRotThreads, 0, st>>>(a);
+    bytes += (S::weights(a.P) + std::min(a.tokens * a.heads * a.units, kRotUnits)) *
+             static_cast<int>(sizeof(float4));
+    auto* kernel = pairs ? rotary_kernel<T, VB, true, true> : rotary_kernel<T, VB, false, true>;
+    if (bytes > 48 << 10) {
+      const cudaError_t err =
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      if (err != cudaSuccess) return err;
+    }
+    kernel<<<grid, kRotThreads, bytes, st>>>(a);
   } else {
-    if (pairs) rotary_kernel<T, VB, true, false><<<grid, kRotThreads, 0, st>>>(a);
-    else rotary_kernel<T, VB, false, false><<<grid, kRotThreads, 0, st>>>(a);
+    auto* kernel = pairs ? rotary_kernel<T, VB, true, false> : rotary_kernel<T, VB, false, false>;
+    kernel<<<grid, kRotThreads, bytes, st>>>(a);
   }
   return cudaGetLastError();
 }
@@ -359,6 +418,17 @@ int msda_rotary(int dtype, int64_t batch, int64_t num_tokens, int64_t channels, 
   a.axis = axis_index;
   a.sign = inverse ? -1.f : 1.f;
   a.gpos = grad_positions;
+  a.hop = per_token <= kRotThreads && kRotThreads % per_token == 0
+              ? static_cast<int32_t>(kRotThreads / per_token) : 0;
+  a.flat = 1;
+  for (int i = 0; i < num_tensors; ++i) {
+    RotTensor& t = a.t[i];
+    t.xb -= num_tokens * t.xq;
+    t.yb -= num_tokens * t.yq;
+    t.ib -= num_tokens * t.iq;
+    if (batch > 1 && heads[i] > 0 && (t.xb != 0 || t.yb != 0 || (t.in != nullptr && t.ib != 0)))
+      a.flat = 0;
+  }
   cudaError_t err;
   if (dtype == MSDA_FLOAT32) err = rotary_dispatch<float>(a, static_cast<int>(vb), interleaved, st);
   else if (dtype == MSDA_FLOAT16)

@@ -1,0 +1,173 @@
+"""What pyramid_group_norm, rotary and AdamW do without a GPU: the binding
+loads beside the library, CPU tensors and bad arguments are refused, the C
+entries check their arguments on the host, and the helpers' tables are right."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import msda_triton_b200 as msda
+from msda_triton_b200 import _lib
+
+
+def test_binding_loads_and_names_exported_functions():
+    assert callable(_lib.binding().rotary)
+    assert set(_lib.BINDING_SYMBOLS) <= set(_lib.EXPORTED_SYMBOLS)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: msda.pyramid_group_norm(torch.zeros(1, 4, 8), [(2, 2)], 2),
+    lambda: msda.PyramidGroupNorm(2, 8)(torch.zeros(1, 4, 8), [(2, 2)]),
+    lambda: msda.rotary(torch.zeros(1, 4, 2, 8), torch.zeros(4, 2), *msda.axial_frequencies(8, 2)),
+    lambda: msda.AxialRotary(8, 2)(*[torch.zeros(1, 4, 2, 8)] * 2, torch.zeros(4, 2)),
+    lambda: msda.adamw_step([torch.zeros(3)], [torch.zeros(3)], {}, step=1),
+    lambda: msda.adamw_state([torch.zeros(3)]),
+])
+def test_cpu_tensors_are_refused(call):
+    with pytest.raises(ValueError, match="requires CUDA tensors"):
+        call()
+
+
+def test_frequencies():
+    freq, axis = msda.axial_frequencies(16, 3, theta=64.0)
+    assert axis.tolist() == [0, 1, 2, 0, 1, 2, 0, 1]
+    # 3, 3 and 2 pairs: each axis falls from 1 towards 1 / theta
+    want = [64.0 ** -(i / n) for i, n in ((0, 3), (0, 3), (0, 2), (1, 3), (1, 3), (1, 2), (2, 3), (2, 3))]
+    torch.testing.assert_close(freq, torch.tensor(want))
+    freq, axis = msda.axial_frequencies(12, 2, sections=(4, 2))
+    assert axis.tolist() == [0, 0, 0, 0, 1, 1] and freq[0] == freq[4] == 1
+    assert msda.axial_frequencies(0, 1)[0].numel() == 0
+    for bad in ((5, 2), (8, 0), (8, 5)):
+        with pytest.raises(ValueError):
+            msda.axial_frequencies(*bad)
+    with pytest.raises(ValueError, match="sections"):
+        msda.axial_frequencies(8, 2, sections=(3, 2))
+    with pytest.raises(ValueError, match="exceeds"):
+        msda.AxialRotary(8, 2, rotated=10)
+
+
+def test_pyramid_positions():
+    pos = msda.pyramid_positions([(4, 6), (2, 3)])
+    assert pos.shape == (1, 30, 2)
+    assert pos[0, 7].tolist() == [1.0, 1.0]  # (x, y) of cell (1, 1)
+    assert pos[0, 24].tolist() == [0.5, 0.5]  # the centre of the first four cells
+    assert pos[0, 29].tolist() == [4.5, 2.5]
+    assert msda.pyramid_positions([(2, 3, 4)])[0, 23].tolist() == [3.0, 2.0, 1.0]
+
+
+def test_modules_hold_their_parameters():
+    m = msda.PyramidGroupNorm(4, 32, num_levels=3)
+    assert m.weight.shape == m.bias.shape == (3, 32)
+    assert not list(msda.PyramidGroupNorm(4, 32, affine=False).parameters())
+    with pytest.raises(ValueError, match="multiple"):
+        msda.PyramidGroupNorm(3, 32)
+    with pytest.raises(ValueError, match="activation"):
+        msda.PyramidGroupNorm(4, 32, activation="tanh")
+    r = msda.AxialRotary(32, 3).half()
+    assert r.inv_freq.dtype == torch.float32 and not r.state_dict()
+
+
+def _rows(*n):
+    return np.array(n, dtype=np.int64)
+
+
+def test_norm_workspace_is_a_function_of_sizes():
+    lib = _lib.lib()
+    ws = lambda dt, B, C, G, rows, bwd: lib.msda_group_norm_workspace_bytes(  # noqa: E731
+        dt, B, C, G, len(rows), rows.ctypes.data, bwd)
+    small, large = _rows(100, 25), _rows(64 * 128 * 128)
+    assert 0 < ws(_lib.BFLOAT16, 2, 256, 32, small, 0) < ws(_lib.BFLOAT16, 2, 256, 32, small, 1)
+    # the 3D xl level: below 5 % of its features
+    assert ws(_lib.BFLOAT16, 1, 256, 32, large, 1) < 0.05 * large[0] * 256 * 2
+    assert ws(_lib.BFLOAT16, 2, 256, 33, small, 0) == 0
+    assert ws(9, 2, 256, 32, small, 0) == 0
+    assert ws(_lib.FLOAT32, 2, 256, 32, _rows(-1), 0) == 0
+
+
+def test_norm_entry_checks():
+    lib = _lib.lib()
+    buf = np.zeros(4096, dtype=np.float32)
+    at = (buf.ctypes.data + 255) // 256 * 256
+    rows, strides = _rows(4), _rows(32, 8)
+    x = (ctypes.c_void_p * 1)(at)
+
+    def call(dtype=_lib.FLOAT32, C=8, G=2, L=1, rows=rows.ctypes.data, x=x, affine=_lib.FLOAT32,
+             eps=1e-5, act=0, y=at, stats=at, ws=at, ws_bytes=1 << 20):
+        return lib.msda_group_norm_fwd(dtype, 1, C, G, L, rows, x, strides.ctypes.data, None, None,
+                                       affine, 0, eps, act, y, stats, ws, ws_bytes, None)
+
+    assert call(dtype=7) == _lib.ERROR_UNSUPPORTED_DTYPE
+    assert call(affine=7) == _lib.ERROR_UNSUPPORTED_DTYPE
+    assert call(G=3) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(act=9) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(eps=-1.0) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(L=17) == _lib.ERROR_TOO_MANY_LEVELS
+    assert call(rows=None) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(x=None) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(x=(ctypes.c_void_p * 1)(at + 1)) == _lib.ERROR_MISALIGNED
+    assert call(stats=None) == _lib.ERROR_MISALIGNED
+    assert call(ws=at + 4) == _lib.ERROR_WORKSPACE
+    assert call(ws_bytes=0) == _lib.ERROR_WORKSPACE
+    assert "workspace" in _lib.last_error()
+    assert call(rows=_rows(1 << 31).ctypes.data) == _lib.ERROR_INT32_OVERFLOW
+
+
+def test_rotary_entry_checks():
+    lib = _lib.lib()
+    buf = np.zeros(4096, dtype=np.float32)
+    at = (buf.ctypes.data + 255) // 256 * 256
+    heads, strides = _rows(2), _rows(64, 16, 8)
+
+    def call(dtype=_lib.FLOAT32, Q=4, C=8, tensors=1, x=at, pos=at, pos_dtype=0, axes=2, freq=at,
+             pairs=4, gpos=None):
+        table = (ctypes.c_void_p * 1)(x)
+        return lib.msda_rotary(dtype, 1, Q, C, tensors, heads.ctypes.data, table,
+                               strides.ctypes.data, table, strides.ctypes.data, pos, pos_dtype, 0,
+                               axes, freq, freq, pairs, 0, 0, None, None, gpos, None)
+
+    assert call(dtype=5) == _lib.ERROR_UNSUPPORTED_DTYPE
+    assert call(pos_dtype=5) == _lib.ERROR_UNSUPPORTED_DTYPE
+    assert call(tensors=3) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(axes=5) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(pairs=5) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(Q=-1) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(Q=1 << 31) == _lib.ERROR_INT32_OVERFLOW
+    assert call(pos=None) == _lib.ERROR_MISALIGNED
+    assert call(freq=None) == _lib.ERROR_MISALIGNED
+    assert call(x=at + 2) == _lib.ERROR_MISALIGNED
+    assert call(gpos=at) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(Q=0, x=None, pos=None) == _lib.SUCCESS
+
+
+def test_adamw_entry_checks():
+    lib = _lib.lib()
+    buf = np.zeros(4096, dtype=np.float32)
+    at = (buf.ctypes.data + 255) // 256 * 256
+    counts, steps = _rows(100), _rows(1)
+
+    def call(dtype=_lib.FLOAT32, bits=32, p=at, g=at, counts=counts, steps=steps, lr=1e-3, b1=0.9,
+             m=at, me=None, master=None, elements=128):
+        return lib.msda_adamw_step(dtype, bits, 1, (ctypes.c_void_p * 1)(p), (ctypes.c_void_p * 1)(g),
+                                   counts.ctypes.data, steps.ctypes.data, lr, b1, 0.999, 1e-8, 0.0,
+                                   0, None, m, at, me, me, master, elements, None)
+
+    assert call(dtype=5) == _lib.ERROR_UNSUPPORTED_DTYPE
+    assert call(bits=16) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(lr=float("nan")) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(b1=1.0) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(counts=_rows(-1)) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(steps=_rows(0)) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(master=at) == _lib.ERROR_INVALID_ARGUMENT
+    assert call(p=at + 2) == _lib.ERROR_MISALIGNED
+    assert call(m=at + 4) == _lib.ERROR_MISALIGNED
+    assert call(bits=8, me=None) == _lib.ERROR_MISALIGNED
+    assert call(elements=127) == _lib.ERROR_SHAPE_MISMATCH
+    assert call(counts=_rows(0), p=None, g=None, elements=0) == _lib.SUCCESS
+    assert lib.msda_adamw_values(None, None, None, None, 100, None, None, None) == \
+        _lib.ERROR_INVALID_ARGUMENT
+    assert lib.msda_adamw_values(None, None, None, None, 128, None, None, None) == \
+        _lib.ERROR_MISALIGNED
