@@ -9,6 +9,7 @@
 // The functions come from the library that _lib.py has loaded, by address.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/python.h>
@@ -79,7 +80,7 @@ void* current_stream(const Tensor& t) {
 void* ptr(const optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
 
 Tensor empty(at::IntArrayRef shape, const Tensor& like, at::ScalarType dtype) {
-  return at::empty(shape, like.options().dtype(dtype).memory_format(at::MemoryFormat::Contiguous));
+  return at::detail::empty_cuda(shape, dtype, like.device(), at::MemoryFormat::Contiguous);
 }
 Tensor empty(at::IntArrayRef shape, const Tensor& like) {
   return empty(shape, like, like.scalar_type());

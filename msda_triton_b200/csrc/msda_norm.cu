@@ -8,12 +8,15 @@
 namespace msda {
 namespace {
 
-// Row pieces that a slab takes (of 64 bytes, DRAM was read in 128: 336 MB a
-// pass where 200 were wanted), and bytes of x in a tile: at most the first, as
-// little as the second where there would be fewer than kManyTiles.
-constexpr int64_t kPiece = 256;
-constexpr int64_t kTile = 128 << 10, kDirectTile = 64 << 10, kSmallTile = 8 << 10;
-constexpr int64_t kManyTiles = 148 * 4;
+constexpr int64_t kSMs = 148;
+// Row pieces that a slab takes, direct or not (of 64 bytes, DRAM was read in
+// 128: 336 MB a pass where 200 were wanted).
+constexpr int64_t kDirectPiece = 128, kPiece = 256;
+// Bytes of x in a tile.  Direct: as many tiles as CTAs run at once, nearly (of
+// the 2D encoder's 41 MB, 632 tiles where 592 run took 32 us forward, 556 take
+// 27), but no fewer bytes than the first.  Else the third, or the second where
+// there would be few tiles.
+constexpr int64_t kSmallTile = 16 << 10, kMediumTile = 64 << 10, kTile = 128 << 10;
 // Direct: at most so many tiles a unit, and (for the affine map's gradients) in
 // all batch entries' and levels' units of a slab.
 constexpr int64_t kDirectTiles = 64, kDirectSum = 2048;
@@ -45,9 +48,11 @@ int make_plan(int dtype, int64_t B, int64_t C, int64_t G, int64_t L, const int64
   }
   for (int attempt = 0; attempt < 2; ++attempt) {
     p.direct = attempt == 0;
-    const int64_t tile = std::min(p.direct ? kDirectTile : kTile,
-                                  std::max(total / kManyTiles, p.direct ? kSmallTile : kDirectTile));
-    sg = std::min(G, std::max<int64_t>(1, std::min(ceil_div(kPiece, cg * es), kNormMaxSlab / cg)));
+    const int64_t at_once = kSMs * (backward ? 3 : 4);
+    const int64_t tile = p.direct ? std::max(kSmallTile, total * 12 / (11 * at_once))
+                                  : std::min(kTile, std::max(total / at_once, kMediumTile));
+    const int64_t piece = p.direct ? kDirectPiece : kPiece;
+    sg = std::min(G, std::max<int64_t>(1, std::min(ceil_div(piece, cg * es), kNormMaxSlab / cg)));
     p.tiles = p.counters = 0;
     int64_t most = 0, sum = 0;
     for (int64_t l = 0; l < L; ++l) {
@@ -68,7 +73,7 @@ int make_plan(int dtype, int64_t B, int64_t C, int64_t G, int64_t L, const int64
       if (p.counters > (1 << 29) || p.tiles > (1 << 29))
         return report(MSDA_ERROR_INT32_OVERFLOW, "too many tiles of work");
     }
-    if (p.direct && most <= kDirectTiles && (!backward || sum <= kDirectSum)) break;
+    if (p.direct && tile <= kTile && most <= kDirectTiles && (!backward || sum <= kDirectSum)) break;
   }
   p.partial_stride = static_cast<int32_t>(sg * (backward ? cg : 1));
   int64_t at = 0;

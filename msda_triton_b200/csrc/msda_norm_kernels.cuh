@@ -420,12 +420,39 @@ __device__ void norm_apply(const NormArgs& a, const NormTile& t) {
 }
 
 // ------------------------------------------------------------------ backward
+// Rows of the sums' pass that a thread has on their way, in shared memory that
+// it alone uses.  Two rows in registers kept 49 KB an SM in flight, which is
+// 4.3 TB/s; registers for more would cost a CTA.
+constexpr int kNormStages = 5;
+
+__device__ __forceinline__ void norm_copy(void* shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(shared))),
+               "l"(global)
+               : "memory");
+}
+__device__ __forceinline__ Raw<16> norm_staged(const char* shared) {
+  const uint4 v = *reinterpret_cast<const uint4*>(shared);
+  Raw<16> r;
+  r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+  return r;
+}
+__device__ __forceinline__ void norm_copies_end() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void norm_copies_wait() {  // for all but the last kNormStages - 2
+  asm volatile("cp.async.wait_group %0;" ::"n"(kNormStages - 2) : "memory");
+}
+
 // Sums s1, s2 per channel of one tile, and the groups' coefficients a, q of the unit.
 template <typename T, int VB, int ACT, bool DIRECT, int U>
 __device__ void norm_grad_stats(const NormArgs& a, const NormTile& t) {
   using P = Pairs<T, VB>;
   constexpr int EPV = P::EPV;
-  __shared__ float2 part[kNormThreads * EPV];
+  constexpr bool kStaged = VB == 16;
+  __shared__ __align__(16) char space[kStaged ? kNormStages * 2 * kNormThreads * 16
+                                              : kNormThreads * EPV * 8];
+  float2* const part = reinterpret_cast<float2*>(space);
   const NormLevel& v = a.lv[t.l];
   const NormThread me(a, t);
   const int64_t hop = t.trows * v.x_row, ghop = t.trows * v.gy_row;
@@ -435,6 +462,7 @@ __device__ void norm_grad_stats(const NormArgs& a, const NormTile& t) {
     uint64_t s1[P::N], s2[P::N];
 #pragma unroll
     for (int i = 0; i < P::N; ++i) s1[i] = s2[i] = 0;  // two zeros
+    if (kStaged && col0 > 0) __syncthreads();  // the sums before are read
     if (col < t.nvc) {
       const int c0 = t.g0 * a.cg + col * EPV;
       const NormCentre<T> centre(__ldg(a.stats + me.segment * a.G + c0 / a.cg));
@@ -451,31 +479,59 @@ __device__ void norm_grad_stats(const NormArgs& a, const NormTile& t) {
           reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row + c0;
       const T* g =
           reinterpret_cast<const T*>(v.gy) + v.gy_batch * t.b + (t.row0 + me.tr) * v.gy_row + c0;
-      norm_rows<U>(t, me.tr, [&](auto count) {
-        constexpr int K = decltype(count)::value;
-        Raw<VB> rx[K], rg[K];
+      auto add = [&](const Raw<VB>& rx, const Raw<VB>& rg) {
+        uint64_t f[P::N], e[P::N];
+        P::unpack(rx, f);
+        P::unpack(rg, e);
 #pragma unroll
-        for (int u = 0; u < K; ++u) {
-          rx[u] = ld_chunk<VB>(p + u * hop);
-          rg[u] = ld_chunk<VB>(g + u * ghop);
+        for (int i = 0; i < P::N; ++i) {
+          const uint64_t h = centre(f[i]);
+          const uint64_t dz =
+              ACT == MSDA_ACT_NONE ? e[i] : mul2(e[i], norm_dact<ACT>(fma2(h, w[i], d[i])));
+          s1[i] = add2(s1[i], dz);
+          s2[i] = fma2(dz, h, s2[i]);
         }
-        p += K * hop;
-        g += K * ghop;
-#pragma unroll
-        for (int u = 0; u < K; ++u) {
-          uint64_t f[P::N], e[P::N];
-          P::unpack(rx[u], f);
-          P::unpack(rg[u], e);
-#pragma unroll
-          for (int i = 0; i < P::N; ++i) {
-            const uint64_t h = centre(f[i]);
-            const uint64_t dz =
-                ACT == MSDA_ACT_NONE ? e[i] : mul2(e[i], norm_dact<ACT>(fma2(h, w[i], d[i])));
-            s1[i] = add2(s1[i], dz);
-            s2[i] = fma2(dz, h, s2[i]);
+      };
+      if constexpr (kStaged) {
+        constexpr int kStage = 2 * kNormThreads * 16;
+        char* const slot = space + threadIdx.x * 16;
+        int ahead = me.tr;  // the row to copy next
+        auto copy = [&](int stage) {
+          if (ahead < t.rows) {
+            norm_copy(slot + stage * kStage, p);
+            norm_copy(slot + stage * kStage + kStage / 2, g);
+            p += hop;
+            g += ghop;
+            ahead += t.trows;
           }
+          norm_copies_end();
+        };
+#pragma unroll
+        for (int i = 0; i < kNormStages - 1; ++i) copy(i);
+        int stage = 0;
+        for (int r = me.tr; r < t.rows; r += t.trows) {
+          norm_copies_wait();
+          const Raw<16> rx = norm_staged(slot + stage * kStage);
+          const Raw<16> rg = norm_staged(slot + stage * kStage + kStage / 2);
+          copy(stage == 0 ? kNormStages - 1 : stage - 1);
+          stage = stage == kNormStages - 1 ? 0 : stage + 1;
+          add(rx, rg);
         }
-      });
+      } else {
+        norm_rows<U>(t, me.tr, [&](auto count) {
+          constexpr int K = decltype(count)::value;
+          Raw<VB> rx[K], rg[K];
+#pragma unroll
+          for (int u = 0; u < K; ++u) {
+            rx[u] = ld_chunk<VB>(p + u * hop);
+            rg[u] = ld_chunk<VB>(g + u * ghop);
+          }
+          p += K * hop;
+          g += K * ghop;
+#pragma unroll
+          for (int u = 0; u < K; ++u) add(rx[u], rg[u]);
+        });
+      }
     }
     __syncthreads();
 #pragma unroll
