@@ -425,17 +425,21 @@ __device__ void norm_apply(const NormArgs& a, const NormTile& t) {
 // 4.3 TB/s; registers for more would cost a CTA.
 constexpr int kNormStages = 5;
 
-__device__ __forceinline__ void norm_copy(void* shared, const void* global) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                   static_cast<uint32_t>(__cvta_generic_to_shared(shared))),
-               "l"(global)
+template <int AT> __device__ __forceinline__ void norm_copy(uint32_t shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1], 16;" ::"r"(shared), "l"(global), "n"(AT)
                : "memory");
 }
-__device__ __forceinline__ Raw<16> norm_staged(const char* shared) {
-  const uint4 v = *reinterpret_cast<const uint4*>(shared);
+template <int AT> __device__ __forceinline__ Raw<16> norm_staged(uint32_t shared) {
   Raw<16> r;
-  r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];"
+               : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
+               : "r"(shared), "n"(AT) : "memory");
   return r;
+}
+// f(Count<0>) ... f(Count<N - 1>) until one returns false.
+template <int I, int N, typename F> __device__ __forceinline__ bool norm_each(F f) {
+  if constexpr (I == N) return true;
+  else return f(Count<I>{}) && norm_each<I + 1, N>(f);
 }
 __device__ __forceinline__ void norm_copies_end() {
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -494,28 +498,33 @@ __device__ void norm_grad_stats(const NormArgs& a, const NormTile& t) {
       };
       if constexpr (kStaged) {
         constexpr int kStage = 2 * kNormThreads * 16;
-        char* const slot = space + threadIdx.x * 16;
-        int ahead = me.tr;  // the row to copy next
-        auto copy = [&](int stage) {
+        const uint32_t slot =
+            static_cast<uint32_t>(__cvta_generic_to_shared(space)) + threadIdx.x * 16;
+        int ahead = me.tr, r = me.tr;  // the rows to copy and to add next
+        auto copy = [&](auto stage) {
+          constexpr int kAt = decltype(stage)::value * kStage;
           if (ahead < t.rows) {
-            norm_copy(slot + stage * kStage, p);
-            norm_copy(slot + stage * kStage + kStage / 2, g);
+            norm_copy<kAt>(slot, p);
+            norm_copy<kAt + kStage / 2>(slot, g);
             p += hop;
             g += ghop;
             ahead += t.trows;
           }
           norm_copies_end();
+          return true;
         };
-#pragma unroll
-        for (int i = 0; i < kNormStages - 1; ++i) copy(i);
-        int stage = 0;
-        for (int r = me.tr; r < t.rows; r += t.trows) {
+        norm_each<0, kNormStages - 1>(copy);
+        while (norm_each<0, kNormStages>([&](auto stage) {
+          constexpr int kNow = decltype(stage)::value;
+          if (r >= t.rows) return false;
           norm_copies_wait();
-          const Raw<16> rx = norm_staged(slot + stage * kStage);
-          const Raw<16> rg = norm_staged(slot + stage * kStage + kStage / 2);
-          copy(stage == 0 ? kNormStages - 1 : stage - 1);
-          stage = stage == kNormStages - 1 ? 0 : stage + 1;
+          const Raw<16> rx = norm_staged<kNow * kStage>(slot);
+          const Raw<16> rg = norm_staged<kNow * kStage + kStage / 2>(slot);
+          copy(Count<(kNow + kNormStages - 1) % kNormStages>{});
           add(rx, rg);
+          r += t.trows;
+          return true;
+        })) {
         }
       } else {
         norm_rows<U>(t, me.tr, [&](auto count) {
