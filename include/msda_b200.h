@@ -364,7 +364,7 @@ MSDA_API int msda_group_norm_bwd(int dtype, int64_t batch, int64_t channels, int
  *                      position_batch elements between batch entries (0: one
  *                      set for all); integers are exact up to 2^24
  *   inv_freq           (num_pairs) fp32;  axis_index (num_pairs) int32 in
- *                      [0, num_axes), not checked
+ *                      [0, num_axes): a pair of another axis becomes NaN
  *   grad_positions     NULL, or (batch, num_tokens, num_axes) fp32 for the
  *                      positions' gradient (with `inverse`); `inputs` then
  *                      holds the forward's inputs and their strides */

@@ -12,6 +12,8 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/python.h>
 
 #include <array>
@@ -89,6 +91,16 @@ Tensor empty(at::IntArrayRef shape, const Tensor& like) {
 const Tensor& tensor_of(PyObject* o, const char* what) {
   TORCH_CHECK_TYPE(THPVariable_Check(o), what, " must be tensors, got ", Py_TYPE(o)->tp_name);
   return THPVariable_Unpack(o);
+}
+
+// The gradients of a backward have none themselves: under create_graph they
+// say so where they are differentiated, instead of passing for constants.
+void once_differentiable(const variable_list& grads, variable_list& out) {
+  if (!at::GradMode::is_enabled()) return;
+  auto node = std::make_shared<torch::autograd::Error>(
+      "this operator's backward has no derivative", torch::autograd::collect_next_edges(grads));
+  for (Tensor& t : out)
+    if (t.defined()) torch::autograd::set_history(t, node);
 }
 
 // ------------------------------------------------------------------ group norm
@@ -350,6 +362,7 @@ class PyramidGroupNormFn : public torch::autograd::Function<PyramidGroupNormFn> 
                  static_cast<int>(ctx->saved_data["activation"].toInt())};
     auto some = [](const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; };
     variable_list out = norm_backward(n, saved, some(weight), some(bias), stats, grads[0]);
+    once_differentiable(grads, out);
     out.push_back(Tensor());  // the sizes
     return out;
   }
@@ -533,6 +546,7 @@ class RotaryFn : public torch::autograd::Function<RotaryFn> {
     const at::TensorList inputs = at::TensorList(saved).slice(3);
     variable_list out = rotary_backward(grads, inputs, saved[0], saved[1], saved[2],
                                         ctx->saved_data["interleaved"].toBool());
+    once_differentiable(grads, out);
     if (inputs.empty()) out.push_back(Tensor());  // the positions
     out.insert(out.end(), 3, Tensor());           // inv_freq, axis_index, interleaved
     return out;

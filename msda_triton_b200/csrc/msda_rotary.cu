@@ -194,8 +194,10 @@ rotary_kernel(const __grid_constant__ RotArgs a) {
   for (int i = threadIdx.x; i < tokens * a.P; i += kRotThreads) {
     const int k = a.dpair(i), p = i - k * a.P;
     const uint32_t n = token0 + k, b = a.dq(n), q = n - b * a.dq.d;
-    const float x = rot_position(a, b * a.pos_batch + static_cast<int64_t>(q) * a.axes +
-                                        __ldg(a.axis + p));
+    const int on = __ldg(a.axis + p);
+    const float x = static_cast<unsigned int>(on) < static_cast<unsigned int>(a.axes)
+                        ? rot_position(a, b * a.pos_batch + static_cast<int64_t>(q) * a.axes + on)
+                        : __uint_as_float(0x7fc00000u);  // no such axis
     turn[k * row + p + p / N * S::kPad] = rot_angle(x, __ldg(a.inv_freq + p), a.sign);
   }
   if (GPOS)

@@ -186,6 +186,10 @@ class AdamW(torch.optim.Optimizer):
         self._parts: list[list[_Part]] = []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed,
+                "master_weights": self.master_weights, "_parts": self._parts}
+
     def _allocate(self) -> None:
         """States for groups that have none yet (the first step, or a group added later)."""
         for group in self.param_groups[len(self._parts):]:

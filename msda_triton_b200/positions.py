@@ -83,8 +83,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
         positions: (Q, A) or (1 or B, Q, A), A = 1 to 4 axes; fp32, or integers
             (exact up to 2^24); other floating types are converted to fp32.
         inv_freq: (pairs,) fp32 angle per unit of position.
-        axis_index: (pairs,) int32, each in [0, A) (not checked: it stays on the
-            device).
+        axis_index: (pairs,) int32, each in [0, A); it stays on the device, so
+            a pair with another index is no error but becomes NaN.
         interleaved: pairs are channels (2j, 2j + 1) instead of (j, j + pairs).
 
     Returns:

@@ -429,6 +429,19 @@ def test_group_added_later_and_closure():
     assert not torch.equal(before, net[2].weight)
 
 
+def test_copies_with_its_model():
+    net = model()
+    opt = msda.AdamW(net.parameters(), lr=1e-2, state_bits=8)
+    train(net, opt, 2)
+    net2, opt2 = copy.deepcopy((net, opt))
+    train(net, opt, 2, 2)
+    train(net2, opt2, 2, 2)
+    for p, q in zip(net.parameters(), net2.parameters()):
+        assert p is not q and torch.equal(p, q)
+    assert all(a.data_ptr() != b.data_ptr() for a, b in
+               zip(opt._parts[0][0].state.values(), opt2._parts[0][0].state.values()))
+
+
 def test_autograd_sees_the_change():
     p = torch.ones(4, device=DEV, requires_grad=True)
     out = (p * p).sum()

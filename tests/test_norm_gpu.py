@@ -269,6 +269,16 @@ def test_gradient_against_differences(activation):
         assert abs(float(slope - (grad.double() * d).sum())) < 0.02 * float(grad.norm())
 
 
+def test_no_second_derivative():
+    x = features(1, [6], 8, torch.float32).requires_grad_(True)
+    g = torch.ones(1, 6, 8, device=DEV, requires_grad=True)
+    (gx,) = torch.autograd.grad(msda.pyramid_group_norm(x, [(6,)], 2), x, g, create_graph=True)
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.autograd.grad(gx.sum(), g)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(gx.square().sum(), x)
+
+
 def test_module_stream_and_graph():
     """On a stream of its own, and captured in a CUDA graph: the same bits as by itself."""
     rows = [900, 200]

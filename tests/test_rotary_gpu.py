@@ -186,6 +186,25 @@ def test_positions_that_are_not_finite_stay_with_their_token():
     assert bool(y[hit].isnan().all()) and torch.equal(y[~hit], clean[~hit])
 
 
+def test_pairs_of_no_axis_become_nan():
+    (x,), pos, freq, axis = make(2, 9, (3,), 16, torch.float32)
+    axis = axis.clone()
+    axis[2], axis[5] = 2, -1
+    y = msda.rotary(x, pos, freq, axis)
+    lost = torch.zeros(16, dtype=torch.bool, device=DEV)
+    lost[[2, 5, 10, 13]] = True
+    assert bool(y[..., lost].isnan().all()) and bool(y[..., ~lost].isfinite().all())
+
+
+def test_no_second_derivative():
+    (x,), pos, freq, axis = make(1, 4, (2,), 8, torch.float32)
+    x.requires_grad_(True)
+    g = torch.ones(1, 4, 2, 8, device=DEV, requires_grad=True)
+    (gx,) = torch.autograd.grad(msda.rotary(x, pos, freq, axis), x, g, create_graph=True)
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.autograd.grad(gx.sum(), g)
+
+
 def test_zero_is_no_turn_and_lengths_stay():
     xs, pos, freq, axis = make(2, 20, (4,), 32, torch.float32)
     assert torch.equal(msda.rotary(xs[0], torch.zeros_like(pos), freq, axis), xs[0])
