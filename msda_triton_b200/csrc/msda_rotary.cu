@@ -126,13 +126,16 @@ template <int N> struct RotShared {
   }
 };
 
-// A thread has one vector (two, of both halves) in flight; six CTAs an SM (five with
-// interleaved pairs, which take more registers) were
+// A thread has one vector (two, of both halves) in flight; six CTAs an SM were
 // faster than three with four each (759 us against 925 for 4.9 GB, 6.5 TB/s).
 template <typename T, int VB, bool PAIRS, bool GPOS>
-__global__ void __launch_bounds__(kRotThreads, GPOS ? 4 : PAIRS ? 5 : 6)
+__global__ void __launch_bounds__(kRotThreads, GPOS ? 4 : 6)
 rotary_kernel(const __grid_constant__ RotArgs a) {
-  constexpr int N = Chunk<T, VB>::EPV;  // pairs per turned vector
+  constexpr int N = Chunk<T, VB>::EPV;  // pairs that a thread turns at a time
+  // It loads vectors j of the turned channels' two halves.  They hold N pairs
+  // in either order of channels, but for single interleaved elements, which are
+  // a pair side by side.
+  constexpr bool kAdjacent = PAIRS && N == 1;
   using S = RotShared<N>;
   extern __shared__ __align__(16) char shared[];
   const int token0 = blockIdx.x * a.tokens;
@@ -160,8 +163,8 @@ rotary_kernel(const __grid_constant__ RotArgs a) {
       second = h >= a.heads0;
       const RotTensor& x = a.t[second];
       if (second) h -= a.heads0;
-      int c = PAIRS ? 2 * N * j : N * j;
-      gap = PAIRS ? N : a.P;
+      int c = kAdjacent ? 2 * j : N * j;
+      gap = kAdjacent ? 1 : a.P;
       if (j >= a.turned) {
         c = 2 * a.P + (j - a.turned) * N;
         gap = 0;
@@ -215,7 +218,13 @@ rotary_kernel(const __grid_constant__ RotArgs a) {
     if (j >= a.turned) {
       st_chunk<VB>(out, va);
     } else {
-      const float2* const angle = turn + t * row + j * (N + S::kPad);
+      // the first of N pairs, or of N / 2 in each half
+      constexpr bool kSplit = PAIRS && N > 1;
+      const int j2 = a.turned + j;
+      const float2* const angle =
+          turn + t * row + (kSplit ? j * N / 2 + j / 2 * S::kPad : j * (N + S::kPad));
+      const float2* const angle2 = turn + t * row + j2 * N / 2 + j2 / 2 * S::kPad;
+      const int w1 = kSplit ? j * N / 2 + j / 2 : j * (N + 1), w2 = j2 * N / 2 + j2 / 2;
       float f[2 * N], s[2 * N];
       Chunk<T, VB>::unpack(va, f);
       Chunk<T, VB>::unpack(vb, f + N);
@@ -225,14 +234,16 @@ rotary_kernel(const __grid_constant__ RotArgs a) {
       }
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const float2 cs = angle[k];
-        const int x1 = PAIRS ? 2 * k : k, x2 = PAIRS ? 2 * k + 1 : k + N;
+        const bool upper = kSplit && k >= N / 2;
+        const int kk = upper ? k - N / 2 : k;
+        const float2 cs = upper ? angle2[kk] : angle[kk];
+        const int x1 = kSplit ? 2 * k : k, x2 = kSplit ? 2 * k + 1 : k + N;
         const float y1 = f[x1] * cs.x - f[x2] * cs.y, y2 = f[x2] * cs.x + f[x1] * cs.y;
         f[x1] = y1;
         f[x2] = y2;
         if (GPOS) {
           const float g = s[x1] * y2 - s[x2] * y1;
-          const float4 w = weight[j * (N + 1) + k];
+          const float4 w = weight[(upper ? w2 : w1) + kk];
           ax.x += g * w.x;
           ax.y += g * w.y;
           ax.z += g * w.z;
@@ -240,7 +251,7 @@ rotary_kernel(const __grid_constant__ RotArgs a) {
         }
       }
       st_chunk<VB>(out, Chunk<T, VB>::pack(f));
-      st_chunk<VB>(out + (PAIRS ? N : a.P), Chunk<T, VB>::pack(f + N));
+      st_chunk<VB>(out + (kAdjacent ? 1 : a.P), Chunk<T, VB>::pack(f + N));
     }
     if (GPOS) {
       // one token's vectors may take several passes over the same slots
