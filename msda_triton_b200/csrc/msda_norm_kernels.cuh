@@ -421,9 +421,11 @@ __device__ void norm_apply(const NormArgs& a, const NormTile& t) {
 
 // ------------------------------------------------------------------ backward
 // Rows of the sums' pass that a thread has on their way, in shared memory that
-// it alone uses.  Two rows in registers kept 49 KB an SM in flight, which is
-// 4.3 TB/s; registers for more would cost a CTA.
-constexpr int kNormStages = 5;
+// it alone uses.  Two rows in registers, at three CTAs an SM, kept 49 KB in
+// flight (566 us for the 2.45 GB of two 3D xl pyramids); this way four CTAs
+// fit, with 96 KB: 418 us, 5.9 TB/s.  Then issue is the bound (16 instructions
+// an element with SiLU).
+constexpr int kNormStages = 4;
 
 template <int AT> __device__ __forceinline__ void norm_copy(uint32_t shared, const void* global) {
   asm volatile("cp.async.cg.shared.global [%0 + %2], [%1], 16;" ::"r"(shared), "l"(global), "n"(AT)
@@ -757,9 +759,11 @@ __device__ void norm_grad_apply(const NormArgs& a, const NormTile& t) {
 
 // ------------------------------------------------------------------ the launches
 // CTAs per SM and vectors in flight per thread: of the combinations that were
-// timed (3 to 6 CTAs, 2 to 8 vectors) the fastest.
+// timed (3 to 6 CTAs, 2 to 8 vectors) the fastest.  Two 3D xl pyramids, 1.23 GB
+// of bf16 with SiLU: statistics 202 us (6.1 TB/s) and application 382 us
+// (6.4 TB/s) forward, 418 us (5.9) and 585 us (6.3) backward.
 template <typename T, int VB, int ACT, bool BWD, bool DIRECT>
-__global__ void __launch_bounds__(kNormThreads, BWD ? 3 : 4)
+__global__ void __launch_bounds__(kNormThreads, 4)
 norm_stats_kernel(const __grid_constant__ NormArgs a) {
   norm_let_next_start();
   const NormTile t = norm_tile<Chunk<T, VB>::EPV>(a, blockIdx.x);
