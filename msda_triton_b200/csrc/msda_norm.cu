@@ -17,6 +17,8 @@ constexpr int64_t kDirectPiece = 128, kPiece = 256;
 // 27), but no fewer bytes than the first.  Else the third, or the second where
 // there would be few tiles.
 constexpr int64_t kSmallTile = 16 << 10, kMediumTile = 64 << 10, kTile = 128 << 10;
+// The one launch: the narrowest piece of a row, and from where on whole lines.
+constexpr int64_t kOncePiece = 32, kOnceMuch = 32 << 20;
 // Direct: at most so many tiles a unit, and (for the affine map's gradients) in
 // all batch entries' and levels' units of a slab.
 constexpr int64_t kDirectTiles = 64, kDirectSum = 2048;
@@ -180,18 +182,51 @@ int check_common(const Plan& p, int64_t L, int64_t es, const void* weight, const
   return MSDA_SUCCESS;
 }
 
-// Zeroes what starts as zeros, then both launches.
-cudaError_t run(const NormArgs& a, const Plan& p, int dtype, int act, bool backward,
-                void* workspace, cudaStream_t st) {
-  if (p.zero_bytes > 0) {
+// The one launch's units, if a CTA's registers hold each: as wide pieces of
+// rows as that allows, down to kOncePiece, or to whole lines where much is read.
+bool make_once(NormArgs& a, int vb, int64_t es) {
+  const int64_t epv = vb / es;
+  int64_t total = 0, tiles = 0;
+  for (int l = 0; l < a.L; ++l) total += a.B * a.lv[l].rows * a.C * es;
+  const int64_t least = total > kOnceMuch ? kDirectPiece : kOncePiece;
+  NormLevel lv[kMaxLevels];
+  for (int l = 0; l < a.L; ++l) {
+    NormLevel& v = lv[l] = a.lv[l];
+    int64_t groups = std::min<int64_t>(
+        {a.G, kNormMaxSlab, std::max<int64_t>(1, kDirectPiece / (a.cg * es))});
+    for (;; groups = (groups + 1) / 2) {
+      const int64_t columns = groups * a.cg / epv;
+      if (columns <= kNormOnceThreads &&
+          v.rows <= kNormOnceThreads / columns * kNormOnceVectors)
+        break;
+      if (groups == 1 || groups * a.cg * es <= least) return false;
+    }
+    v.tile0 = static_cast<int32_t>(tiles);
+    v.slab_groups = static_cast<int32_t>(groups);
+    v.slabs = static_cast<int32_t>(ceil_div(a.G, groups));
+    v.tiles = 1;
+    v.tile_rows = static_cast<int32_t>(v.rows);
+    tiles += v.rows > 0 ? static_cast<int64_t>(a.B) * v.slabs : 0;
+    if (tiles > (1 << 29)) return false;
+  }
+  std::copy(lv, lv + a.L, a.lv);
+  a.tiles = static_cast<int32_t>(tiles);
+  return true;
+}
+
+// Zeroes what starts as zeros, then both launches; or the one.
+cudaError_t run(NormArgs& a, const Plan& p, int dtype, int act, bool backward, void* workspace,
+                cudaStream_t st) {
+  const int vb = vector_bytes(p, a.L, a.cg, elem_bytes(dtype), backward);
+  const bool once = !backward && make_once(a, vb, elem_bytes(dtype));
+  if (p.zero_bytes > 0 && !once) {
     const cudaError_t err = cudaMemsetAsync(static_cast<char*>(workspace) + p.done, 0,
                                             static_cast<size_t>(p.zero_bytes), st);
     if (err != cudaSuccess) return err;
   }
-  const int vb = vector_bytes(p, a.L, a.cg, elem_bytes(dtype), backward);
-  if (dtype == MSDA_FLOAT32) return norm_launch<float>(a, vb, act, backward, st);
-  if (dtype == MSDA_FLOAT16) return norm_launch<__half>(a, vb, act, backward, st);
-  return norm_launch<__nv_bfloat16>(a, vb, act, backward, st);
+  if (dtype == MSDA_FLOAT32) return norm_launch<float>(a, vb, act, backward, once, st);
+  if (dtype == MSDA_FLOAT16) return norm_launch<__half>(a, vb, act, backward, once, st);
+  return norm_launch<__nv_bfloat16>(a, vb, act, backward, once, st);
 }
 
 }  // namespace

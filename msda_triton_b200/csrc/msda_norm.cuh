@@ -16,6 +16,9 @@
 // second applies them, from the last tile back: what the first read last is
 // then still in L2.
 //
+// A forward whose segments are small takes one launch instead: a CTA keeps a
+// unit's rows in registers from the statistics to the application.
+//
 // Tiles leave partial results.  Where a unit has few tiles, each CTA of the
 // second launch joins those of its groups itself ("direct"): that costs 1 us at
 // its start, and neither counters nor a wait.  Else the CTA that finishes a
@@ -75,10 +78,15 @@ struct NormArgs {
   void* gbias;
 };
 
+// Forward of segments that a CTA holds in registers: threads, and vectors of each.
+constexpr int kNormOnceThreads = 512, kNormOnceVectors = 8;
+
 constexpr int kNormParamChannels = 8;  // of a CTA that sums gradients of the affine map
 
-// Both launches; one instance per dtype (msda_norm_{f32,f16,bf16}.cu).
+// Both launches, or (once) the one of units that are one tile each; one
+// instance per dtype (msda_norm_{f32,f16,bf16}.cu).
 template <typename T>
-cudaError_t norm_launch(const NormArgs& a, int vb, int act, bool backward, cudaStream_t st);
+cudaError_t norm_launch(const NormArgs& a, int vb, int act, bool backward, bool once,
+                        cudaStream_t st);
 
 }  // namespace msda
