@@ -1,6 +1,7 @@
 // msda_norm.cu -- msda_group_norm_{fwd,bwd}: checks, and the plan of units
 // and tiles.
 #include <algorithm>
+#include <numeric>
 
 #include "msda_norm.cuh"
 #include "msda_status.cuh"
@@ -55,6 +56,9 @@ int make_plan(int dtype, int64_t B, int64_t C, int64_t G, int64_t L, const int64
                                   : std::min(kTile, std::max(total / at_once, kMediumTile));
     const int64_t piece = p.direct ? kDirectPiece : kPiece;
     sg = std::min(G, std::max<int64_t>(1, std::min(ceil_div(piece, cg * es), kNormMaxSlab / cg)));
+    // of whole vectors, for those that hold several groups
+    const int64_t whole = std::min(G, round_up(sg, 16 / es / std::gcd(cg, 16 / es)));
+    if (whole * cg <= kNormMaxSlab) sg = whole;
     p.tiles = p.counters = 0;
     int64_t most = 0, sum = 0;
     for (int64_t l = 0; l < L; ++l) {
@@ -112,15 +116,14 @@ int check_sizes(int dtype, int64_t B, int64_t C, int64_t G, int64_t L, const int
   return MSDA_SUCCESS;
 }
 
-// The largest vector that divides a group, every stride and every address.
-int vector_bytes(const Plan& p, int64_t L, int64_t cg, int64_t es, bool backward) {
+// The largest vector that divides every stride and every address.
+int vector_bytes(const NormArgs& a, int64_t es, bool backward) {
   int64_t vb = 16;
   auto fit = [&](int64_t bytes) {
     while (vb > es && bytes % vb != 0) vb >>= 1;
   };
-  fit(cg * es);
-  for (int64_t l = 0; l < L; ++l) {
-    const NormLevel& v = p.lv[l];
+  for (int64_t l = 0; l < a.L; ++l) {
+    const NormLevel& v = a.lv[l];
     if (v.rows == 0) continue;
     fit(static_cast<int64_t>(reinterpret_cast<uintptr_t>(v.x) % 16));
     fit(static_cast<int64_t>(reinterpret_cast<uintptr_t>(v.out) % 16));
@@ -217,16 +220,23 @@ bool make_once(NormArgs& a, int vb, int64_t es) {
 // Zeroes what starts as zeros, then both launches; or the one.
 cudaError_t run(NormArgs& a, const Plan& p, int dtype, int act, bool backward, void* workspace,
                 cudaStream_t st) {
-  const int vb = vector_bytes(p, a.L, a.cg, elem_bytes(dtype), backward);
-  const bool once = !backward && make_once(a, vb, elem_bytes(dtype));
+  const int64_t es = elem_bytes(dtype);
+  const int wide = vector_bytes(a, es, backward);
+  int vb = wide;  // dividing a group too
+  while (a.cg * es % vb != 0) vb >>= 1;
+  const bool once = !backward && make_once(a, vb, es);
+  // slabs of whole vectors, where those hold several groups
+  const bool mixed = !once && wide == 16 && vb < 16 && a.C * es % 16 == 0 &&
+                     (a.lv[0].slab_groups == a.G || a.lv[0].slab_groups * a.cg * es % 16 == 0) &&
+                     a.lv[0].slab_groups * a.cg <= kNormMaxSlab;
   if (p.zero_bytes > 0 && !once) {
     const cudaError_t err = cudaMemsetAsync(static_cast<char*>(workspace) + p.done, 0,
                                             static_cast<size_t>(p.zero_bytes), st);
     if (err != cudaSuccess) return err;
   }
-  if (dtype == MSDA_FLOAT32) return norm_launch<float>(a, vb, act, backward, once, st);
-  if (dtype == MSDA_FLOAT16) return norm_launch<__half>(a, vb, act, backward, once, st);
-  return norm_launch<__nv_bfloat16>(a, vb, act, backward, once, st);
+  if (dtype == MSDA_FLOAT32) return norm_launch<float>(a, vb, mixed, act, backward, once, st);
+  if (dtype == MSDA_FLOAT16) return norm_launch<__half>(a, vb, mixed, act, backward, once, st);
+  return norm_launch<__nv_bfloat16>(a, vb, mixed, act, backward, once, st);
 }
 
 }  // namespace

@@ -226,53 +226,102 @@ __device__ __forceinline__ void norm_wait_previous() {
 }
 
 // ------------------------------------------------------------------ forward
-template <typename T, int VB, bool DIRECT, int U>
+// MIXED, here and below: a vector holds channels of several groups (groups of
+// no whole vectors: 320 channels in 32).  Sums are then carried per channel.
+// Read in pieces of 4 or 2 bytes, 168 MB of bf16 with 10 channels a group take
+// 169 us forward and 392 backward; in such vectors 129 and 232.
+template <typename T, int VB, bool DIRECT, bool MIXED, int U>
 __device__ void norm_stats(const NormArgs& a, const NormTile& t) {
   using P = Pairs<T, VB>;
   constexpr int EPV = P::EPV;
-  __shared__ float3 part[kNormThreads];
+  // MIXED: each thread's channels' (mean, squared deviations); else (count,
+  // mean, squared deviations) of its vectors
+  __shared__ float2 channels[MIXED ? kNormThreads * EPV : 1];
+  __shared__ float3 part[MIXED ? 1 : kNormThreads];
   const NormLevel& v = a.lv[t.l];
   const NormThread me(a, t);
   const T* x = reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row +
                static_cast<int64_t>(t.g0) * a.cg;
   const int64_t hop = t.trows * v.x_row;
   float n = 0.f, mean = 0.f, m2 = 0.f;
-  for (int col = me.tc; col < t.nvc; col += t.tcols) {
-    const T* p = x + col * EPV;
-    norm_rows<U>(t, me.tr, [&](auto count) {
+  if constexpr (MIXED) {
+    // deviations from the thread's first row, which no outlier elsewhere spoils
+    const T* p = x + me.tc * EPV;
+    uint64_t minus[P::N], s[P::N], q[P::N];
+    if (me.tr < t.rows) P::unpack(norm_ld<VB>(p), minus);
+#pragma unroll
+    for (int i = 0; i < P::N; ++i) {
+      minus[i] = mul2(minus[i], pair(-1.f, -1.f));
+      s[i] = q[i] = 0;  // two zeros
+    }
+    norm_rows<U / 2>(t, me.tr, [&](auto count) {
       constexpr int K = decltype(count)::value;
       Raw<VB> w[K];
 #pragma unroll
       for (int u = 0; u < K; ++u) w[u] = norm_ld<VB>(p + u * hop);
       p += K * hop;
-      uint64_t s = 0, q = 0;  // two zeros
-#pragma unroll
-      for (int u = 0; u < K; ++u) {
-        uint64_t f[P::N];
-        P::unpack(w[u], f);
-#pragma unroll
-        for (int i = 0; i < P::N; ++i) s = add2(s, f[i]);
-      }
-      float sa, sb;
-      unpair(s, sa, sb);
-      const float cm = (sa + sb) * (1.f / (K * EPV));
-      // a single element's second half is no element
-      const uint64_t minus = pair(-cm, EPV == 1 ? 0.f : -cm);
 #pragma unroll
       for (int u = 0; u < K; ++u) {
         uint64_t f[P::N];
         P::unpack(w[u], f);
 #pragma unroll
         for (int i = 0; i < P::N; ++i) {
-          const uint64_t d = add2(f[i], minus);
-          q = fma2(d, d, q);
+          const uint64_t d = add2(f[i], minus[i]);
+          s[i] = add2(s[i], d);
+          q[i] = fma2(d, d, q[i]);
         }
       }
-      unpair(q, sa, sb);
-      norm_join(n, mean, m2, K * EPV, cm, sa + sb);
     });
+    const float inv = 1.f / static_cast<float>(max(1, (t.rows - me.tr + t.trows - 1) / t.trows));
+#pragma unroll
+    for (int i = 0; i < P::N; ++i) {
+      float m0, m1, s0, s1, q0, q1;
+      unpair(minus[i], m0, m1);
+      unpair(s[i], s0, s1);
+      unpair(q[i], q0, q1);
+      channels[threadIdx.x * EPV + 2 * i] =
+          make_float2(s0 * inv - m0, fmaxf(q0 - s0 * s0 * inv, 0.f));
+      channels[threadIdx.x * EPV + 2 * i + 1] =
+          make_float2(s1 * inv - m1, fmaxf(q1 - s1 * s1 * inv, 0.f));
+    }
+  } else {
+    for (int col = me.tc; col < t.nvc; col += t.tcols) {
+      const T* p = x + col * EPV;
+      norm_rows<U>(t, me.tr, [&](auto count) {
+        constexpr int K = decltype(count)::value;
+        Raw<VB> w[K];
+#pragma unroll
+        for (int u = 0; u < K; ++u) w[u] = norm_ld<VB>(p + u * hop);
+        p += K * hop;
+        uint64_t s = 0, q = 0;  // two zeros
+#pragma unroll
+        for (int u = 0; u < K; ++u) {
+          uint64_t f[P::N];
+          P::unpack(w[u], f);
+#pragma unroll
+          for (int i = 0; i < P::N; ++i) s = add2(s, f[i]);
+        }
+        float sa, sb;
+        unpair(s, sa, sb);
+        const float cm = (sa + sb) * (1.f / (K * EPV));
+        // a single element's second half is no element
+        const uint64_t minus = pair(-cm, EPV == 1 ? 0.f : -cm);
+#pragma unroll
+        for (int u = 0; u < K; ++u) {
+          uint64_t f[P::N];
+          P::unpack(w[u], f);
+#pragma unroll
+          for (int i = 0; i < P::N; ++i) {
+            const uint64_t d = add2(f[i], minus);
+            q = fma2(d, d, q);
+          }
+        }
+        unpair(q, sa, sb);
+        norm_join(n, mean, m2, K * EPV, cm, sa + sb);
+      });
+    }
+    part[threadIdx.x] = make_float3(n, mean, m2);
   }
-  part[threadIdx.x] = make_float3(n, mean, m2);
   __syncthreads();
   // `lanes` threads of a group join its threads' results
   int lanes = 32;
@@ -281,11 +330,19 @@ __device__ void norm_stats(const NormArgs& a, const NormTile& t) {
   const bool on = g < t.groups;
   const int per = t.groups == 1 ? t.tcols : a.cg / EPV;  // columns of a group
   n = mean = m2 = 0.f;
-  if (on)
+  if (MIXED && on) {
+    for (int k = j; k < a.cg * t.trows; k += lanes) {
+      const int row = k / a.cg;
+      const float2 o = channels[row * t.tcols * EPV + g * a.cg + (k - row * a.cg)];
+      norm_join(n, mean, m2, static_cast<float>(max(0, (t.rows - row + t.trows - 1) / t.trows)),
+                o.x, o.y);
+    }
+  } else if (on) {
     for (int k = j; k < per * t.trows; k += lanes) {
       const float3 o = part[k / per * t.tcols + g * per + k % per];
       norm_join(n, mean, m2, o.x, o.y, o.z);
     }
+  }
   for (int d = 1; d < lanes; d <<= 1) {
     const float nb = __shfl_xor_sync(~0u, n, d), mb = __shfl_xor_sync(~0u, mean, d),
                 sb = __shfl_xor_sync(~0u, m2, d);
@@ -321,17 +378,40 @@ __device__ void norm_stats(const NormArgs& a, const NormTile& t) {
   });
 }
 
-// h = x * scale + shift of one group, as pairs.  16-bit x has no digits that
-// the mean's product could lose; fp32 x is centred first (shift: -mean).
-template <typename T> struct NormCentre {
-  uint64_t shift, scale;
-  __device__ __forceinline__ NormCentre(float2 st) {
-    const float s = sizeof(T) == 2 ? -st.x * st.y : -st.x;
-    shift = pair(s, s);
-    scale = pair(st.y, st.y);
+// A group's two values (of `values`, whose first is group g0's) for each of a
+// vector's channels c0 ..., as pairs: once, or MIXED for each pair of channels.
+enum NormOf { kNormMinusX, kNormMinusBoth, kNormMinusProduct };  // (-x, y), (-x, -y), (-x y, y)
+
+template <int EPV, bool MIXED, bool SHARED, NormOf OF>
+__device__ __forceinline__ void norm_of_groups(const float2* values, int cg, int g0, int c0,
+                                               uint64_t* x, uint64_t* y) {
+  auto value = [&](int c) {
+    // other CTAs' results are read in L2
+    float2 p = SHARED ? values[c / cg - g0] : __ldcg(values + (c / cg - g0));
+    p.x = OF == kNormMinusProduct ? -p.x * p.y : -p.x;
+    if (OF == kNormMinusBoth) p.y = -p.y;
+    return p;
+  };
+#pragma unroll
+  for (int i = 0; i < (MIXED ? EPV : 1); i += 2) {
+    const float2 p = value(c0 + i), q = MIXED ? value(c0 + i + 1) : p;
+    x[i / 2] = pair(p.x, q.x);
+    y[i / 2] = pair(p.y, q.y);
   }
-  __device__ __forceinline__ uint64_t operator()(uint64_t x) const {
-    return sizeof(T) == 2 ? fma2(x, scale, shift) : mul2(add2(x, shift), scale);
+}
+
+// h = x * scale + shift, as pairs.  16-bit x has no digits that the mean's
+// product could lose; fp32 x is centred first (shift: -mean).
+template <typename T, int EPV, bool MIXED> struct NormCentre {
+  static constexpr int N = MIXED ? EPV / 2 : 1;
+  uint64_t shift[N], scale[N];
+  __device__ __forceinline__ NormCentre(const float2* stats, int cg, int c0) {
+    norm_of_groups<EPV, MIXED, false, sizeof(T) == 2 ? kNormMinusProduct : kNormMinusX>(
+        stats, cg, 0, c0, shift, scale);
+  }
+  __device__ __forceinline__ uint64_t operator()(uint64_t x, int i) const {
+    const int k = MIXED ? i : 0;
+    return sizeof(T) == 2 ? fma2(x, scale[k], shift[k]) : mul2(add2(x, shift[k]), scale[k]);
   }
 };
 
@@ -371,7 +451,7 @@ __device__ __forceinline__ void norm_join_here(const NormArgs& a, const NormTile
   __syncthreads();
 }
 
-template <typename T, int VB, int ACT, bool DIRECT, int U>
+template <typename T, int VB, int ACT, bool DIRECT, bool MIXED, int U>
 __device__ void norm_apply(const NormArgs& a, const NormTile& t) {
   using P = Pairs<T, VB>;
   constexpr int EPV = P::EPV;
@@ -382,8 +462,13 @@ __device__ void norm_apply(const NormArgs& a, const NormTile& t) {
   const int64_t hop = t.trows * v.x_row, yhop = t.trows * v.out_row;
   for (int col = me.tc; col < t.nvc; col += t.tcols) {
     const int c0 = t.g0 * a.cg + col * EPV;
-    const float2 st = DIRECT ? joined[c0 / a.cg - t.g0]
-                               : __ldcg(a.stats + me.segment * a.G + c0 / a.cg);
+    constexpr int M = MIXED ? P::N : 1;  // pairs with statistics of their own
+    uint64_t minus[M], r2[M];
+    if (DIRECT)
+      norm_of_groups<EPV, MIXED, true, kNormMinusX>(joined, a.cg, t.g0, c0, minus, r2);
+    else
+      norm_of_groups<EPV, MIXED, false, kNormMinusX>(a.stats + me.segment * a.G, a.cg, 0, c0,
+                                                     minus, r2);
     float f[EPV];
     uint64_t w[P::N], d[P::N];
     const int64_t at = static_cast<int64_t>(t.l) * a.affine_level + c0;
@@ -391,11 +476,10 @@ __device__ void norm_apply(const NormArgs& a, const NormTile& t) {
     P::of(f, w);
     norm_params<EPV>(a.bias, a.affine_dtype, at, 0.f, f);
     P::of(f, d);
-    const uint64_t minus = pair(-st.x, -st.x), r2 = pair(st.y, st.y);
 #pragma unroll
     for (int i = 0; i < P::N; ++i) {
-      w[i] = mul2(w[i], r2);
-      if (sizeof(T) == 2) d[i] = fma2(w[i], minus, d[i]);  // as NormCentre
+      w[i] = mul2(w[i], r2[MIXED ? i : 0]);
+      if (sizeof(T) == 2) d[i] = fma2(w[i], minus[MIXED ? i : 0], d[i]);  // as NormCentre
     }
     const T* p = reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row + c0;
     T* y = reinterpret_cast<T*>(v.out) + v.out_batch * t.b + (t.row0 + me.tr) * v.out_row + c0;
@@ -411,7 +495,8 @@ __device__ void norm_apply(const NormArgs& a, const NormTile& t) {
         P::unpack(raw[u], e);
 #pragma unroll
         for (int i = 0; i < P::N; ++i)
-          e[i] = norm_act<ACT>(fma2(sizeof(T) == 2 ? e[i] : add2(e[i], minus), w[i], d[i]));
+          e[i] = norm_act<ACT>(
+              fma2(sizeof(T) == 2 ? e[i] : add2(e[i], minus[MIXED ? i : 0]), w[i], d[i]));
         norm_st<VB>(y + u * yhop, P::pack(e));
       }
       y += K * yhop;
@@ -552,7 +637,7 @@ __device__ __forceinline__ void norm_copies_wait() {  // for all but the last kN
 }
 
 // Sums s1, s2 per channel of one tile, and the groups' coefficients a, q of the unit.
-template <typename T, int VB, int ACT, bool DIRECT, int U>
+template <typename T, int VB, int ACT, bool DIRECT, bool MIXED, int U>
 __device__ void norm_grad_stats(const NormArgs& a, const NormTile& t) {
   using P = Pairs<T, VB>;
   constexpr int EPV = P::EPV;
@@ -572,7 +657,7 @@ __device__ void norm_grad_stats(const NormArgs& a, const NormTile& t) {
     if (kStaged && col0 > 0) __syncthreads();  // the sums before are read
     if (col < t.nvc) {
       const int c0 = t.g0 * a.cg + col * EPV;
-      const NormCentre<T> centre(__ldg(a.stats + me.segment * a.G + c0 / a.cg));
+      const NormCentre<T, EPV, MIXED> centre(a.stats + me.segment * a.G, a.cg, c0);
       uint64_t w[P::N], d[P::N];
       if (ACT != MSDA_ACT_NONE) {
         float f[EPV];
@@ -592,7 +677,7 @@ __device__ void norm_grad_stats(const NormArgs& a, const NormTile& t) {
         P::unpack(rg, e);
 #pragma unroll
         for (int i = 0; i < P::N; ++i) {
-          const uint64_t h = centre(f[i]);
+          const uint64_t h = centre(f[i], i);
           const uint64_t dz =
               ACT == MSDA_ACT_NONE ? e[i] : mul2(e[i], norm_dact<ACT>(fma2(h, w[i], d[i])));
           s1[i] = add2(s1[i], dz);
@@ -800,7 +885,7 @@ __device__ __forceinline__ void norm_param_grad(const NormArgs& a, int cta) {
   put(a.gbias, s.x);
 }
 
-template <typename T, int VB, int ACT, bool DIRECT, int U>
+template <typename T, int VB, int ACT, bool DIRECT, bool MIXED, int U>
 __device__ void norm_grad_apply(const NormArgs& a, const NormTile& t) {
   using P = Pairs<T, VB>;
   constexpr int EPV = P::EPV;
@@ -811,10 +896,14 @@ __device__ void norm_grad_apply(const NormArgs& a, const NormTile& t) {
   const int64_t hop = t.trows * v.x_row, ghop = t.trows * v.gy_row, yhop = t.trows * v.out_row;
   for (int col = me.tc; col < t.nvc; col += t.tcols) {
     const int c0 = t.g0 * a.cg + col * EPV;
-    const float2 st = __ldg(a.stats + me.segment * a.G + c0 / a.cg);
-    const float2 co = DIRECT ? joined[c0 / a.cg - t.g0]
-                               : __ldcg(a.coef + me.segment * a.G + c0 / a.cg);
-    const NormCentre<T> centre(st);
+    const NormCentre<T, EPV, MIXED> centre(a.stats + me.segment * a.G, a.cg, c0);
+    constexpr int M = MIXED ? P::N : 1;
+    uint64_t ma[M], mq[M];
+    if (DIRECT)
+      norm_of_groups<EPV, MIXED, true, kNormMinusBoth>(joined, a.cg, t.g0, c0, ma, mq);
+    else
+      norm_of_groups<EPV, MIXED, false, kNormMinusBoth>(a.coef + me.segment * a.G, a.cg, 0, c0, ma,
+                                                        mq);
     float f[EPV];
     uint64_t w[P::N], d[P::N];
     const int64_t at = static_cast<int64_t>(t.l) * a.affine_level + c0;
@@ -828,7 +917,6 @@ __device__ void norm_grad_apply(const NormArgs& a, const NormTile& t) {
     const T* g =
         reinterpret_cast<const T*>(v.gy) + v.gy_batch * t.b + (t.row0 + me.tr) * v.gy_row + c0;
     T* y = reinterpret_cast<T*>(v.out) + v.out_batch * t.b + (t.row0 + me.tr) * v.out_row + c0;
-    const uint64_t r2 = pair(st.y, st.y), ma = pair(-co.x, -co.x), mq = pair(-co.y, -co.y);
     norm_rows<U>(t, me.tr, [&](auto count) {
       constexpr int K = decltype(count)::value;
       Raw<VB> rx[K], rg[K];
@@ -846,10 +934,11 @@ __device__ void norm_grad_apply(const NormArgs& a, const NormTile& t) {
         P::unpack(rg[u], e);
 #pragma unroll
         for (int i = 0; i < P::N; ++i) {
-          const uint64_t h = centre(x[i]);
+          const uint64_t h = centre(x[i], i);
           const uint64_t dz =
               ACT == MSDA_ACT_NONE ? e[i] : mul2(e[i], norm_dact<ACT>(fma2(h, w[i], d[i])));
-          x[i] = mul2(r2, fma2(dz, w[i], fma2(h, mq, ma)));
+          const int k = MIXED ? i : 0;
+          x[i] = mul2(centre.scale[k], fma2(dz, w[i], fma2(h, mq[k], ma[k])));
         }
         st_chunk<VB>(y + u * yhop, P::pack(x));
       }
@@ -863,17 +952,17 @@ __device__ void norm_grad_apply(const NormArgs& a, const NormTile& t) {
 // timed (3 to 6 CTAs, 2 to 8 vectors) the fastest.  Two 3D xl pyramids, 1.23 GB
 // of bf16 with SiLU: statistics 202 us (6.1 TB/s) and application 382 us
 // (6.4 TB/s) forward, 418 us (5.9) and 585 us (6.3) backward.
-template <typename T, int VB, int ACT, bool BWD, bool DIRECT>
-__global__ void __launch_bounds__(kNormThreads, 4)
+template <typename T, int VB, int ACT, bool BWD, bool DIRECT, bool MIXED>
+__global__ void __launch_bounds__(kNormThreads, BWD && (MIXED || VB < 16) ? 3 : 4)
 norm_stats_kernel(const __grid_constant__ NormArgs a) {
   norm_let_next_start();
   const NormTile t = norm_tile<Chunk<T, VB>::EPV>(a, blockIdx.x);
-  if (BWD) norm_grad_stats<T, VB, ACT, DIRECT, 2>(a, t);
-  else norm_stats<T, VB, DIRECT, 8>(a, t);
+  if (BWD) norm_grad_stats<T, VB, ACT, DIRECT, MIXED, 2>(a, t);
+  else norm_stats<T, VB, DIRECT, MIXED, 8>(a, t);
 }
 
-template <typename T, int VB, int ACT, bool BWD, bool DIRECT>
-__global__ void __launch_bounds__(kNormThreads, BWD ? 3 : 4)
+template <typename T, int VB, int ACT, bool BWD, bool DIRECT, bool MIXED>
+__global__ void __launch_bounds__(kNormThreads, (BWD ? 3 : 4) - MIXED)
 norm_apply_kernel(const __grid_constant__ NormArgs a) {
   const int block = static_cast<int>(blockIdx.x) - a.param_ctas;
   if (BWD && block < 0) {
@@ -883,16 +972,16 @@ norm_apply_kernel(const __grid_constant__ NormArgs a) {
   }
   const NormTile t = norm_tile<Chunk<T, VB>::EPV>(a, a.tiles - 1 - block);
   norm_wait_previous();
-  if (BWD) norm_grad_apply<T, VB, ACT, DIRECT, 2>(a, t);
-  else norm_apply<T, VB, ACT, DIRECT, 4>(a, t);
+  if (BWD) norm_grad_apply<T, VB, ACT, DIRECT, MIXED, 2>(a, t);
+  else norm_apply<T, VB, ACT, DIRECT, MIXED, 4>(a, t);
 }
 
-template <typename T, int VB, int ACT, bool BWD, bool DIRECT>
+template <typename T, int VB, int ACT, bool BWD, bool DIRECT, bool MIXED>
 cudaError_t norm_launch_one(const NormArgs& a, cudaStream_t st) {
   // the forward's statistics are the same for every activation
   constexpr int kAct = BWD ? ACT : MSDA_ACT_NONE;
   if (a.tiles > 0) {
-    norm_stats_kernel<T, VB, kAct, BWD, DIRECT><<<a.tiles, kNormThreads, 0, st>>>(a);
+    norm_stats_kernel<T, VB, kAct, BWD, DIRECT, MIXED><<<a.tiles, kNormThreads, 0, st>>>(a);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
   }
@@ -906,24 +995,25 @@ cudaError_t norm_launch_one(const NormArgs& a, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = a.tiles > 0 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, norm_apply_kernel<T, VB, ACT, BWD, DIRECT>, a);
+  return cudaLaunchKernelEx(&cfg, norm_apply_kernel<T, VB, ACT, BWD, DIRECT, MIXED>, a);
 }
 
-template <typename T, int VB>
+template <typename T, int VB, bool MIXED>
 cudaError_t norm_launch_act(const NormArgs& a, int act, bool backward, bool once,
                             cudaStream_t st) {
   switch (act) {
-#define MSDA_NORM_ACT(ACT)                                                       \
-  case ACT:                                                                      \
-    if (once) {                                                                  \
-      norm_once_kernel<T, VB, ACT><<<a.tiles, kNormOnceThreads, 0, st>>>(a);     \
-      return cudaGetLastError();                                                 \
-    }                                                                            \
-    if (a.direct)                                                                \
-      return backward ? norm_launch_one<T, VB, ACT, true, true>(a, st)           \
-                      : norm_launch_one<T, VB, ACT, false, true>(a, st);         \
-    return backward ? norm_launch_one<T, VB, ACT, true, false>(a, st)            \
-                    : norm_launch_one<T, VB, ACT, false, false>(a, st);
+#define MSDA_NORM_ACT(ACT)                                                              \
+  case ACT:                                                                             \
+    if constexpr (!MIXED)                                                               \
+      if (once) {                                                                       \
+        norm_once_kernel<T, VB, ACT><<<a.tiles, kNormOnceThreads, 0, st>>>(a);          \
+        return cudaGetLastError();                                                      \
+      }                                                                                 \
+    if (a.direct)                                                                       \
+      return backward ? norm_launch_one<T, VB, ACT, true, true, MIXED>(a, st)           \
+                      : norm_launch_one<T, VB, ACT, false, true, MIXED>(a, st);         \
+    return backward ? norm_launch_one<T, VB, ACT, true, false, MIXED>(a, st)            \
+                    : norm_launch_one<T, VB, ACT, false, false, MIXED>(a, st);
     MSDA_NORM_ACT(MSDA_ACT_RELU)
     MSDA_NORM_ACT(MSDA_ACT_SILU)
     MSDA_NORM_ACT(MSDA_ACT_GELU)
@@ -934,14 +1024,16 @@ cudaError_t norm_launch_act(const NormArgs& a, int act, bool backward, bool once
 }
 
 template <typename T>
-cudaError_t norm_launch(const NormArgs& a, int vb, int act, bool backward, bool once,
+cudaError_t norm_launch(const NormArgs& a, int vb, bool mixed, int act, bool backward, bool once,
                         cudaStream_t st) {
+  if (mixed) return norm_launch_act<T, 16, true>(a, act, backward, once, st);
   switch (vb) {
-    case 16: return norm_launch_act<T, 16>(a, act, backward, once, st);
-    case 8: return norm_launch_act<T, 8>(a, act, backward, once, st);
-    case 4: return norm_launch_act<T, 4>(a, act, backward, once, st);
+    case 16: return norm_launch_act<T, 16, false>(a, act, backward, once, st);
+    case 8: return norm_launch_act<T, 8, false>(a, act, backward, once, st);
+    case 4: return norm_launch_act<T, 4, false>(a, act, backward, once, st);
     default:
-      if constexpr (sizeof(T) == 2) return norm_launch_act<T, 2>(a, act, backward, once, st);
+      if constexpr (sizeof(T) == 2)
+        return norm_launch_act<T, 2, false>(a, act, backward, once, st);
       return cudaErrorInvalidValue;
   }
 }

@@ -126,6 +126,28 @@ def test_group_widths(C, G, dt):
     check(features(2, rows, C, dt), rows, G, *affine((C,)), activation="silu")
 
 
+@pytest.mark.parametrize("dt", DTYPES, ids=ids)
+@pytest.mark.parametrize("C,G", [(320, 32), (96, 32), (24, 8), (48, 16), (40, 4), (384, 32), (16, 16)])
+@pytest.mark.parametrize("rows", [[700, 3], [30011]], ids=str)
+def test_vectors_of_several_groups(rows, C, G, dt):
+    """Groups of 1 to 12 channels in vectors of 4 or 8, few tiles and many."""
+    x = features(1, rows, C, dt)
+    check(x, rows, G, *affine((len(rows), C)), activation="silu")
+
+
+def test_mixed_groups_keep_to_themselves():
+    """Neighbouring groups of one vector: a mean of 1000 and an outlier in one leave the next alone."""
+    x = torch.randn(1, 5000, 24, generator=torch.Generator().manual_seed(8)).to(DEV)
+    clean = msda.pyramid_group_norm(x, [(5000,)], 8)
+    x[..., 3:6] += 1000.0
+    x[0, 17, 6:9] = 1e4
+    y = msda.pyramid_group_norm(x, [(5000,)], 8)
+    assert torch.equal(y[..., :3], clean[..., :3]) and torch.equal(y[..., 9:], clean[..., 9:])
+    want = norm64([x.double()], 8, [1.0], [0.0], 1e-5, "none")
+    assert float((y.double() - want)[..., 3:6].abs().max()) < 4 * 1000 * 2.0 ** -24
+    assert float((y.double() - want)[..., 6:9].abs().max()) < 1e-5 * float(want[..., 6:9].abs().max())
+
+
 @pytest.mark.parametrize("rows", [[1], [0, 5], [5, 0, 0], [1, 1, 1, 1], [257], [16] * 16],
                          ids=str)
 def test_row_counts(rows):
