@@ -8,8 +8,8 @@
 // if there is one).  With fp32 moments it is bound by memory: 28 bytes a
 // parameter in fp32 (22 in bf16), 335 M of them in 1.35 ms (1.07 ms), 6.9 TB/s.
 // With 8-bit moments and bf16 parameters, 10 bytes a parameter, the coding is:
-// about 75 instructions a parameter, 0.90 ms for 335 M (3.8 TB/s; fp32
-// parameters 0.98 ms, 5.5 TB/s).
+// about 77 instructions a parameter, half of them on the integer units that are
+// 78 % busy, 0.87 ms for 335 M (3.8 TB/s; fp32 parameters 0.97 ms, 5.5 TB/s).
 //
 // States of all tensors lie in one array each; tensor i's elements start at
 // the sum of the earlier tensors' sizes, each rounded up to kBlock.
@@ -84,29 +84,30 @@ template <int N> struct AdamTable {
 
 constexpr uint32_t kMaxFinite = 0x7f7fffffu;
 
-// Byte i of a word of codes as a value; `shift` is 8 (E - top).
-template <bool SIGNED>
-__device__ __forceinline__ float adam_decode(uint32_t word, int i, uint32_t shift) {
-  constexpr uint32_t kCode = (SIGNED ? 127u : 255u) << 20;
-  const int up = 20 - 8 * i;
-  const uint32_t size = (up >= 0 ? word << up : word >> -up) & kCode;
-  uint32_t bits = min(size, 1u << 20) * shift + size;  // zero stays zero
-  if (SIGNED) bits |= word << (24 - 8 * i) & 0x80000000u;
-  return __uint_as_float(bits);
-}
-__device__ __forceinline__ uint32_t adam_shift(uint32_t e, uint32_t top) {
-  return (e - top) << 3;
-}
-// The highest code is no number: whether one of a word's is tested at once.
-template <bool SIGNED>
-__device__ __forceinline__ void adam_decode_odd(uint32_t word, float* f) {
-  constexpr uint32_t kTopCode = SIGNED ? 127u : 255u;
-  const bool odd = SIGNED ? ((word & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u) != 0u
-                          : (~word - 0x01010101u & word & 0x80808080u) != 0u;
-  if (!odd) return;
+// A lane's four first and four second moments.  Zero stays zero.  The highest
+// code, which is no number, is rare: whether there is one is tested for all
+// eight codes at once.
+__device__ __forceinline__ void adam_decode(uint32_t wm, uint32_t wv, uint32_t em, uint32_t ev,
+                                            float* m, float* v) {
+  const uint32_t sm = (em - 15u) << 23, sv = (ev - 31u) << 23;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if ((word >> (8 * i) & kTopCode) == kTopCode) f[i] = __uint_as_float(0x7fc00000u);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t top = wm << (24 - 8 * i);
+    uint32_t x = top >> 4 & 0x07f00000u;
+    if (x != 0u) x += sm;
+    m[i] = __uint_as_float(x | (top & 0x80000000u));
+    uint32_t y = (i < 3 ? wv << (20 - 8 * i) : wv >> 4) & 0x0ff00000u;
+    if (y != 0u) y += sv;
+    v[i] = __uint_as_float(y);
+  }
+  constexpr uint32_t kOnes = 0x01010101u;
+  const uint32_t odd = ((wm & 0x7f7f7f7fu) + kOnes) | (~(wv + kOnes) & wv);
+  if ((odd & 0x80808080u) == 0u) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((wm >> (8 * i) & 127u) == 127u) m[i] = __uint_as_float(0x7fc00000u);
+    if ((wv >> (8 * i) & 255u) == 255u) v[i] = __uint_as_float(0x7fc00000u);
+  }
 }
 
 // Four values as codes where some are not finite, or at the end of the range.
@@ -126,7 +127,7 @@ __device__ __noinline__ uint32_t adam_encode_odd(float4 x, uint4 r, uint32_t& e)
   uint32_t word = 0u;
   for (int i = 0; i < 4; ++i) {
     const uint32_t b = __float_as_uint(f[i]) & 0x7fffffffu;
-    int c = static_cast<int>(min(b + rnd[i], kMaxFinite) >> 20) - base;
+    int c = static_cast<int>(min(b + rnd[i] * 16u + 8u, kMaxFinite) >> 20) - base;
     c = max(c, !SIGNED && b != 0u ? 1 : 0);
     if (b > kMaxFinite) c = kTopCode;
     if (SIGNED) c |= __float_as_uint(f[i]) >> 24 & 128u;
@@ -135,7 +136,8 @@ __device__ __noinline__ uint32_t adam_encode_odd(float4 x, uint4 r, uint32_t& e)
   return word;
 }
 
-// The codes of four values per lane; `r` holds 20 random bits each.
+// The codes of four values per lane; `r` holds 16 random bits each, which with
+// a set bit below them are the upper 17 of the 20 that are added.
 template <uint32_t TOP, bool SIGNED>
 __device__ __forceinline__ uint32_t adam_encode(const float* x, const uint32_t* r, uint32_t& e) {
   uint32_t b[4], most = 0u;
@@ -150,20 +152,15 @@ __device__ __forceinline__ uint32_t adam_encode(const float* x, const uint32_t* 
     return adam_encode_odd<TOP, SIGNED>(make_float4(x[0], x[1], x[2], x[3]),
                                         make_uint4(r[0], r[1], r[2], r[3]), e);
   e = max((most + 0x1fffffu) >> 23, TOP);
-  const int base = static_cast<int>(e - TOP) << 3;
-  uint32_t word = 0u;
+  const int less = 8 - static_cast<int>((e - TOP) << 23);
+  uint32_t c[4];  // a code's byte on top
 #pragma unroll
-  for (int i = 3; i >= 0; --i) {
-    int c = static_cast<int>((b[i] + r[i]) >> 20) - base;
-    c = max(c, SIGNED ? 0 : min(static_cast<int>(b[i]), 1));
-    word = word * 256u + c;
+  for (int i = 0; i < 4; ++i) {
+    const int least = SIGNED ? 0 : static_cast<int>(min(b[i], 1u) << 20);
+    c[i] = static_cast<uint32_t>(max(static_cast<int>(r[i] * 16u + b[i]) + less, least)) << 4;
+    if (SIGNED) c[i] = (c[i] & 0x7fffffffu) | (__float_as_uint(x[i]) & 0x80000000u);
   }
-  if (SIGNED) {  // the top bytes side by side
-    const uint32_t s01 = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x73);
-    const uint32_t s23 = __byte_perm(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x73);
-    word |= __byte_perm(s01, s23, 0x5410) & 0x80808080u;
-  }
-  return word;
+  return __byte_perm(__byte_perm(c[0], c[1], 0x73), __byte_perm(c[2], c[3], 0x73), 0x5410);
 }
 
 __device__ __forceinline__ uint32_t adam_random(uint32_t index, uint32_t key) {
@@ -264,7 +261,7 @@ adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
     Raw<4 * sizeof(T)> rg[U], rp[U];
     Raw<16> rx[U], rm[U], rv[U];
     uint32_t cm[U], cv[U], em[U], ev[U];
-  #pragma unroll
+#pragma unroll
     for (int u = 0; u < U; ++u) {
       const int valid = left - u * kBlock;
       if (valid + lane * 4 <= 0) continue;  // the whole warp: a block that is not there
@@ -281,7 +278,7 @@ adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
         rv[u] = adam_load(v32 + u * kBlock, 4, true);
       }
     }
-  #pragma unroll
+#pragma unroll
     for (int u = 0; u < U; ++u) {
       const int valid = left - u * kBlock;
       if (valid + lane * 4 <= 0) return;
@@ -290,19 +287,12 @@ adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
       if (MASTER) Chunk<float, 16>::unpack(rx[u], x);
       else Chunk<T, 4 * sizeof(T)>::unpack(rp[u], x);
       if (SMALL) {
-        const uint32_t sm = adam_shift(em[u], 15u), sv = adam_shift(ev[u], 31u);
-  #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          m[i] = adam_decode<true>(cm[u], i, sm);
-          v[i] = adam_decode<false>(cv[u], i, sv);
-        }
-        adam_decode_odd<true>(cm[u], m);
-        adam_decode_odd<false>(cv[u], v);
+        adam_decode(cm[u], cv[u], em[u], ev[u], m, v);
       } else {
         Chunk<float, 16>::unpack(rm[u], m);
         Chunk<float, 16>::unpack(rv[u], v);
       }
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 4; i += 2) {
         uint64_t e = mul2(pair(d[i], d[i + 1]), gs);
         uint64_t mm = pair(m[i], m[i + 1]), vv = pair(v[i], v[i + 1]);
@@ -317,7 +307,7 @@ adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
         unpair(fma2(size, q, mul2(decay, pair(x[i], x[i + 1]))), x[i], x[i + 1]);
       }
       if (valid < 4) {  // between tensors
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < 4; ++i)
           if (i >= valid) m[i] = v[i] = x[i] = 0.f;
       }
@@ -325,11 +315,11 @@ adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
       if (MASTER) adam_store(master + u * kBlock, 4, true, x);
       if (SMALL) {
         uint32_t qm[4], qv[4], nm, nv;
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t r = adam_random(static_cast<uint32_t>(s0) + u * kBlock + i, t.key);
-          qm[i] = (r << 4 & 0xffff0u) | 8u;
-          qv[i] = (r >> 12 & 0xffff0u) | 8u;
+          qm[i] = r & 0xffffu;
+          qv[i] = r >> 16;
         }
         const uint32_t wm = adam_encode<15u, true>(m, qm, nm);
         const uint32_t wv = adam_encode<31u, false>(v, qv, nv);
@@ -356,17 +346,9 @@ adamw_values_kernel(const uint8_t* m, const uint8_t* me, const uint8_t* v, const
   const uint2 cm = __ldg(reinterpret_cast<const uint2*>(m + i));
   const uint2 cv = __ldg(reinterpret_cast<const uint2*>(v + i));
   const uint32_t em = __ldg(me + i / kBlock), ev = __ldg(ve + i / kBlock);
-  const uint32_t sm = adam_shift(em, 15u), sv = adam_shift(ev, 31u);
   float fm[8], fv[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    fm[k] = adam_decode<true>(k < 4 ? cm.x : cm.y, k & 3, sm);
-    fv[k] = adam_decode<false>(k < 4 ? cv.x : cv.y, k & 3, sv);
-  }
-  adam_decode_odd<true>(cm.x, fm);
-  adam_decode_odd<true>(cm.y, fm + 4);
-  adam_decode_odd<false>(cv.x, fv);
-  adam_decode_odd<false>(cv.y, fv + 4);
+  adam_decode(cm.x, cv.x, em, ev, fm, fv);
+  adam_decode(cm.y, cv.y, em, ev, fm + 4, fv + 4);
   st_chunk<16>(mo + i, Chunk<__nv_bfloat16, 16>::pack(fm));
   st_chunk<16>(vo + i, Chunk<__nv_bfloat16, 16>::pack(fv));
 }
@@ -498,8 +480,8 @@ int msda_adamw_step(int dtype, int state_bits, int64_t num_tensors, void* const*
   a.ve = exp_avg_sq_exponent;
   a.master = master;
   // Two rounds a CTA for 8-bit states, whose kernel is bound by instructions
-  // (finding the tensor costs seven an element in one round: 930 us against
-  // 895 for 335 M bf16 parameters), where each SM still gets many CTAs; one
+  // (finding the tensor costs seven an element in one round: 909 us against
+  // 875 for 335 M bf16 parameters), where each SM still gets many CTAs; one
   // where memory is the bound (fp32 states: 1070 us against 1082).
   a.rounds = small && total >= int64_t{148} * 64 * kChunk ? 2 : 1;
   const Step s{dtype, small, num_tensors, params, grads, counts, steps, lr, beta1, beta2, seed};
