@@ -65,8 +65,9 @@ struct RotArgs {
   int32_t turned;          // vectors per head that are turned
   int32_t tokens;          // per CTA
   int32_t total;           // B * Q
-  int32_t hop;             // tokens between a thread's vectors if those of a token divide the
+  int32_t hop;             // tokens between a thread's vectors if a token's are no more than a
                            // CTA's threads (then head and pair stay the same), else 0
+  int32_t step;            // vectors between a thread's; the threads that take any
   int32_t flat;            // no tensor has a gap between batch entries
   Divider dq, dunit, dhead, dpair;
   const void* pos;
@@ -79,7 +80,8 @@ struct RotArgs {
 };
 
 __device__ __forceinline__ float rot_position(const RotArgs& a, int64_t i) {
-  if (a.pos_dtype == MSDA_POSITION_INT32) return static_cast<float>(__ldg(static_cast<const int32_t*>(a.pos) + i));
+  if (a.pos_dtype == MSDA_POSITION_INT32)
+    return static_cast<float>(__ldg(static_cast<const int32_t*>(a.pos) + i));
   if (a.pos_dtype == MSDA_POSITION_INT64)
     return static_cast<float>(__ldg(static_cast<const long long*>(a.pos) + i));
   return __ldg(static_cast<const float*>(a.pos) + i);
@@ -126,8 +128,11 @@ template <int N> struct RotShared {
   }
 };
 
-// A thread has one vector (two, of both halves) in flight; six CTAs an SM were
-// faster than three with four each (759 us against 925 for 4.9 GB, 6.5 TB/s).
+// A thread has one vector of 16 bytes (two, of both halves) in flight; six CTAs
+// an SM were faster than three with four each (762 us against 925 for 4.9 GB,
+// 6.4 TB/s).  Of smaller vectors, which pairs of an odd number leave, it has two,
+// and what bounds it is their instructions (20 of 24 channels in 16 bits, 0.69 GB:
+// 233 us; 286 with one, and with 256 threads of which each finds its head anew).
 template <typename T, int VB, bool PAIRS, bool GPOS>
 __global__ void __launch_bounds__(kRotThreads, GPOS ? 4 : 6)
 rotary_kernel(const __grid_constant__ RotArgs a) {
@@ -147,36 +152,40 @@ rotary_kernel(const __grid_constant__ RotArgs a) {
   float4* const weight = reinterpret_cast<float4*>(shared + S::turn_bytes(a.P, a.tokens));
   float4* const sums = weight + S::weights(a.P);
 
-  Raw<VB> va, vb, ia, ib;
-  T* out = nullptr;
-  int t = 0, j = 0, gap = 0;
+  constexpr int U = VB == 16 ? 1 : 2;
+  Raw<VB> va[U], vb[U], ia[U], ib[U];
+  T* out[U];
+  int t[U], j[U];
+  int tt = 0, jj = 0, gap = 0;
   bool second = false;
   const T *px = nullptr, *pi = nullptr;
   T* py = nullptr;
-  auto load = [&](int u) {
+  auto load = [&](int u, int k) {
     if (u >= count) return;
-    if (u < kRotThreads || a.hop == 0) {
-      t = a.dhead(u);
-      const int rest = u - t * per_token;
+    if (u < a.step || a.hop == 0) {
+      tt = a.dhead(u);
+      const int rest = u - tt * per_token;
       int h = a.dunit(rest);
-      j = rest - h * a.units;
+      jj = rest - h * a.units;
       second = h >= a.heads0;
       const RotTensor& x = a.t[second];
       if (second) h -= a.heads0;
-      int c = kAdjacent ? 2 * j : N * j;
+      int c = kAdjacent ? 2 * jj : N * jj;
       gap = kAdjacent ? 1 : a.P;
-      if (j >= a.turned) {
-        c = 2 * a.P + (j - a.turned) * N;
+      if (jj >= a.turned) {
+        c = 2 * a.P + (jj - a.turned) * N;
         gap = 0;
       }
       px = reinterpret_cast<const T*>(x.x) + h * x.xh + c;
       py = reinterpret_cast<T*>(x.y) + h * x.yh + c;
       if (GPOS) pi = reinterpret_cast<const T*>(x.in) + h * x.ih + c;
     } else {
-      t += a.hop;
+      tt += a.hop;
     }
+    t[k] = tt;
+    j[k] = jj;
     const RotTensor& x = a.t[second];
-    const int64_t n = token0 + t;
+    const int64_t n = token0 + tt;
     int64_t ox = n * x.xq, oy = n * x.yq, oi = GPOS ? n * x.iq : 0;
     if (!a.flat) {
       const int64_t b = a.dq(static_cast<uint32_t>(n));
@@ -184,17 +193,23 @@ rotary_kernel(const __grid_constant__ RotArgs a) {
       oy += b * x.yb;
       if (GPOS) oi += b * x.ib;
     }
-    va = rot_load<VB>(px + ox);
-    vb = rot_load<VB>(px + ox + gap);
-    out = py + oy;
+    va[k] = rot_load<VB>(px + ox);
+    vb[k] = rot_load<VB>(px + ox + gap);
+    out[k] = py + oy;
     if (GPOS) {
-      ia = rot_load<VB>(pi + oi);
-      ib = rot_load<VB>(pi + oi + gap);
+      ia[k] = rot_load<VB>(pi + oi);
+      ib[k] = rot_load<VB>(pi + oi + gap);
     }
   };
+  auto load_all = [&](int u) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) load(u + k * a.step, k);
+  };
 
-  load(threadIdx.x);
-  for (int i = threadIdx.x; i < tokens * a.P; i += kRotThreads) {
+  // first those before the angles' latency; threads past the step have none
+  const int u0 = static_cast<int>(threadIdx.x) < a.step ? threadIdx.x : count;
+  load_all(u0);
+  for (int i = threadIdx.x; i < tokens * a.P; i += blockDim.x) {
     const int k = a.dpair(i), p = i - k * a.P;
     const uint32_t n = token0 + k, b = a.dq(n), q = n - b * a.dq.d;
     const int on = __ldg(a.axis + p);
@@ -204,7 +219,7 @@ rotary_kernel(const __grid_constant__ RotArgs a) {
     turn[k * row + p + p / N * S::kPad] = rot_angle(x, __ldg(a.inv_freq + p), a.sign);
   }
   if (GPOS)
-    for (int p = threadIdx.x; p < a.P; p += kRotThreads) {
+    for (int p = threadIdx.x; p < a.P; p += blockDim.x) {
       const float f = __ldg(a.inv_freq + p);
       const int on = __ldg(a.axis + p);
       weight[p + p / N] = make_float4(on == 0 ? f : 0.f, on == 1 ? f : 0.f, on == 2 ? f : 0.f,
@@ -212,46 +227,47 @@ rotary_kernel(const __grid_constant__ RotArgs a) {
     }
   __syncthreads();
 
-  for (int u = threadIdx.x; u < count; u += kRotThreads) {
-    if (u >= kRotThreads) load(u);
+  auto turn_one = [&](int u, int k) {
     float4 ax = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (j >= a.turned) {
-      st_chunk<VB>(out, va);
+    const int jk = j[k];
+    if (jk >= a.turned) {
+      st_chunk<VB>(out[k], va[k]);
     } else {
       // the first of N pairs, or of N / 2 in each half
       constexpr bool kSplit = PAIRS && N > 1;
-      const int j2 = a.turned + j;
+      const int j2 = a.turned + jk;
+      const float2* const angles = turn + t[k] * row;
       const float2* const angle =
-          turn + t * row + (kSplit ? j * N / 2 + j / 2 * S::kPad : j * (N + S::kPad));
-      const float2* const angle2 = turn + t * row + j2 * N / 2 + j2 / 2 * S::kPad;
-      const int w1 = kSplit ? j * N / 2 + j / 2 : j * (N + 1), w2 = j2 * N / 2 + j2 / 2;
+          angles + (kSplit ? jk * N / 2 + jk / 2 * S::kPad : jk * (N + S::kPad));
+      const float2* const angle2 = angles + j2 * N / 2 + j2 / 2 * S::kPad;
+      const int w1 = kSplit ? jk * N / 2 + jk / 2 : jk * (N + 1), w2 = j2 * N / 2 + j2 / 2;
       float f[2 * N], s[2 * N];
-      Chunk<T, VB>::unpack(va, f);
-      Chunk<T, VB>::unpack(vb, f + N);
+      Chunk<T, VB>::unpack(va[k], f);
+      Chunk<T, VB>::unpack(vb[k], f + N);
       if (GPOS) {
-        Chunk<T, VB>::unpack(ia, s);
-        Chunk<T, VB>::unpack(ib, s + N);
+        Chunk<T, VB>::unpack(ia[k], s);
+        Chunk<T, VB>::unpack(ib[k], s + N);
       }
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const bool upper = kSplit && k >= N / 2;
-        const int kk = upper ? k - N / 2 : k;
-        const float2 cs = upper ? angle2[kk] : angle[kk];
-        const int x1 = kSplit ? 2 * k : k, x2 = kSplit ? 2 * k + 1 : k + N;
+      for (int i = 0; i < N; ++i) {
+        const bool upper = kSplit && i >= N / 2;
+        const int ii = upper ? i - N / 2 : i;
+        const float2 cs = upper ? angle2[ii] : angle[ii];
+        const int x1 = kSplit ? 2 * i : i, x2 = kSplit ? 2 * i + 1 : i + N;
         const float y1 = f[x1] * cs.x - f[x2] * cs.y, y2 = f[x2] * cs.x + f[x1] * cs.y;
         f[x1] = y1;
         f[x2] = y2;
         if (GPOS) {
           const float g = s[x1] * y2 - s[x2] * y1;
-          const float4 w = weight[(upper ? w2 : w1) + kk];
+          const float4 w = weight[(upper ? w2 : w1) + ii];
           ax.x += g * w.x;
           ax.y += g * w.y;
           ax.z += g * w.z;
           ax.w += g * w.w;
         }
       }
-      st_chunk<VB>(out, Chunk<T, VB>::pack(f));
-      st_chunk<VB>(out + (kAdjacent ? 1 : a.P), Chunk<T, VB>::pack(f + N));
+      st_chunk<VB>(out[k], Chunk<T, VB>::pack(f));
+      st_chunk<VB>(out[k] + (kAdjacent ? 1 : a.P), Chunk<T, VB>::pack(f + N));
     }
     if (GPOS) {
       // one token's vectors may take several passes over the same slots
@@ -262,12 +278,18 @@ rotary_kernel(const __grid_constant__ RotArgs a) {
       }
       slot = ax;
     }
+  };
+  for (int u = u0; u < count; u += a.step * U) {
+    if (u >= a.step * U) load_all(u);
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (u + k * a.step < count) turn_one(u + k * a.step, k);
   }
   if (GPOS) {
     __syncthreads();
     // a warp per token, in the same order every time
     const int slots = min(per_token, kRotUnits);
-    for (int k = threadIdx.x >> 5; k < tokens; k += kRotThreads / 32) {
+    for (int k = threadIdx.x >> 5; k < tokens; k += blockDim.x >> 5) {
       float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int i = threadIdx.x & 31; i < slots; i += 32) {
         const float4 o = sums[k * slots + i];
@@ -292,6 +314,7 @@ template <typename T, int VB>
 cudaError_t rotary_launch(const RotArgs& a, bool pairs, cudaStream_t st) {
   using S = RotShared<Chunk<T, VB>::EPV>;
   const unsigned int grid = (a.total + a.tokens - 1) / a.tokens;
+  const int threads = (a.step + 31) / 32 * 32;
   int bytes = S::turn_bytes(a.P, a.tokens);
   if (a.gpos != nullptr) {
     bytes += (S::weights(a.P) + std::min(a.tokens * a.heads * a.units, kRotUnits)) *
@@ -302,10 +325,10 @@ cudaError_t rotary_launch(const RotArgs& a, bool pairs, cudaStream_t st) {
           cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
       if (err != cudaSuccess) return err;
     }
-    kernel<<<grid, kRotThreads, bytes, st>>>(a);
+    kernel<<<grid, threads, bytes, st>>>(a);
   } else {
     auto* kernel = pairs ? rotary_kernel<T, VB, true, false> : rotary_kernel<T, VB, false, false>;
-    kernel<<<grid, kRotThreads, bytes, st>>>(a);
+    kernel<<<grid, threads, bytes, st>>>(a);
   }
   return cudaGetLastError();
 }
@@ -431,8 +454,8 @@ int msda_rotary(int dtype, int64_t batch, int64_t num_tokens, int64_t channels, 
   a.axis = axis_index;
   a.sign = inverse ? -1.f : 1.f;
   a.gpos = grad_positions;
-  a.hop = per_token <= kRotThreads && kRotThreads % per_token == 0
-              ? static_cast<int32_t>(kRotThreads / per_token) : 0;
+  a.hop = static_cast<int32_t>(kRotThreads / per_token);
+  a.step = a.hop == 0 ? kRotThreads : a.hop * static_cast<int32_t>(per_token);
   a.flat = 1;
   for (int i = 0; i < num_tensors; ++i) {
     RotTensor& t = a.t[i];
