@@ -320,7 +320,8 @@ variable_list norm_backward(const Norm& n, const variable_list& xs, const option
   Tensor gw, gb;
   if (affine.weight) gw = at::empty_like(*affine.weight);
   if (affine.bias) gb = at::empty_like(*affine.bias);
-  const size_t bytes = api.norm_workspace(code, batch, channels, n.groups, levels, n.rows.data(), 1);
+  const size_t bytes =
+      api.norm_workspace(code, batch, channels, n.groups, levels, n.rows.data(), 1);
   Tensor ws = empty({static_cast<int64_t>(bytes)}, first, at::kByte);
   check(api.norm_bwd(code, batch, channels, n.groups, levels, n.rows.data(), x.at.data(),
                      x.strides.data(), ptr(affine.weight), ptr(affine.bias), affine.dtype,
@@ -532,7 +533,8 @@ variable_list rotary_backward(at::TensorList grads, at::TensorList inputs, const
 
 class RotaryFn : public torch::autograd::Function<RotaryFn> {
  public:
-  static variable_list forward(AutogradContext* ctx, at::TensorList xs, const Tensor& positions, const Tensor& inv_freq,
+  static variable_list forward(AutogradContext* ctx, at::TensorList xs,
+                               const Tensor& positions, const Tensor& inv_freq,
                                const Tensor& axis_index, bool interleaved) {
     variable_list out = rotary_forward(xs, positions, inv_freq, axis_index, interleaved);
     variable_list saved{positions, inv_freq, axis_index};

@@ -50,7 +50,7 @@ constexpr int kAdamThreads = 256;
 constexpr int kBlock = 128;                                 // elements per exponent
 constexpr int kAdamUnroll = 4;                              // blocks per warp
 constexpr int kChunk = kAdamThreads / 32 * kBlock * kAdamUnroll;  // elements per CTA
-constexpr int kFewTensors = 64, kManyTensors = 640;         // per launch: 4 KB and 32 KB of parameters
+constexpr int kFewTensors = 64, kManyTensors = 640;  // per launch: 4 KB, 32 KB of parameters
 
 struct AdamTensor {
   void* p;
@@ -253,7 +253,8 @@ adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
     const T* g = static_cast<const T*>(t.g) + first;
     const int64_t s0 = static_cast<int64_t>(t.offset) * kBlock + first;
     float* const master = a.master + s0;
-    uint8_t *const m8 = static_cast<uint8_t*>(a.m) + s0, *const v8 = static_cast<uint8_t*>(a.v) + s0;
+    uint8_t* const m8 = static_cast<uint8_t*>(a.m) + s0;
+    uint8_t* const v8 = static_cast<uint8_t*>(a.v) + s0;
     uint8_t *const me = a.me + s0 / kBlock, *const ve = a.ve + s0 / kBlock;
     float *const m32 = static_cast<float*>(a.m) + s0, *const v32 = static_cast<float*>(a.v) + s0;
 

@@ -79,7 +79,8 @@ int make_plan(int dtype, int64_t B, int64_t C, int64_t G, int64_t L, const int64
       if (p.counters > (1 << 29) || p.tiles > (1 << 29))
         return report(MSDA_ERROR_INT32_OVERFLOW, "too many tiles of work");
     }
-    if (p.direct && tile <= kTile && most <= kDirectTiles && (!backward || sum <= kDirectSum)) break;
+    if (p.direct && tile <= kTile && most <= kDirectTiles && (!backward || sum <= kDirectSum))
+      break;
   }
   p.partial_stride = static_cast<int32_t>(sg * (backward ? cg : 1));
   int64_t at = 0;
@@ -136,8 +137,9 @@ int vector_bytes(const NormArgs& a, int64_t es, bool backward) {
   return static_cast<int>(vb);
 }
 
-void fill(NormArgs& a, const Plan& p, int64_t B, int64_t C, int64_t G, int64_t L, const void* weight,
-         const void* bias, int affine_dtype, int affine_per_level, void* workspace) {
+void fill(NormArgs& a, const Plan& p, int64_t B, int64_t C, int64_t G, int64_t L,
+          const void* weight, const void* bias, int affine_dtype, int affine_per_level,
+          void* workspace) {
   std::copy(p.lv, p.lv + L, a.lv);
   a.L = static_cast<int32_t>(L);
   a.C = static_cast<int32_t>(C);

@@ -84,7 +84,8 @@ constexpr int kNormOnceThreads = 512, kNormOnceVectors = 8;
 constexpr int kNormParamChannels = 8;  // of a CTA that sums gradients of the affine map
 
 // Both launches, or (once) the one of units that are one tile each, with
-// vectors of vb bytes (mixed: 16, of several groups); one instance per dtype (msda_norm_{f32,f16,bf16}.cu).
+// vectors of vb bytes (mixed: 16, of several groups); one instance per dtype
+// (msda_norm_{f32,f16,bf16}.cu).
 template <typename T>
 cudaError_t norm_launch(const NormArgs& a, int vb, bool mixed, int act, bool backward, bool once,
                         cudaStream_t st);

@@ -424,10 +424,12 @@ __device__ __forceinline__ void norm_join_here(const NormArgs& a, const NormTile
   while (lanes * t.groups > kNormThreads) lanes >>= 1;
   const int g = threadIdx.x / lanes, j = threadIdx.x & (lanes - 1);
   const bool on = g < t.groups;
-  const float2* q = a.partial + (t.block - static_cast<int64_t>(t.tile) * t.step) * a.partial_stride + g;
+  const float2* q =
+      a.partial + (t.block - static_cast<int64_t>(t.tile) * t.step) * a.partial_stride + g;
   const int64_t next = static_cast<int64_t>(t.step) * a.partial_stride;
   const float full = static_cast<float>(v.tile_rows) * a.cg;
-  const float tail = static_cast<float>(v.rows - static_cast<int64_t>(v.tiles - 1) * v.tile_rows) * a.cg;
+  const float tail =
+      static_cast<float>(v.rows - static_cast<int64_t>(v.tiles - 1) * v.tile_rows) * a.cg;
   const float all = static_cast<float>(v.rows) * a.cg;
   float mu = 0.f, dev = 0.f;
   if (on) {
@@ -481,7 +483,8 @@ __device__ void norm_apply(const NormArgs& a, const NormTile& t) {
       w[i] = mul2(w[i], r2[MIXED ? i : 0]);
       if (sizeof(T) == 2) d[i] = fma2(w[i], minus[MIXED ? i : 0], d[i]);  // as NormCentre
     }
-    const T* p = reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row + c0;
+    const T* p =
+        reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row + c0;
     T* y = reinterpret_cast<T*>(v.out) + v.out_batch * t.b + (t.row0 + me.tr) * v.out_row + c0;
     norm_rows<U>(t, me.tr, [&](auto count) {
       constexpr int K = decltype(count)::value;
@@ -843,7 +846,8 @@ __device__ __forceinline__ void norm_grad_join_here(const NormArgs& a, const Nor
 __device__ __forceinline__ void norm_param_grad(const NormArgs& a, int cta) {
   const int per_row = (a.C + kNormParamChannels - 1) / kNormParamChannels;
   const int row = cta / per_row;
-  const int c = (cta - row * per_row) * kNormParamChannels + (threadIdx.x & (kNormParamChannels - 1));
+  const int c =
+      (cta - row * per_row) * kNormParamChannels + (threadIdx.x & (kNormParamChannels - 1));
   const int lane = threadIdx.x / kNormParamChannels;
   constexpr int kLanes = kNormThreads / kNormParamChannels;
   __shared__ float2 sums[kNormThreads];
@@ -913,7 +917,8 @@ __device__ void norm_grad_apply(const NormArgs& a, const NormTile& t) {
       norm_params<EPV>(a.bias, a.affine_dtype, at, 0.f, f);
       P::of(f, d);
     }
-    const T* p = reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row + c0;
+    const T* p =
+        reinterpret_cast<const T*>(v.x) + v.x_batch * t.b + (t.row0 + me.tr) * v.x_row + c0;
     const T* g =
         reinterpret_cast<const T*>(v.gy) + v.gy_batch * t.b + (t.row0 + me.tr) * v.gy_row + c0;
     T* y = reinterpret_cast<T*>(v.out) + v.out_batch * t.b + (t.row0 + me.tr) * v.out_row + c0;
