@@ -8,8 +8,8 @@
 // if there is one).  With fp32 moments it is bound by memory: 28 bytes a
 // parameter in fp32 (22 in bf16), 335 M of them in 1.35 ms (1.07 ms), 6.9 TB/s.
 // With 8-bit moments and bf16 parameters, 10 bytes a parameter, the coding is:
-// about 77 instructions a parameter, half of them on the integer units that are
-// 78 % busy, 0.87 ms for 335 M (3.8 TB/s; fp32 parameters 0.97 ms, 5.5 TB/s).
+// about 73 instructions a parameter, half of them on the integer units that are
+// 74 % busy, 0.82 ms for 335 M (4.1 TB/s; fp32 parameters 1.00 ms, 5.4 TB/s).
 //
 // States of all tensors lie in one array each; tensor i's elements start at
 // the sum of the earlier tensors' sizes, each rounded up to kBlock.
@@ -60,7 +60,6 @@ struct AdamTensor {
   uint32_t key;
   uint32_t offset;  // of its states, in blocks
   uint32_t cta0;    // first CTA of the launch
-  uint32_t ctas;
 };
 
 struct AdamArgs {
@@ -73,12 +72,18 @@ struct AdamArgs {
   void *m, *v;
   uint8_t *me, *ve;
   float* master;
-  int32_t tensors;
-  int32_t rounds;  // of kChunk elements per CTA
 };
+
+// A CTA looks for its tensor among those of its part of the grid.  By a search
+// over all tensors this cost seven instructions an element, which two rounds of
+// elements a CTA would have halved; the loop over rounds then cost more than the
+// search (335 M bf16 parameters, 8 bits: 875 us against 818).
+constexpr int kAdamParts = 64;
 
 template <int N> struct AdamTable {
   AdamArgs a;
+  int32_t part_shift;              // of a CTA's index
+  uint16_t first[kAdamParts + 1];  // tensor of each part's first CTA
   AdamTensor t[N];
 };
 
@@ -221,7 +226,9 @@ __global__ void __launch_bounds__(kAdamThreads)
 adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
   constexpr int U = kAdamUnroll;
   const AdamArgs& a = tab.a;
-  int lo = 0, hi = a.tensors;  // the last tensor whose first CTA is not after this one
+  // the last tensor whose first CTA is not after this one
+  const int part = blockIdx.x >> tab.part_shift;
+  int lo = tab.first[part], hi = tab.first[part + 1] + 1;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (tab.t[mid].cta0 <= blockIdx.x) lo = mid;
@@ -238,102 +245,97 @@ adamw_kernel(const __grid_constant__ AdamTable<N> tab) {
   const bool vec = (reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g)) %
                        (4 * sizeof(T)) == 0;
 
-  // rounds of neighbouring CTAs lie side by side: with a CTA's own rounds next
-  // to one another, all CTAs at once touch every other 4 KB of the codes, and
-  // half of the memory channels (1726 us)
-  for (int round = 0; round < a.rounds; ++round) {
-    const int64_t first =
-        static_cast<int64_t>(blockIdx.x - t.cta0 + round * t.ctas) * kChunk +
-        (threadIdx.x >> 5) * (kBlock * U) + lane * 4;
-    // elements from this lane's first one to the tensor's end
-    const int left = static_cast<int>(max(min(t.n - first, static_cast<int64_t>(kChunk)),
-                                          -static_cast<int64_t>(kChunk)));
-    if (left + lane * 4 <= 0) return;  // the whole warp
-    T* p = static_cast<T*>(t.p) + first;
-    const T* g = static_cast<const T*>(t.g) + first;
-    const int64_t s0 = static_cast<int64_t>(t.offset) * kBlock + first;
-    float* const master = a.master + s0;
-    uint8_t* const m8 = static_cast<uint8_t*>(a.m) + s0;
-    uint8_t* const v8 = static_cast<uint8_t*>(a.v) + s0;
-    uint8_t *const me = a.me + s0 / kBlock, *const ve = a.ve + s0 / kBlock;
-    float *const m32 = static_cast<float*>(a.m) + s0, *const v32 = static_cast<float*>(a.v) + s0;
+  const int64_t first =
+      static_cast<int64_t>(blockIdx.x - t.cta0) * kChunk +
+      (threadIdx.x >> 5) * (kBlock * U) + lane * 4;
+  // elements from this lane's first one to the tensor's end
+  const int left = static_cast<int>(max(min(t.n - first, static_cast<int64_t>(kChunk)),
+                                        -static_cast<int64_t>(kChunk)));
+  if (left + lane * 4 <= 0) return;  // the whole warp
+  T* p = static_cast<T*>(t.p) + first;
+  const T* g = static_cast<const T*>(t.g) + first;
+  const int64_t s0 = static_cast<int64_t>(t.offset) * kBlock + first;
+  float* const master = a.master + s0;
+  uint8_t* const m8 = static_cast<uint8_t*>(a.m) + s0;
+  uint8_t* const v8 = static_cast<uint8_t*>(a.v) + s0;
+  uint8_t *const me = a.me + s0 / kBlock, *const ve = a.ve + s0 / kBlock;
+  float *const m32 = static_cast<float*>(a.m) + s0, *const v32 = static_cast<float*>(a.v) + s0;
 
-    // everything is on its way before the first use
-    Raw<4 * sizeof(T)> rg[U], rp[U];
-    Raw<16> rx[U], rm[U], rv[U];
-    uint32_t cm[U], cv[U], em[U], ev[U];
+  // everything is on its way before the first use
+  Raw<4 * sizeof(T)> rg[U], rp[U];
+  Raw<16> rx[U], rm[U], rv[U];
+  uint32_t cm[U], cv[U], em[U], ev[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int valid = left - u * kBlock;
-      if (valid + lane * 4 <= 0) continue;  // the whole warp: a block that is not there
-      rg[u] = adam_load(g + u * kBlock, min(valid, 4), vec);
-      if (MASTER) rx[u] = adam_load(master + u * kBlock, 4, true);
-      else rp[u] = adam_load(p + u * kBlock, min(valid, 4), vec);
-      if (SMALL) {
-        cm[u] = *reinterpret_cast<const uint32_t*>(m8 + u * kBlock);
-        cv[u] = *reinterpret_cast<const uint32_t*>(v8 + u * kBlock);
-        em[u] = me[u];
-        ev[u] = ve[u];
-      } else {
-        rm[u] = adam_load(m32 + u * kBlock, 4, true);
-        rv[u] = adam_load(v32 + u * kBlock, 4, true);
-      }
+  for (int u = 0; u < U; ++u) {
+    const int valid = left - u * kBlock;
+    if (valid + lane * 4 <= 0) continue;  // the whole warp: a block that is not there
+    rg[u] = adam_load(g + u * kBlock, min(valid, 4), vec);
+    if (MASTER) rx[u] = adam_load(master + u * kBlock, 4, true);
+    else rp[u] = adam_load(p + u * kBlock, min(valid, 4), vec);
+    if (SMALL) {
+      cm[u] = *reinterpret_cast<const uint32_t*>(m8 + u * kBlock);
+      cv[u] = *reinterpret_cast<const uint32_t*>(v8 + u * kBlock);
+      em[u] = me[u];
+      ev[u] = ve[u];
+    } else {
+      rm[u] = adam_load(m32 + u * kBlock, 4, true);
+      rv[u] = adam_load(v32 + u * kBlock, 4, true);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int valid = left - u * kBlock;
+    if (valid + lane * 4 <= 0) return;
+    float x[4], d[4], m[4], v[4];
+    Chunk<T, 4 * sizeof(T)>::unpack(rg[u], d);
+    if (MASTER) Chunk<float, 16>::unpack(rx[u], x);
+    else Chunk<T, 4 * sizeof(T)>::unpack(rp[u], x);
+    if (SMALL) {
+      adam_decode(cm[u], cv[u], em[u], ev[u], m, v);
+    } else {
+      Chunk<float, 16>::unpack(rm[u], m);
+      Chunk<float, 16>::unpack(rv[u], v);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int valid = left - u * kBlock;
-      if (valid + lane * 4 <= 0) return;
-      float x[4], d[4], m[4], v[4];
-      Chunk<T, 4 * sizeof(T)>::unpack(rg[u], d);
-      if (MASTER) Chunk<float, 16>::unpack(rx[u], x);
-      else Chunk<T, 4 * sizeof(T)>::unpack(rp[u], x);
-      if (SMALL) {
-        adam_decode(cm[u], cv[u], em[u], ev[u], m, v);
-      } else {
-        Chunk<float, 16>::unpack(rm[u], m);
-        Chunk<float, 16>::unpack(rv[u], v);
-      }
+    for (int i = 0; i < 4; i += 2) {
+      uint64_t e = mul2(pair(d[i], d[i + 1]), gs);
+      uint64_t mm = pair(m[i], m[i + 1]), vv = pair(v[i], v[i + 1]);
+      mm = fma2(c1, fma2(l1, mm, e), mul2(k1, mm));
+      e = mul2(e, e);
+      vv = fma2(c2, fma2(l2, vv, e), mul2(k2, vv));
+      unpair(mm, m[i], m[i + 1]);
+      unpair(vv, v[i], v[i + 1]);
+      float den[2];
+      unpair(fma2(pair(adam_sqrt(v[i]), adam_sqrt(v[i + 1])), bc, eps), den[0], den[1]);
+      const uint64_t q = mul2(mm, pair(adam_rcp(den[0]), adam_rcp(den[1])));
+      unpair(fma2(size, q, mul2(decay, pair(x[i], x[i + 1]))), x[i], x[i + 1]);
+    }
+    if (valid < 4) {  // between tensors
 #pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        uint64_t e = mul2(pair(d[i], d[i + 1]), gs);
-        uint64_t mm = pair(m[i], m[i + 1]), vv = pair(v[i], v[i + 1]);
-        mm = fma2(c1, fma2(l1, mm, e), mul2(k1, mm));
-        e = mul2(e, e);
-        vv = fma2(c2, fma2(l2, vv, e), mul2(k2, vv));
-        unpair(mm, m[i], m[i + 1]);
-        unpair(vv, v[i], v[i + 1]);
-        float den[2];
-        unpair(fma2(pair(adam_sqrt(v[i]), adam_sqrt(v[i + 1])), bc, eps), den[0], den[1]);
-        const uint64_t q = mul2(mm, pair(adam_rcp(den[0]), adam_rcp(den[1])));
-        unpair(fma2(size, q, mul2(decay, pair(x[i], x[i + 1]))), x[i], x[i + 1]);
-      }
-      if (valid < 4) {  // between tensors
+      for (int i = 0; i < 4; ++i)
+        if (i >= valid) m[i] = v[i] = x[i] = 0.f;
+    }
+    adam_store(p + u * kBlock, min(valid, 4), vec, x);
+    if (MASTER) adam_store(master + u * kBlock, 4, true, x);
+    if (SMALL) {
+      uint32_t qm[4], qv[4], nm, nv;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i >= valid) m[i] = v[i] = x[i] = 0.f;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t r = adam_random(static_cast<uint32_t>(s0) + u * kBlock + i, t.key);
+        qm[i] = r & 0xffffu;
+        qv[i] = r >> 16;
       }
-      adam_store(p + u * kBlock, min(valid, 4), vec, x);
-      if (MASTER) adam_store(master + u * kBlock, 4, true, x);
-      if (SMALL) {
-        uint32_t qm[4], qv[4], nm, nv;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t r = adam_random(static_cast<uint32_t>(s0) + u * kBlock + i, t.key);
-          qm[i] = r & 0xffffu;
-          qv[i] = r >> 16;
-        }
-        const uint32_t wm = adam_encode<15u, true>(m, qm, nm);
-        const uint32_t wv = adam_encode<31u, false>(v, qv, nv);
-        *reinterpret_cast<uint32_t*>(m8 + u * kBlock) = wm;
-        *reinterpret_cast<uint32_t*>(v8 + u * kBlock) = wv;
-        if (lane == 0) {
-          me[u] = static_cast<uint8_t>(nm);
-          ve[u] = static_cast<uint8_t>(nv);
-        }
-      } else {
-        adam_store(m32 + u * kBlock, 4, true, m);
-        adam_store(v32 + u * kBlock, 4, true, v);
+      const uint32_t wm = adam_encode<15u, true>(m, qm, nm);
+      const uint32_t wv = adam_encode<31u, false>(v, qv, nv);
+      *reinterpret_cast<uint32_t*>(m8 + u * kBlock) = wm;
+      *reinterpret_cast<uint32_t*>(v8 + u * kBlock) = wv;
+      if (lane == 0) {
+        me[u] = static_cast<uint8_t>(nm);
+        ve[u] = static_cast<uint8_t>(nv);
       }
+    } else {
+      adam_store(m32 + u * kBlock, 4, true, m);
+      adam_store(v32 + u * kBlock, 4, true, v);
     }
   }
 }
@@ -382,14 +384,19 @@ struct Step {
 template <int N> cudaError_t adamw_all(const Step& s, const AdamArgs& args, cudaStream_t st) {
   AdamTable<N> tab;
   tab.a = args;
-  const int64_t per_cta = static_cast<int64_t>(kChunk) * args.rounds;
   int used = 0;
   int64_t chunks = 0, offset = 0, known = -1;
   float step_size = 0.f, inv_sqrt_bc2 = 0.f;
   auto flush = [&]() {
     if (used == 0) return cudaSuccess;
-    tab.a.tensors = used;
     const unsigned int grid = static_cast<unsigned int>(chunks);
+    tab.part_shift = 0;
+    while ((grid - 1) >> tab.part_shift >= kAdamParts) ++tab.part_shift;
+    for (int part = 0, i = 0; part <= kAdamParts; ++part) {
+      while (i + 1 < used && tab.t[i + 1].cta0 <= static_cast<uint64_t>(part) << tab.part_shift)
+        ++i;
+      tab.first[part] = static_cast<uint16_t>(i);
+    }
     used = 0;
     chunks = 0;
     if (s.dtype == MSDA_FLOAT32) return adamw_launch<float, N>(tab, s.small, grid, st);
@@ -406,15 +413,14 @@ template <int N> cudaError_t adamw_all(const Step& s, const AdamArgs& args, cuda
       step_size = static_cast<float>(s.lr / (1.0 - std::pow(s.b1, t)));
       inv_sqrt_bc2 = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(s.b2, t)));
     }
-    const int64_t own = (n + per_cta - 1) / per_cta;
+    const int64_t own = (n + kChunk - 1) / kChunk;
     if (used == N || chunks + own > 0x7fffffff) {
       const cudaError_t err = flush();
       if (err != cudaSuccess) return err;
     }
     tab.t[used++] = AdamTensor{s.params[i], s.grads[i], n, step_size, inv_sqrt_bc2,
                                s.seed + static_cast<uint32_t>(known) * 0x632be5abu,
-                               static_cast<uint32_t>(at / kBlock), static_cast<uint32_t>(chunks),
-                               static_cast<uint32_t>(own)};
+                               static_cast<uint32_t>(at / kBlock), static_cast<uint32_t>(chunks)};
     chunks += own;
   }
   return flush();
@@ -480,11 +486,6 @@ int msda_adamw_step(int dtype, int state_bits, int64_t num_tensors, void* const*
   a.me = exp_avg_exponent;
   a.ve = exp_avg_sq_exponent;
   a.master = master;
-  // Two rounds a CTA for 8-bit states, whose kernel is bound by instructions
-  // (finding the tensor costs seven an element in one round: 909 us against
-  // 875 for 335 M bf16 parameters), where each SM still gets many CTAs; one
-  // where memory is the bound (fp32 states: 1070 us against 1082).
-  a.rounds = small && total >= int64_t{148} * 64 * kChunk ? 2 : 1;
   const Step s{dtype, small, num_tensors, params, grads, counts, steps, lr, beta1, beta2, seed};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // a launch copies its parameters: the short table where it is enough
