@@ -249,7 +249,7 @@ def test_many_tensors_and_missing_gradients(bits):
 
 @pytest.mark.parametrize("bits,dt", [(8, torch.bfloat16), (32, torch.float32)])
 def test_large_tensor(bits, dt):
-    """Sizes at which a CTA takes several rounds, with a ragged end."""
+    """Many CTAs for one tensor, with a ragged end."""
     n = 148 * 64 * 4096 + 4096 * 3 + 77
     gen = torch.Generator(device=DEV).manual_seed(0)
     p = torch.randn(n, generator=gen, device=DEV).to(dt)
