@@ -124,6 +124,16 @@ def adamw_state_values(state: dict[str, Tensor]) -> tuple[Tensor, Tensor]:
     return _lib.binding().adamw_values(state)
 
 
+def _refuse_other_updates(group: dict) -> None:
+    """ValueError for a group that asks for another update than AdamW's."""
+    for key in ("maximize", "amsgrad"):
+        if group.get(key):
+            raise ValueError(f"AdamW has no {key}: a group with {key}=True is another update")
+    if not group.get("decoupled_weight_decay", True) and group.get("weight_decay", 0) != 0:
+        raise ValueError("a group with decoupled_weight_decay=False and a weight_decay of "
+                         f"{group['weight_decay']} is another update than AdamW's")
+
+
 class _Part:
     """The parameters of one group that share a dtype and device, and their states."""
 
@@ -168,8 +178,9 @@ class AdamW(torch.optim.Optimizer):
 
     Parameters without a gradient are skipped, and count their own steps.  A
     state_dict of torch.optim.AdamW can be loaded where state_bits is 32; an
-    8-bit one holds the codes and exponents themselves.  `step` cannot be
-    captured in a CUDA graph.
+    8-bit one holds the codes and exponents themselves.  A group that asks for
+    another update (maximize, amsgrad, a decay that is not decoupled) is a
+    ValueError.  `step` cannot be captured in a CUDA graph.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
@@ -189,6 +200,11 @@ class AdamW(torch.optim.Optimizer):
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed,
                 "master_weights": self.master_weights, "_parts": self._parts}
+
+    def add_param_group(self, param_group: dict) -> None:
+        """As torch.optim.Optimizer's."""
+        _refuse_other_updates({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def _allocate(self) -> None:
         """States for groups that have none yet (the first step, or a group added later)."""
@@ -236,6 +252,8 @@ class AdamW(torch.optim.Optimizer):
         """Hyperparameters and states of a state_dict of this optimizer's (or, with 32-bit
         states, of torch.optim.AdamW's) over the same parameters."""
         groups = state_dict["param_groups"]
+        for group in groups:
+            _refuse_other_updates(group)
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the state_dict's parameter groups differ from the optimizer's")
         self._allocate()

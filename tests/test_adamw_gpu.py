@@ -398,6 +398,45 @@ def test_loads_torch_state():
         msda.AdamW(b.parameters()).load_state_dict(theirs.state_dict())
 
 
+@pytest.mark.parametrize("theirs,text", [
+    (lambda ps: torch.optim.AdamW(ps, lr=1e-3, maximize=True), "maximize"),
+    (lambda ps: torch.optim.AdamW(ps, lr=1e-3, amsgrad=True), "amsgrad"),
+    (lambda ps: torch.optim.Adam(ps, lr=1e-3, weight_decay=0.1), "decoupled_weight_decay"),
+], ids=["maximize", "amsgrad", "coupled"])
+def test_refuses_the_state_of_another_update(theirs, text):
+    """A state_dict whose update is another one is refused, and changes nothing."""
+    a, b = model(), model(1)
+    opt = theirs(a.parameters())
+    train(a, opt, 2)
+    ours = msda.AdamW(b.parameters(), lr=5e-3, weight_decay=0.0)
+    train(b, ours, 2)
+    before = copy.deepcopy(ours.state_dict())
+    with pytest.raises(ValueError, match=text):
+        ours.load_state_dict(opt.state_dict())
+    after = ours.state_dict()
+    assert after["param_groups"] == before["param_groups"]
+    for i, s in before["state"].items():
+        assert all(torch.equal(torch.as_tensor(v), torch.as_tensor(after["state"][i][k]))
+                   for k, v in s.items())
+    with pytest.raises(ValueError, match=text):
+        group = {k: v for k, v in opt.state_dict()["param_groups"][0].items() if k != "params"}
+        msda.AdamW([{**group, "params": list(b.parameters())}])
+
+
+def test_loads_adam_without_decay():
+    """Without decay Adam's update is AdamW's."""
+    a, b = model(), model()
+    theirs = torch.optim.Adam(a.parameters(), lr=1e-3)
+    train(a, theirs, 3)
+    b.load_state_dict(a.state_dict())
+    ours = msda.AdamW(b.parameters())
+    ours.load_state_dict(theirs.state_dict())
+    train(a, theirs, 3, 3)
+    train(b, ours, 3, 3)
+    for p, q in zip(a.parameters(), b.parameters()):
+        torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-6)
+
+
 def test_parameters_without_gradient_count_their_own_steps():
     a, b = model(), model()
     ours, theirs = msda.AdamW(a.parameters(), lr=1e-2), torch.optim.AdamW(b.parameters(), lr=1e-2)
