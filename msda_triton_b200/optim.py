@@ -10,6 +10,7 @@ CPU fallback.
 
 from __future__ import annotations
 
+import copy
 from collections.abc import Sequence
 
 import torch
@@ -122,6 +123,10 @@ def adamw_state_values(state: dict[str, Tensor]) -> tuple[Tensor, Tensor]:
     """(exp_avg, exp_avg_sq) that a state stands for, flat as the state is.
     8-bit moments come as bf16, which holds them exactly; fp32 ones as they are."""
     return _lib.binding().adamw_values(state)
+
+
+# What torch's Adam family keeps in its groups for other updates than this one.
+_OTHER_UPDATES = ("maximize", "amsgrad", "decoupled_weight_decay")
 
 
 def _refuse_other_updates(group: dict) -> None:
@@ -250,7 +255,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """Hyperparameters and states of a state_dict of this optimizer's (or, with 32-bit
-        states, of torch.optim.AdamW's) over the same parameters."""
+        states, of torch.optim.AdamW's) over the same parameters.  Every key of a group is
+        taken over."""
         groups = state_dict["param_groups"]
         for group in groups:
             _refuse_other_updates(group)
@@ -287,9 +293,8 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     t.zero_()
         for saved, group in zip(groups, self.param_groups):
-            for key in ("lr", "betas", "eps", "weight_decay"):
-                if key in saved:
-                    group[key] = saved[key]
+            group.update((key, copy.deepcopy(value)) for key, value in saved.items()
+                         if key not in ("params", "param_names", *_OTHER_UPDATES))
 
 
 __all__ = ["AdamW", "adamw_step", "adamw_state", "adamw_state_values"]

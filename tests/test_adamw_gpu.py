@@ -437,6 +437,26 @@ def test_loads_adam_without_decay():
         torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-6)
 
 
+def test_keeps_every_key_of_a_group():
+    """A scheduler that goes on where another ended finds initial_lr, and a user's keys stay."""
+    net, other = model(), model()
+    opt = msda.AdamW([{"params": net.parameters(), "tag": ["all"]}], lr=1e-2)
+    halve = lambda o, **kw: torch.optim.lr_scheduler.LambdaLR(o, lambda t: 0.5 ** t, **kw)  # noqa: E731
+    scheduler = halve(opt)
+    for t in range(3):
+        train(net, opt, 1, t)
+        scheduler.step()
+    saved = opt.state_dict()
+    opt2 = msda.AdamW(other.parameters(), lr=9.0)
+    opt2.load_state_dict(saved)
+    group = opt2.param_groups[0]
+    assert group["initial_lr"] == 1e-2 and group["tag"] == ["all"]
+    assert group["params"][0] is next(other.parameters())
+    assert group["tag"] is not opt.param_groups[0]["tag"]
+    halve(opt2, last_epoch=3)
+    assert group["lr"] == pytest.approx(1e-2 * 0.5 ** 4)
+
+
 def test_parameters_without_gradient_count_their_own_steps():
     a, b = model(), model()
     ours, theirs = msda.AdamW(a.parameters(), lr=1e-2), torch.optim.AdamW(b.parameters(), lr=1e-2)
