@@ -257,6 +257,10 @@ class AdamW(torch.optim.Optimizer):
         """Hyperparameters and states of a state_dict of this optimizer's (or, with 32-bit
         states, of torch.optim.AdamW's) over the same parameters.  Every key of a group is
         taken over."""
+        state_dict = state_dict.copy()
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            replaced = hook(self, state_dict)
+            state_dict = state_dict if replaced is None else replaced
         groups = state_dict["param_groups"]
         for group in groups:
             _refuse_other_updates(group)
@@ -295,6 +299,8 @@ class AdamW(torch.optim.Optimizer):
         for saved, group in zip(groups, self.param_groups):
             group.update((key, copy.deepcopy(value)) for key, value in saved.items()
                          if key not in ("params", "param_names", *_OTHER_UPDATES))
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
 
 __all__ = ["AdamW", "adamw_step", "adamw_state", "adamw_state_values"]

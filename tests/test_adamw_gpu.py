@@ -457,6 +457,23 @@ def test_keeps_every_key_of_a_group():
     assert group["lr"] == pytest.approx(1e-2 * 0.5 ** 4)
 
 
+def test_load_hooks_run():
+    net, other = model(), model()
+    opt = msda.AdamW(net.parameters(), lr=1e-2)
+    train(net, opt, 2)
+    opt2, seen = msda.AdamW(other.parameters()), []
+
+    def before(o, d):
+        seen.append(len(o.state_dict()["state"]))
+        return {**d, "param_groups": [{**g, "lr": 0.25} for g in d["param_groups"]]}
+
+    opt2.register_load_state_dict_pre_hook(before)
+    opt2.register_load_state_dict_post_hook(lambda o: seen.append(len(o.state_dict()["state"])))
+    opt2.load_state_dict(opt.state_dict())
+    assert seen == [0, 4] and opt2.param_groups[0]["lr"] == 0.25
+    assert opt.param_groups[0]["lr"] == 1e-2
+
+
 def test_parameters_without_gradient_count_their_own_steps():
     a, b = model(), model()
     ours, theirs = msda.AdamW(a.parameters(), lr=1e-2), torch.optim.AdamW(b.parameters(), lr=1e-2)
