@@ -526,6 +526,18 @@ def test_autograd_sees_the_change():
         out.backward()
 
 
+def test_no_forward_mode_derivative():
+    from torch.autograd import forward_ad
+
+    p, g = torch.ones(4, device=DEV), torch.ones(4, device=DEV)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(p, torch.ones_like(p))
+        for ps, gs in (([dual], [g]), ([p], [dual])):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                msda.adamw_step(ps, gs, msda.adamw_state([p]), step=1)
+    assert torch.equal(p, g)
+
+
 def test_capture_is_refused():
     p = torch.ones(4, device=DEV)
     state = msda.adamw_state([p])

@@ -301,6 +301,30 @@ def test_no_second_derivative():
         torch.autograd.grad(gx.square().sum(), x)
 
 
+def test_no_forward_mode_derivative():
+    """A tangent is refused, not dropped: of any input, of the gradient, of a transformed call."""
+    from torch.autograd import forward_ad
+
+    x = features(1, [6], 8, torch.float32)
+    w, b = affine((8,))
+    run = lambda *a: msda.pyramid_group_norm(a[0], [(6,)], 2, *a[1:])  # noqa: E731
+    y = run(x.requires_grad_(True), w, b)
+    with forward_ad.dual_level():
+        for i in range(3):
+            args = [x.detach(), w, b]
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            for call in (run, lambda *a: msda.pyramid_group_norm([a[0]], None, 2, *a[1:])):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*args)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                msda.ops.group_norm_forward([args[0]], True, None, 2, *args[1:], 1e-5, "none")
+        g = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, x, g)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(run, (x.detach(), w, b), (torch.ones_like(x), w, b))
+
+
 def test_module_stream_and_graph():
     """On a stream of its own, and captured in a CUDA graph: the same bits as by itself."""
     rows = [900, 200]

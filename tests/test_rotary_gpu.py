@@ -205,6 +205,30 @@ def test_no_second_derivative():
         torch.autograd.grad(gx.sum(), g)
 
 
+def test_no_forward_mode_derivative():
+    """A tangent is refused, not dropped: of any input, of the gradient, of a transformed call."""
+    from torch.autograd import forward_ad
+
+    (x,), pos, freq, axis = make(1, 4, (2,), 8, torch.float32)
+    y = msda.rotary(x.requires_grad_(True), pos, freq, axis)
+    with forward_ad.dual_level():
+        for i in range(3):
+            args = [x.detach(), pos, freq]
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            for call in (msda.rotary, lambda a, *r: msda.rotary_qk(a, a, *r),
+                         lambda a, *r: msda.rotary_qk(x.detach(), a, *r),
+                         lambda a, *r: msda.rotary_qk_(a, a.clone(), *r),
+                         lambda a, *r: msda.ops.rotary_forward([a], *r, False)):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*args, axis)
+        g = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, x, g)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda a: msda.rotary(a, pos, freq, axis), (x.detach(),),
+                       (torch.ones_like(x),))
+
+
 def test_zero_is_no_turn_and_lengths_stay():
     xs, pos, freq, axis = make(2, 20, (4,), 32, torch.float32)
     assert torch.equal(msda.rotary(xs[0], torch.zeros_like(pos), freq, axis), xs[0])
