@@ -432,6 +432,8 @@ Tensor rotary_check(at::TensorList xs, const Tensor& positions, const Tensor& in
   dtype_code(first, "rotary");
   no_tangents(xs, "rotary");
   no_tangents({positions, inv_freq}, "rotary");
+  TORCH_CHECK(!at::GradMode::is_enabled() || !inv_freq.requires_grad(),
+              "rotary forms no gradient for inv_freq: detach it");
   TORCH_CHECK_VALUE(first.dim() == 4, "expected (B, Q, H, C), got ", first.sizes());
   const int64_t B = first.size(0), Q = first.size(1), C = first.size(3);
   for (const Tensor& x : xs)

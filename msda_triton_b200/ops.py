@@ -227,6 +227,8 @@ def _rotary_backward_fake(grads, inputs, positions, inv_freq, axis_index, interl
 
 def _rotary_setup(ctx, inputs, output):
     xs, positions, inv_freq, axis_index, interleaved = inputs
+    if inv_freq.requires_grad:
+        raise RuntimeError("rotary forms no gradient for inv_freq: detach it")
     ctx.count, ctx.interleaved = len(xs), interleaved
     ctx.save_for_backward(positions, inv_freq, axis_index,
                           *(xs if positions.requires_grad else ()))

@@ -82,7 +82,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
         x: fp32, fp16 or bf16; any strides with dense channels are read in place.
         positions: (Q, A) or (1 or B, Q, A), A = 1 to 4 axes; fp32, or integers
             (exact up to 2^24); other floating types are converted to fp32.
-        inv_freq: (pairs,) fp32 angle per unit of position.
+        inv_freq: (pairs,) fp32 angle per unit of position; a constant.
         axis_index: (pairs,) int32, each in [0, A); it stays on the device, so
             a pair with another index is no error but becomes NaN.
         interleaved: pairs are channels (2j, 2j + 1) instead of (j, j + pairs).
@@ -92,7 +92,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
 
     Raises:
         ValueError: CPU tensors, shapes that do not fit.
-        NotImplementedError: dtype other than fp32/fp16/bf16.
+        NotImplementedError: dtype other than fp32/fp16/bf16; a forward-mode tangent.
+        RuntimeError: an inv_freq that requires a gradient.
     """
     if torch.compiler.is_compiling():
         return _traced((x,), positions, inv_freq, axis_index, interleaved)[0]

@@ -229,6 +229,26 @@ def test_no_forward_mode_derivative():
                        (torch.ones_like(x),))
 
 
+def test_frequencies_have_no_gradient():
+    """Learned frequencies are refused where their gradient would be missing, in every form."""
+    (q,), pos, freq, axis = make(1, 4, (2,), 8, torch.float32)
+    want = msda.rotary(q, pos, freq, axis)
+    freq.requires_grad_(True)
+    forms = (lambda x: msda.rotary(x, pos, freq, axis),
+             lambda x: msda.rotary_qk(x, x, pos, freq, axis),
+             lambda x: msda.rotary_qk_(x.detach().clone(), x.detach().clone(), pos, freq, axis),
+             lambda x: msda.ops.rotary_forward([x], pos[None] if pos.dim() == 2 else pos, freq,
+                                               axis, False),
+             torch.compile(lambda x: msda.rotary(x, pos, freq, axis) + 1, fullgraph=True))
+    for x in (q, q.clone().requires_grad_(True)):
+        for form in forms:
+            with pytest.raises(RuntimeError, match="no gradient for inv_freq"):
+                form(x)
+    with torch.no_grad():
+        assert torch.equal(msda.rotary(q, pos, freq, axis), want)
+    assert torch.equal(msda.rotary(q, pos, freq.detach(), axis), want)
+
+
 def test_zero_is_no_turn_and_lengths_stay():
     xs, pos, freq, axis = make(2, 20, (4,), 32, torch.float32)
     assert torch.equal(msda.rotary(xs[0], torch.zeros_like(pos), freq, axis), xs[0])
