@@ -26,8 +26,10 @@
 // unit's.  Both go in tile order whichever CTA is last, so results
 // do not depend on the schedule.  Statistics are carried in fp32 as (count,
 // mean, sum of squared deviations): each thread takes the mean and deviations
-// of a chunk of rows in registers, and chunks, threads and tiles are joined
-// pairwise (Chan, Golub, LeVeque), so a mean far from zero costs no digits.
+// of a chunk of rows in registers, chunks and threads are joined pairwise (Chan,
+// Golub, LeVeque), and tiles by what their means lie off the first tile's.  So
+// a mean far from zero costs no digits but those of its own last place, and
+// elements that are all the same have that value as their mean.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -30,6 +30,22 @@ template <int VB> __device__ __forceinline__ void norm_st(void* p, const Raw<VB>
 
 template <int K> struct Count { static constexpr int value = K; };
 
+// -x twice, as a pair (a vector of a single element has no second half), where
+// T is fp32; else zeros.  A chunk's mean is taken from what its elements lie off
+// its first one: a sum of 32 elements of 31000 is off by several units of its
+// last place, and their mean then by as many of its own, 0.004.  Such sums of
+// 16-bit elements are exact.
+template <typename T, int EPV> __device__ __forceinline__ uint64_t norm_off(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  return sizeof(T) == 2 ? 0 : pair(-a, EPV == 1 ? 0.f : -a);
+}
+__device__ __forceinline__ float norm_first(uint64_t off) {
+  float a, b;
+  unpair(off, a, b);
+  return -a;
+}
+
 // EPV parameters from element i on.
 template <int EPV>
 __device__ __forceinline__ void norm_params(const void* p, int dtype, int64_t i, float none,
@@ -293,17 +309,20 @@ __device__ void norm_stats(const NormArgs& a, const NormTile& t) {
 #pragma unroll
         for (int u = 0; u < K; ++u) w[u] = norm_ld<VB>(p + u * hop);
         p += K * hop;
-        uint64_t s = 0, q = 0;  // two zeros
+        uint64_t s = 0, q = 0, off = 0;  // two zeros
 #pragma unroll
         for (int u = 0; u < K; ++u) {
           uint64_t f[P::N];
           P::unpack(w[u], f);
+          if (u == 0) off = norm_off<T, EPV>(f[0]);
 #pragma unroll
-          for (int i = 0; i < P::N; ++i) s = add2(s, f[i]);
+          for (int i = 0; i < P::N; ++i)
+            s = add2(s, sizeof(T) == 2 ? f[i] : add2(f[i], off));
         }
         float sa, sb;
         unpair(s, sa, sb);
-        const float cm = (sa + sb) * (1.f / (K * EPV));
+        float cm = (sa + sb) * (1.f / (K * EPV));
+        if (sizeof(T) == 4) cm += norm_first(off);
         // a single element's second half is no element
         const uint64_t minus = pair(-cm, EPV == 1 ? 0.f : -cm);
 #pragma unroll
@@ -358,15 +377,18 @@ __device__ void norm_stats(const NormArgs& a, const NormTile& t) {
   if (DIRECT) return;
   norm_join_tiles(a, t, [&](int slot, int next, int count, int64_t full, int64_t tail,
                             bool final) {
-    // the mean of the means, then the deviations from it
+    // the mean of the means, as what they lie off the first, then the deviations
+    // from it
     const float nf = static_cast<float>(full) * a.cg, nt = static_cast<float>(tail) * a.cg;
     const float all = nf * (count - 1) + nt;
     const float2* q = mine + slot * next_tile;
+    const float near = on ? __ldcg(&q->x) : 0.f;
     float mu = 0.f, dev = 0.f;
     if (on)
       for (int k = j; k < count; k += lanes)
-        mu += __ldcg(&q[k * next * next_tile].x) * ((k + 1 < count ? nf : nt) / all);
+        mu += (__ldcg(&q[k * next * next_tile].x) - near) * ((k + 1 < count ? nf : nt) / all);
     for (int d = 1; d < lanes; d <<= 1) mu += __shfl_xor_sync(~0u, mu, d);
+    mu += near;
     if (on)
       for (int k = j; k < count; k += lanes) {
         const float2 o = __ldcg(q + k * next * next_tile);
@@ -416,7 +438,8 @@ template <typename T, int EPV, bool MIXED> struct NormCentre {
 };
 
 // The statistics of a tile's groups from its unit's partial results (direct):
-// the mean of the means, then the deviations from it.
+// the mean of the means, as what they lie off the first, then the deviations
+// from it.
 __device__ __forceinline__ void norm_join_here(const NormArgs& a, const NormTile& t,
                                                const NormThread& me, float2* st) {
   const NormLevel& v = a.lv[t.l];
@@ -431,13 +454,15 @@ __device__ __forceinline__ void norm_join_here(const NormArgs& a, const NormTile
   const float tail =
       static_cast<float>(v.rows - static_cast<int64_t>(v.tiles - 1) * v.tile_rows) * a.cg;
   const float all = static_cast<float>(v.rows) * a.cg;
+  const float near = on ? __ldcg(&q->x) : 0.f;
   float mu = 0.f, dev = 0.f;
   if (on) {
 #pragma unroll 4
     for (int k = j; k < v.tiles; k += lanes)
-      mu += __ldcg(&q[k * next].x) * ((k + 1 < v.tiles ? full : tail) / all);
+      mu += (__ldcg(&q[k * next].x) - near) * ((k + 1 < v.tiles ? full : tail) / all);
   }
   for (int d = 1; d < lanes; d <<= 1) mu += __shfl_xor_sync(~0u, mu, d);
+  mu += near;
   if (on) {
 #pragma unroll 4
     for (int k = j; k < v.tiles; k += lanes) {
@@ -530,18 +555,20 @@ norm_once_kernel(const __grid_constant__ NormArgs a) {
     if (u < mine) w[u] = norm_ld<VB>(p + u * hop);
   float n = static_cast<float>(mine * EPV), mean = 0.f, m2 = 0.f;
   if (mine > 0) {
-    uint64_t s = 0, q = 0;  // two zeros
+    uint64_t s = 0, q = 0, off = 0;  // two zeros
 #pragma unroll
     for (int u = 0; u < K; ++u)
       if (u < mine) {
         uint64_t f[P::N];
         P::unpack(w[u], f);
+        if (u == 0) off = norm_off<T, EPV>(f[0]);
 #pragma unroll
-        for (int i = 0; i < P::N; ++i) s = add2(s, f[i]);
+        for (int i = 0; i < P::N; ++i) s = add2(s, sizeof(T) == 2 ? f[i] : add2(f[i], off));
       }
     float sa, sb;
     unpair(s, sa, sb);
     mean = (sa + sb) / n;
+    if (sizeof(T) == 4) mean += norm_first(off);
     const uint64_t minus = pair(-mean, EPV == 1 ? 0.f : -mean);
 #pragma unroll
     for (int u = 0; u < K; ++u)

@@ -255,6 +255,33 @@ def test_no_spread():
     assert torch.equal(msda.pyramid_group_norm(big, [(50,)], 4), torch.zeros_like(x))
 
 
+# one launch; tiles that a CTA joins itself; tiles that the last ones join; each with groups of
+# whole vectors and of none, and wider than a CTA's threads
+PLANS = [(rows, C, G) for rows in (50, 1500, 5000, 30011) for C, G in ((16, 4), (64, 8), (24, 8))]
+PLANS += [(40003, 32, 4), (300, 2048, 1), (70, 4100, 1)]
+
+
+@pytest.mark.parametrize("rows,C,G", PLANS)
+def test_mean_far_from_zero_in_every_plan(rows, C, G):
+    """fp32 holds a mean of 1000 to 2^-25 * 1000.  It is rounded in a chunk of elements, a thread's
+    join of its chunks, the threads' and the tiles': 8 such roundings at most, were they all on
+    one side."""
+    x = torch.randn(2, rows, C, generator=torch.Generator().manual_seed(3)).to(DEV) + 1000.0
+    y = msda.pyramid_group_norm(x, [(rows,)], G)
+    want = norm64([x.double()], G, [1.0], [0.0], 1e-5, "none")
+    assert float((y.double() - want).abs().max()) < 4 * 1000 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("value", [3.25, 0.1, -1000.3, 31000.7])
+@pytest.mark.parametrize("rows,C,G", PLANS)
+def test_no_spread_in_every_plan(rows, C, G, value):
+    """Elements that are all the same have that value as their mean, so h is zero and y the bias,
+    whatever digits the value has."""
+    x = torch.full((2, rows, C), value, device=DEV)
+    b = affine((C,))[1]
+    y = msda.pyramid_group_norm(x, [(rows,)], G, None, b)
+    assert torch.equal(y, b.expand_as(y))
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_not_finite_stays_in_its_group(bad):
     rows = [40, 9]
