@@ -282,6 +282,40 @@ def test_no_spread_in_every_plan(rows, C, G, value):
     y = msda.pyramid_group_norm(x, [(rows,)], G, None, b)
     assert torch.equal(y, b.expand_as(y))
 
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("value", [0.1, -1000.3, 31000.7])
+@pytest.mark.parametrize("rows,C,G", PLANS)
+def test_no_spread_in_16_bits(rows, C, G, value, dt):
+    """As in 32 bits: h is zero and y the bias rounded once."""
+    x = torch.full((2, rows, C), value, device=DEV, dtype=dt)
+    b = affine((C,))[1]
+    y = msda.pyramid_group_norm(x, [(rows,)], G, None, b)
+    assert torch.equal(y, b.to(dt).expand_as(y))
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows,C,G", [(50, 16, 4), (5000, 64, 8), (5000, 24, 8), (30011, 64, 8),
+                                      (300, 2048, 1)])
+def test_gradients_without_spread(rows, C, G, dt):
+    """Where h is zero, gx is r (dz w - mean(dz w)) with r = 1 / sqrt(eps) = 316, the weight's
+    gradient zero and the bias's the sum of dz.  gx is held to the suite's 1e-4 of r times the
+    size of its terms (and a 16-bit rounding), dz = gy act'(bias)."""
+    x = torch.full((2, rows, C), 1000.3, device=DEV, dtype=dt).requires_grad_(True)
+    w, b = (p.requires_grad_(True) for p in affine((C,)))
+    y = msda.pyramid_group_norm(x, [(rows,)], G, w, b, activation="silu")
+    g = torch.randn(y.shape, generator=torch.Generator().manual_seed(1)).to(DEV, dt)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), g)
+    z = b.detach().double().requires_grad_(True)
+    (slope,) = torch.autograd.grad(act64(z, "silu").sum(), z)
+    dz = g.double() * slope
+    t = (dz * w.detach().double()).view(2, rows, G, -1)
+    r = 1e-5 ** -0.5
+    want = r * (t - t.mean((1, 3), keepdim=True)).view(2, rows, C)
+    bound = 1e-4 * r * t.abs().amax() + HALF_RTOL.get(dt, 0.0) * want.abs()
+    assert bool(((gx.double() - want).abs() <= bound).all())
+    assert not bool(gw.any())
+    assert bool(((gb.double() - dz.sum((0, 1))).abs() <= 2e-5 * dz.abs().sum((0, 1))).all())
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_not_finite_stays_in_its_group(bad):
     rows = [40, 9]
