@@ -359,7 +359,8 @@ MSDA_API int msda_group_norm_bwd(int dtype, int64_t batch, int64_t channels, int
  *   x, y               device pointers (host tables) of (batch, num_tokens,
  *                      heads[i], channels) with dense channels; strides of
  *                      batch, token and head in elements, three per tensor.
- *                      y may be x.
+ *                      y may be x itself; else no two elements of y may
+ *                      share memory, nor one of y with x or inputs.
  *   positions          (batch, num_tokens, num_axes) of position_dtype,
  *                      position_batch elements between batch entries (0: one
  *                      set for all); integers are exact up to 2^24

@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/python.h>
 
+#include <algorithm>
 #include <array>
 #include <string>
 #include <vector>
@@ -591,6 +592,89 @@ std::pair<Tensor, Tensor> rotary_qk(const Tensor& q, const Tensor& k, const Tens
   return {out[0], out[1]};
 }
 
+// Whether some n_d, each of its range, give sum n_d stride_d = goal: whether two
+// elements lie at one address, the n_d being what their indexes differ by.
+// Ranges are tried from the widest stride on, and of each only what the others
+// can still make up for: one or two where strides hold each other's rows.  Past
+// `tries` the answer is yes.
+struct Step {
+  int64_t stride, lo, hi;
+};
+
+bool meets(const std::vector<Step>& steps, size_t first, int64_t goal, int& tries) {
+  if (first == steps.size()) return goal == 0;
+  if (--tries < 0) return true;
+  int64_t lo = 0, hi = 0;  // what the steps behind can add
+  for (size_t i = first + 1; i < steps.size(); ++i) {
+    lo += steps[i].lo * steps[i].stride;
+    hi += steps[i].hi * steps[i].stride;
+  }
+  const auto [stride, least, most] = steps[first];
+  auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+  const int64_t from = std::max(least, -floor_div(hi - goal, stride)),
+                to = std::min(most, floor_div(goal - lo, stride));
+  for (int64_t n = from; n <= to; ++n)
+    if (meets(steps, first + 1, goal - n * stride, tries)) return true;
+  return false;
+}
+
+void sort_steps(std::vector<Step>& steps) {
+  std::sort(steps.begin(), steps.end(),
+            [](const Step& x, const Step& y) { return x.stride > y.stride; });
+}
+
+// Whether two elements of (B, Q, H) runs of `run` bytes lie at one address.
+bool overlaps_itself(const Tensor& x, int64_t run) {
+  std::vector<Step> steps{{1, 1 - run, run - 1}};
+  for (int64_t d = 0; d < 3; ++d)
+    if (const int64_t n = x.size(d) - 1; n > 0)
+      steps.push_back({x.stride(d) * x.element_size(), -n, n});
+  sort_steps(steps);
+  int tries = 1 << 12;
+  for (; steps.size() > 1; steps.erase(steps.begin())) {  // the first index that differs
+    std::vector<Step> rest = steps;
+    rest[0].lo = 1;
+    if (meets(rest, 0, 0, tries)) return true;
+  }
+  return false;
+}
+
+// Whether an element of a's runs lies at the address of one of b's.
+bool overlap(const Tensor& a, const Tensor& b, int64_t run) {
+  std::vector<Step> all{{1, 1 - run, run - 1}}, steps;
+  for (int64_t d = 0; d < 3; ++d) {
+    if (a.size(d) > 1) all.push_back({a.stride(d) * a.element_size(), 0, a.size(d) - 1});
+    if (b.size(d) > 1) all.push_back({b.stride(d) * b.element_size(), 1 - b.size(d), 0});
+  }
+  sort_steps(all);
+  for (const Step& s : all) {  // those of one stride are one
+    if (!steps.empty() && steps.back().stride == s.stride) {
+      steps.back().lo += s.lo;
+      steps.back().hi += s.hi;
+    } else {
+      steps.push_back(s);
+    }
+  }
+  int tries = 1 << 12;
+  return meets(steps, 0, static_cast<char*>(b.data_ptr()) - static_cast<char*>(a.data_ptr()),
+               tries);
+}
+
+// Refuses tensors whose heads' first `run` bytes lie twice in memory, within one
+// tensor or in both: several threads of the launch would read and write them.
+void no_overlap(const variable_list& xs, int64_t run) {
+  if (run == 0) return;
+  for (size_t i = 0; i < xs.size(); ++i) {
+    if (xs[i].numel() == 0) continue;
+    TORCH_CHECK_VALUE(!overlaps_itself(xs[i], run),
+                      "rotary_qk_ cannot write to a tensor that overlaps itself, strides ",
+                      xs[i].strides(), " for ", xs[i].sizes());
+    for (size_t j = 0; j < i; ++j)
+      TORCH_CHECK_VALUE(xs[j].numel() == 0 || !overlap(xs[j], xs[i], run),
+                        "rotary_qk_ cannot write to queries and keys that share memory");
+  }
+}
+
 void rotary_in_place(const variable_list& xs, const Tensor& positions, const Tensor& inv_freq,
                      const Tensor& axis_index, bool interleaved) {
   const Tensor p = rotary_check(xs, positions, inv_freq, axis_index);
@@ -602,6 +686,7 @@ void rotary_in_place(const variable_list& xs, const Tensor& positions, const Ten
       TORCH_CHECK_VALUE(x.stride(d) != 0 || x.size(d) <= 1,
                         "rotary_qk_ cannot write to an expanded tensor");
   }
+  no_overlap(xs, 2 * inv_freq.size(0) * xs[0].element_size());
   at::NoGradGuard no_grad;
   turn(xs, xs, kernel_positions(p), inv_freq.contiguous(), axis_index.contiguous(), interleaved,
        false, {}, Tensor());
@@ -775,6 +860,7 @@ PYBIND11_MODULE(_binding, m) {
   m.def("rotary", wrap_pybind_function(rotary_one));
   m.def("rotary_qk", wrap_pybind_function(rotary_qk));
   m.def("rotary_in_place", wrap_pybind_function(rotary_in_place));
+  m.def("no_overlap", wrap_pybind_function(no_overlap));
   m.def("rotary_check", wrap_pybind_function([](const variable_list& xs, const Tensor& p,
                                                 const Tensor& f, const Tensor& a) {
           return rotary_check(xs, p, f, a);

@@ -113,7 +113,10 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
 def rotary_qk_(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                axis_index: torch.Tensor, interleaved: bool = False
                ) -> tuple[torch.Tensor, torch.Tensor]:
-    """rotary_qk in place, for inference: q and k are overwritten and returned."""
+    """rotary_qk in place, for inference: q and k are overwritten and returned.
+
+    They may be slices of one tensor, but no element may lie in both, or twice
+    in one: ValueError."""
     _lib.binding().rotary_in_place([q, k], positions, inv_freq, axis_index, interleaved)
     return q, k
 

@@ -71,6 +71,60 @@ def test_modules_hold_their_parameters():
     assert r.inv_freq.dtype == torch.float32 and not r.state_dict()
 
 
+def _addresses(x, run):
+    """Of the first `run` elements of each head, in elements, with repeats."""
+    index = [torch.arange(n) for n in (*x.shape[:3], run)]
+    at = sum(i.view([-1 if d == e else 1 for e in range(4)]) * s
+             for d, (i, s) in enumerate(zip(index, (*x.stride()[:3], 1))))
+    return (at.reshape(-1) + x.storage_offset()).tolist()
+
+
+def _overlaps(xs, run):
+    try:
+        _lib.binding().no_overlap(xs, run * xs[0].element_size())
+    except ValueError:
+        return True
+    return False
+
+
+def test_overlaps_are_found():
+    """What rotary_qk_ refuses, against a list of all addresses: slices of one projection, one
+    behind or inside the other, windows, and random strides."""
+    buf = torch.zeros(3, 10, 12, 8)
+    q, k = buf[:, :, :4], buf[:, :, 4:8]
+    plain = torch.zeros(3, 10, 4, 8)
+    window = torch.zeros(400).as_strided((1, 20, 3, 8), (400, 8, 8, 1))
+    apart = torch.zeros(600).as_strided((1, 20, 3, 8), (600, 8, 160, 1))
+    for xs, run, want in (
+            ((q, k), 8, False), ((q, buf[:, :, 3:7]), 8, True), ((q, q), 8, True),
+            ((q, buf[:, :, 11:]), 8, False), ((plain, plain.clone()), 8, False),
+            ((plain[:, :5], plain[:, 5:]), 8, False), ((plain[:, ::2], plain[:, 1::2]), 8, False),
+            ((plain[:, :6], plain[:, 5:]), 8, True), ((plain[:2], plain[1:]), 8, True),
+            ((plain.transpose(1, 2), q), 8, False), ((plain, plain.transpose(1, 2)), 8, True),
+            ((window, plain), 8, True), ((apart, plain), 8, False),
+            # only the turned channels are written
+            ((plain, buf.as_strided((3, 10, 4, 4), buf.stride(), 4)), 4, False),
+            ((buf[..., :4], buf[..., 4:]), 4, False), ((buf[..., :4], buf[..., 2:6]), 2, False),
+            ((buf[..., :4], buf[..., 2:6]), 4, True), ((q, k), 0, False), ((q, q), 0, False),
+            ((q[:, :0], q[:, :0]), 8, False)):
+        assert _overlaps(list(xs), run) == want, [(x.shape, x.stride()) for x in xs]
+    rng, found = np.random.default_rng(0), [0, 0]
+    storage = torch.zeros(4000)
+    for _ in range(3000):
+        run, xs = int(rng.integers(1, 9)), []
+        strides = None
+        for _ in range(2):
+            shape = [int(n) for n in rng.integers(1, 5, 3)]
+            if strides is None or rng.random() < 0.5:
+                strides = [int(n) for n in rng.choice([4, 8, 9, 16, 24, 32, 33, 64, 96, 128, 300], 3)]
+            xs.append(storage.as_strided((*shape, 8), (*strides, 1), int(rng.integers(0, 200))))
+        at = [a for x in xs for a in _addresses(x, run)]
+        want = len(set(at)) < len(at)
+        found[want] += 1
+        assert _overlaps(xs, run) == want, [(x.shape, x.stride(), x.storage_offset()) for x in xs]
+    assert min(found) > 300
+
+
 def _rows(*n):
     return np.array(n, dtype=np.int64)
 

@@ -287,6 +287,23 @@ def test_in_place():
         msda.rotary_qk_(torch.stack([q, q], -1)[..., 0], k, pos, freq, axis)
 
 
+def test_in_place_refuses_shared_memory():
+    """Elements that lie in both tensors, or twice in one, are refused before anything is written;
+    slices of one tensor that do not meet are turned."""
+    xs, pos, freq, axis = make(2, 6, (8, 1), 8, torch.float32)
+    buf = xs[0]
+    before = buf.clone()
+    rows = torch.zeros(2 * 6 * 8 * 8, device=DEV).as_strided((2, 6, 3, 8), (384, 8, 8, 1))
+    for q, k in ((buf, buf), (buf[:, :, :5], buf[:, :, 4:]), (rows, buf), (buf, rows),
+                 (buf[..., :8], buf[:, :, 2:3])):
+        with pytest.raises(ValueError, match="share memory|overlaps itself"):
+            msda.rotary_qk_(q, k, pos, freq, axis)
+    assert torch.equal(buf, before)
+    want = msda.rotary(buf, pos, freq, axis)
+    msda.rotary_qk_(buf[:, :, ::2], buf[:, :, 1::2], pos, freq, axis)
+    assert torch.equal(buf, want)
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_gradient_against_differences(interleaved):
     """<gradient, d> and the change of <y, g> along d, by central differences of the kernel's own
