@@ -85,6 +85,12 @@ def _is_dense(p: Tensor) -> bool:
     return True
 
 
+def _order(shape, strides) -> list[int]:
+    """What tells one order of a dense tensor's elements in memory from another: its strides,
+    but those of axes of one element, which are arbitrary."""
+    return [s for s, n in zip(strides, shape) if n > 1]
+
+
 # Elements of a parameter for each element of a state.
 _SIZES = {"exp_avg": 1, "exp_avg_sq": 1, "exp_avg_exponent": BLOCK, "exp_avg_sq_exponent": BLOCK,
           "master": 1}
@@ -151,6 +157,16 @@ class _Part:
         master = master and params[0].dtype != torch.float32
         self.state = adamw_state([p.detach() for p in params], bits, master)
         self.steps = [0] * len(params)
+        # the states' order of elements, of parameters that a change of memory format could move
+        self.laid_out = [(p, p.stride()) for p in params if p.dim() > 2]
+
+    def check(self) -> None:
+        """ValueError where the states lie in another order than their parameter's elements."""
+        for p, strides in self.laid_out:
+            if p.stride() != strides and _order(p.shape, p.stride()) != _order(p.shape, strides):
+                raise ValueError(f"a parameter {tuple(p.shape)} has strides {p.stride()} and had "
+                                 f"{strides} when its states were made: change its memory format "
+                                 "before the first step")
 
     def own(self, i: int, at: int) -> dict[str, Tensor]:
         """Parameter i's part of each state tensor."""
@@ -183,7 +199,8 @@ class AdamW(torch.optim.Optimizer):
 
     Parameters without a gradient are skipped, and count their own steps.  A
     state_dict of torch.optim.AdamW can be loaded where state_bits is 32; an
-    8-bit one holds the codes and exponents themselves.  A group that asks for
+    8-bit one holds the codes and exponents themselves, and loads where the
+    parameters lie in memory in the same order.  A group that asks for
     another update (maximize, amsgrad, a decay that is not decoupled) is a
     ValueError.  `step` cannot be captured in a CUDA graph.
     """
@@ -221,7 +238,10 @@ class AdamW(torch.optim.Optimizer):
             self._parts.append(parts)
             for part in parts:
                 for i, at in enumerate(part.places()):
-                    self.state[part.params[i]] = {"step": 0, **part.own(i, at)}
+                    p = part.params[i]
+                    self.state[p] = {"step": 0, **part.own(i, at)}
+                    if self.state_bits == 8:
+                        self.state[p]["strides"] = p.stride()
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -236,6 +256,7 @@ class AdamW(torch.optim.Optimizer):
                 grads = [p.grad for p in part.params]
                 if all(g is None for g in grads):
                     continue
+                part.check()
                 steps = [s + (g is not None) for s, g in zip(part.steps, grads)]
                 adamw_step(part.params, grads, part.state, step=[max(s, 1) for s in steps],
                            lr=group["lr"], betas=group["betas"], eps=group["eps"],
@@ -275,6 +296,11 @@ class AdamW(torch.optim.Optimizer):
                 part, i, at = place[id(p)]
                 own, got = part.own(i, at), state_dict["state"].get(index)
                 if got is not None:
+                    # codes are in the order of their parameter's elements in memory
+                    if self.state_bits == 8 and _order(p.shape, p.stride()) != _order(
+                            p.shape, got.get("strides", p.stride())):
+                        raise ValueError(f"8-bit states of strides {got['strides']} for a "
+                                         f"parameter {tuple(p.shape)} of strides {p.stride()}")
                     for name, t in own.items():
                         if name not in got and name == "master":
                             got = {**got, "master": p.detach()}

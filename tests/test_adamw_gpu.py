@@ -474,6 +474,61 @@ def test_load_hooks_run():
     assert opt.param_groups[0]["lr"] == 1e-2
 
 
+def conv(last, dt=torch.float32):
+    torch.manual_seed(0)
+    net = torch.nn.Conv2d(5, 6, 3).to(DEV, dt)
+    return net.to(memory_format=torch.channels_last) if last else net
+
+
+def train_conv(net, opt, steps, first=0):
+    for t in range(first, first + steps):
+        x = torch.randn(2, 5, 8, 8, generator=torch.Generator().manual_seed(t)).to(DEV)
+        opt.zero_grad()
+        net(x).square().mean().backward()
+        opt.step()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_states_follow_the_order_of_elements(bits):
+    """States saved of a channels-last weight go on as the run that they were saved from: with
+    another channels-last weight, and in 32 bits with a weight of the usual order. 8-bit codes
+    share exponents along memory and are refused there."""
+    net = conv(True)
+    opt = msda.AdamW(net.parameters(), lr=1e-2, state_bits=bits, seed=1)
+    train_conv(net, opt, 3)
+    saved, weights = copy.deepcopy(opt.state_dict()), copy.deepcopy(net.state_dict())
+    train_conv(net, opt, 2, 3)
+    for last in (True, False):
+        other = conv(last)
+        other.load_state_dict(weights)
+        opt2 = msda.AdamW(other.parameters(), lr=1e-2, state_bits=bits, seed=1)
+        if bits == 8 and not last:
+            with pytest.raises(ValueError, match="strides"):
+                opt2.load_state_dict(saved)
+            continue
+        opt2.load_state_dict(saved)
+        train_conv(other, opt2, 2, 3)
+        for p, q in zip(net.parameters(), other.parameters()):
+            torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-5 if bits == 32 else 1e-3)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_later_change_of_memory_format_is_refused(bits):
+    """The states would be another element's."""
+    net = conv(False)
+    opt = msda.AdamW(net.parameters(), state_bits=bits)
+    train_conv(net, opt, 1)
+    net.to(memory_format=torch.channels_last)
+    before = net.weight.clone()
+    with pytest.raises(ValueError, match="memory format"):
+        train_conv(net, opt, 1, 1)
+    assert torch.equal(net.weight, before)
+    flat = torch.nn.Conv2d(5, 6, 1).to(DEV)  # in one order only, whatever its strides say
+    opt = msda.AdamW(flat.parameters(), state_bits=bits)
+    for t in range(2):
+        train_conv(flat, opt, 1, t)
+        flat.to(memory_format=torch.channels_last)
+
 def test_parameters_without_gradient_count_their_own_steps():
     a, b = model(), model()
     ours, theirs = msda.AdamW(a.parameters(), lr=1e-2), torch.optim.AdamW(b.parameters(), lr=1e-2)
