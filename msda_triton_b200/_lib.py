@@ -11,11 +11,11 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 import os
+import sys
 import threading
 
 LIB_PATH = os.environ.get("MSDA_B200_LIB") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), "_lib", "libmsda_b200.so")
-BINDING_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_binding.so")
 
 # Status codes (msda_status in include/msda_b200.h).
 SUCCESS = 0
@@ -230,6 +230,14 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def binding_path() -> str:
+    """Of the binding for this Python and torch, whose C++ interfaces are their versions' own."""
+    import torch
+
+    name = f"_binding-{sys.implementation.cache_tag}-torch{torch.__version__}.so"
+    return os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", name)
+
+
 def binding():
     """Load (once) and return the torch side of the operators in csrc/binding.cpp, which calls
     the functions of lib()."""
@@ -239,14 +247,13 @@ def binding():
     handle = lib()
     with _lock:
         if _binding is None:
-            if not os.path.exists(BINDING_PATH):
+            path = binding_path()  # imports torch, whose libraries are the binding's
+            if not os.path.exists(path):
                 raise RuntimeError(
-                    f"msda_triton_b200: binding not found at {BINDING_PATH}; build it with "
+                    f"msda_triton_b200: binding not found at {path}; build it with "
                     "`python -m msda_triton_b200.build` (there is no CPU fallback)"
                 )
-            import torch  # noqa: F401  (its libraries are the binding's)
-
-            spec = importlib.util.spec_from_file_location("_binding", BINDING_PATH)
+            spec = importlib.util.spec_from_file_location("_binding", path)
             module = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(module)
             module.bind([ctypes.cast(getattr(handle, name), _vp).value

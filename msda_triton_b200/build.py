@@ -8,7 +8,7 @@ Every .cu file in csrc/ is compiled by nvcc in parallel with
 msda_triton_b200/_lib/libmsda_b200.so (statically linked CUDA runtime, so
 the library depends on nothing but the driver).  csrc/binding.cpp, the torch
 side of some operators, is compiled against the installed torch into
-msda_triton_b200/_lib/_binding.so.
+msda_triton_b200/_lib/_binding-<python>-torch<version>.so.
 
     python -m msda_triton_b200.build --checked
 
@@ -36,7 +36,6 @@ OBJ_DIR = os.path.join(PKG, "_build")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(LIB_DIR, "libmsda_b200.so")
 BINDING_SRC = os.path.join(CSRC, "binding.cpp")
-BINDING = os.path.join(LIB_DIR, "_binding.so")
 CHECKED_OBJ_DIR = os.path.join(PKG, "_build_checked")
 CHECKED_LIB = os.path.join(PKG, "_lib_checked", "libmsda_b200.so")
 
@@ -69,9 +68,12 @@ def _compile(src: str, extra: list[str], obj_dir: str) -> str:
 
 def build_binding(force: bool = False) -> str:
     """Compile csrc/binding.cpp against the installed torch; returns the module's path."""
-    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(
+    from msda_triton_b200 import _lib
+
+    path = _lib.binding_path()
+    if not force and os.path.exists(path) and os.path.getmtime(path) >= max(
             os.path.getmtime(f) for f in [BINDING_SRC, *glob.glob(os.path.join(INCLUDE, "*.h"))]):
-        return BINDING
+        return path
     import torch
 
     root = os.path.dirname(torch.__file__)
@@ -80,7 +82,7 @@ def build_binding(force: bool = False) -> str:
             os.path.join(root, "include", "torch", "csrc", "api", "include"),
             os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     os.makedirs(LIB_DIR, exist_ok=True)
-    tmp = BINDING + ".tmp"
+    tmp = path + ".tmp"
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *[a for d in dirs for a in ("-isystem", d)], BINDING_SRC, "-o", tmp,
@@ -89,8 +91,8 @@ def build_binding(force: bool = False) -> str:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {BINDING_SRC}:\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, BINDING)
-    return BINDING
+    os.replace(tmp, path)
+    return path
 
 
 def build(force: bool = False, verbose_ptxas: bool = False, checked: bool = False) -> str:

@@ -19,6 +19,22 @@ def test_binding_loads_and_names_exported_functions():
     assert set(_lib.BINDING_SYMBOLS) <= set(_lib.EXPORTED_SYMBOLS)
 
 
+def test_binding_of_another_torch_is_not_loaded(monkeypatch):
+    """It is built anew instead (here by a compiler that fails)."""
+    from types import SimpleNamespace
+
+    from msda_triton_b200 import build
+
+    monkeypatch.setattr(torch, "__version__", "0.0.0")
+    monkeypatch.setattr(_lib, "_binding", None)
+    with pytest.raises(RuntimeError, match="binding not found"):
+        _lib.binding()
+    monkeypatch.setattr(build.subprocess, "run", lambda *a, **k: SimpleNamespace(
+        returncode=1, stdout="", stderr=""))
+    with pytest.raises(RuntimeError, match="failed on"):
+        build.build_binding()
+
+
 @pytest.mark.parametrize("call", [
     lambda: msda.pyramid_group_norm(torch.zeros(1, 4, 8), [(2, 2)], 2),
     lambda: msda.PyramidGroupNorm(2, 8)(torch.zeros(1, 4, 8), [(2, 2)]),
