@@ -134,7 +134,8 @@ class AxialRotary(nn.Module):
         rotated = head_dim - head_dim % 2 if rotated is None else rotated
         if rotated > head_dim:
             raise ValueError(f"rotated ({rotated}) exceeds head_dim ({head_dim})")
-        inv_freq, axis_index = axial_frequencies(rotated, num_axes, theta, sections, device)
+        self._table = rotated, num_axes, theta, sections
+        inv_freq, axis_index = axial_frequencies(*self._table, device)
         self.register_buffer("inv_freq", inv_freq, persistent=False)
         self.register_buffer("axis_index", axis_index, persistent=False)
         self.num_axes, self.interleaved = num_axes, interleaved
@@ -147,10 +148,13 @@ class AxialRotary(nn.Module):
         return rotary_qk(q, k, positions, self.inv_freq, self.axis_index, self.interleaved)
 
     def _apply(self, fn, recurse=True):
-        # moving the module to a 16-bit dtype must not round the frequencies
+        # moving the module to a 16-bit dtype must not round the frequencies, and no state_dict
+        # fills them where a module made on the meta device gets its memory
         freq = self.inv_freq
         super()._apply(fn, recurse)
-        if self.inv_freq.dtype != torch.float32:
+        if freq.is_meta and not self.inv_freq.is_meta:
+            self.inv_freq, self.axis_index = axial_frequencies(*self._table, self.inv_freq.device)
+        elif self.inv_freq.dtype != torch.float32:
             self.inv_freq = freq.to(self.inv_freq.device)
         return self
 

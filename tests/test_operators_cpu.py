@@ -87,6 +87,20 @@ def test_modules_hold_their_parameters():
     assert r.inv_freq.dtype == torch.float32 and not r.state_dict()
 
 
+@pytest.mark.parametrize("sections", [None, (8, 5, 3)])
+def test_rotary_tables_outlive_the_meta_device(sections):
+    """Memory for a module made on the meta device holds the tables, not what was there."""
+    want = msda.AxialRotary(32, 3, theta=50.0, sections=sections)
+    r = msda.AxialRotary(32, 3, theta=50.0, sections=sections, device="meta")
+    assert r.half().inv_freq.is_meta
+    torch.full((1 << 16,), float("nan"))  # not zeros, if the allocator gives it back
+    r.to_empty(device="cpu")
+    assert torch.equal(r.inv_freq, want.inv_freq) and torch.equal(r.axis_index, want.axis_index)
+    assert r.inv_freq.dtype == torch.float32 and not r.state_dict()
+    r.bfloat16()
+    assert torch.equal(r.inv_freq, want.inv_freq)
+
+
 def _addresses(x, run):
     """Of the first `run` elements of each head, in elements, with repeats."""
     index = [torch.arange(n) for n in (*x.shape[:3], run)]
