@@ -603,6 +603,23 @@ def test_capture_is_refused():
             msda.adamw_step([p2], [p], state, step=1)
 
 
+def test_step_beside_a_compiled_graph():
+    """adamw_step is no traced op: compiled code calls it between its graphs, and a whole graph
+    cannot hold it."""
+    def step(p, g, state):
+        msda.adamw_step([p], [g * 2], state, step=1)
+        return p * 3
+
+    runs = []
+    for f in (step, torch.compile(step)):
+        p, g = (t[0] for t in (tensors([(200,)], torch.float32), tensors([(200,)], torch.float32, 1)))
+        runs.append((f(p, g, msda.adamw_state([p])), p))
+    torch.testing.assert_close(runs[1], runs[0], rtol=1e-6, atol=1e-6)
+    torch._dynamo.reset()  # or the compiled pieces above would be taken again
+    with pytest.raises(torch._dynamo.exc.Unsupported):
+        torch.compile(step, fullgraph=True)(p, g, msda.adamw_state([p]))
+
+
 def test_refusals():
     p, g = torch.ones(300, device=DEV), torch.ones(300, device=DEV)
     st = msda.adamw_state([p])

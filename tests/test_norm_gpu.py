@@ -409,6 +409,38 @@ def test_module_stream_and_graph():
         assert torch.equal(y, m(x, shapes))
 
 
+@pytest.mark.parametrize("rows", [[5000], [30011, 70]], ids=str)
+def test_graph_of_several_launches(rows):
+    """Forward and backward captured: two launches of which the second starts early, and those with
+    the clearing of counters before them.  Every replay gives what a call by itself does."""
+    x = features(2, rows, 64, torch.bfloat16).requires_grad_(True)
+    w, b = (p.requires_grad_(True) for p in affine((len(rows), 64)))
+    shapes = torch.tensor([[1, n] for n in rows])
+    g = torch.randn(x.shape, generator=torch.Generator().manual_seed(1)).to(DEV, x.dtype)
+
+    def run():
+        y = msda.pyramid_group_norm(x, shapes, 8, w, b, activation="silu")
+        return (y, *torch.autograd.grad(y, (x, w, b), g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for seed in (4, 5):
+        with torch.no_grad():
+            x.copy_(features(2, rows, 64, torch.bfloat16, seed=seed))
+        want = run()
+        for _ in range(2):
+            for t in got:
+                t.detach().zero_()
+            graph.replay()
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_compiles():
     m = msda.PyramidGroupNorm(4, 32, activation="gelu", device=DEV)
     x = features(2, [12, 5], 32, torch.float32).requires_grad_(True)

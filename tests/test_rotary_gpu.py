@@ -363,6 +363,49 @@ def test_module_stream_graph_and_compile():
         torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-4)
 
 
+def test_backward_in_a_graph():
+    xs, pos, freq, axis = make(2, 70, (4, 2), 32, torch.bfloat16)
+    leaves = [t.requires_grad_(True) for t in (*xs, pos)]
+    gs = [torch.randn(x.shape, generator=torch.Generator().manual_seed(1)).to(DEV, x.dtype)
+          for x in xs]
+
+    def run():
+        return torch.autograd.grad(msda.rotary_qk(*leaves, freq, axis), leaves, gs)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    with torch.no_grad():
+        pos.mul_(0.5)
+        xs[0].mul_(2)
+    want = run()
+    graph.replay()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_in_place_beside_a_compiled_graph():
+    """rotary_qk_ is no traced op: compiled code calls it between its graphs, and a whole graph
+    cannot hold it."""
+    xs, pos, freq, axis = make(2, 5, (4, 4), 32, torch.float32)
+
+    def step(q, k):
+        q, k = msda.rotary_qk_(q * 2, k + 1, pos, freq, axis)
+        return q.sin(), k
+
+    want = step(*xs)
+    got = torch.compile(step)(*xs)
+    for a, e in zip(got, want):
+        assert_close(a, e, 1e-6, "around the call")
+    torch._dynamo.reset()  # or the compiled pieces above would be taken again
+    with pytest.raises(torch._dynamo.exc.Unsupported):
+        torch.compile(step, fullgraph=True)(*xs)
+
+
 def test_refusals():
     x = torch.zeros(2, 5, 3, 8, device=DEV)
     pos = torch.zeros(2, 5, 2, device=DEV)
