@@ -26,8 +26,13 @@
 // a change of 0.1 % a step (b2 = 0.999) is far below the spacing of 12.5 %, and
 // rounding to the nearest code would freeze the second moment where it is.
 // The random bits are a mixed counter of the element's index, the seed and the
-// step, so a step can be repeated.  A second moment above zero keeps a code
-// above zero: decoded as zero it would divide by eps alone.
+// step, so a step can be repeated.
+//
+// Below the lowest code, 1.125 x 2^-15 or 2^-31 of the power of two that holds
+// the block's largest, rounding is not random.  A first moment becomes zero: an
+// element whose gradients stay that far below a neighbour's keeps no momentum,
+// and its update is about 1 - b1 of what it would be.  A second moment above
+// zero takes the lowest code: decoded as zero it would divide by eps alone.
 //
 // A warp takes a block, a lane four neighbouring elements: 16-byte (8-byte)
 // accesses of fp32 (16-bit) parameters and whole 128-byte lines of codes, and

@@ -192,7 +192,10 @@ class AdamW(torch.optim.Optimizer):
     Args:
         params, lr, betas, eps, weight_decay: as torch.optim.AdamW; groups may
             differ in them.
-        state_bits: 32, or 8: moments in one byte each, with random rounding.
+        state_bits: 32, or 8: moments in one byte each, with random rounding.  128
+            neighbouring elements share a range, 2^15 for the first moment and 2^31
+            for the second; below it the first is zero (no momentum where a gradient
+            stays that far below a neighbour's) and the second the range's end.
         master_weights: keep fp32 copies of 16-bit parameters, which the step
             updates and rounds into the parameters.
         seed: of the 8-bit states' rounding.

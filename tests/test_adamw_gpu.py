@@ -174,6 +174,28 @@ def test_second_moment_never_falls_to_zero():
     assert bool((v > 0).all()) and float(p.abs().max()) <= 3.1e-3
 
 
+def test_below_the_range_rounding_is_not_random():
+    """Gradients down to 2^-50 of their block's largest, whose moments end below both ranges: the
+    first moment is then zero and the second the lowest code, with any random bits, and elements
+    above are still on one of their value's two codes."""
+    g = torch.exp2(-torch.arange(BLOCK, device=DEV) * (50 / BLOCK)).repeat(2)
+    g[BLOCK:] *= -3e4
+    p = torch.zeros_like(g)
+    m64, v64 = 0.1 * g.double(), 0.001 * g.double().square()
+    for seed in range(16):
+        state = msda.adamw_state([p], bits=8)
+        msda.adamw_step([p.clone()], [g], state, step=1, seed=seed)
+        r = bits_of(g.numel(), (seed + 0x632BE5AB) & 0xFFFFFFFF)
+        for x, got, half, top, below in zip((m64, v64), msda.adamw_state_values(state),
+                                            (r & 0xFFFF, r >> 16), (15, 31), (0.0, 1.0)):
+            low, high, take, least = neighbours(x.abs(), half, top)
+            size = got.double().abs().view(-1, BLOCK)
+            small = take < least
+            assert bool((small.sum(1) > BLOCK // 4).all()) and bool((~small).any(1).all())
+            assert torch.equal(size[small], (below * least).expand_as(size)[small])
+            assert bool(((size == low) | (size == high))[~small].all())
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_zero_gradients_and_states(bits):
     p = torch.ones(300, device=DEV)
