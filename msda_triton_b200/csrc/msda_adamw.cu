@@ -173,6 +173,8 @@ __device__ __forceinline__ uint32_t adam_encode(const float* x, const uint32_t* 
   return __byte_perm(__byte_perm(c[0], c[1], 0x73), __byte_perm(c[2], c[3], 0x73), 0x5410);
 }
 
+// A counter times an odd constant, mixed by shifts and products.  The constants
+// are the first three primes of the published 32-bit hash xxHash (Y. Collet).
 __device__ __forceinline__ uint32_t adam_random(uint32_t index, uint32_t key) {
   uint32_t x = index * 0x9e3779b1u + key;
   x = (x ^ (x >> 16)) * 0x85ebca77u;
