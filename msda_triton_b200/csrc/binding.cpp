@@ -12,6 +12,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/python.h>
@@ -106,10 +107,13 @@ void once_differentiable(const variable_list& grads, variable_list& out) {
 
 // Forward-mode derivatives there are none of either, and a dual tensor may not
 // require a gradient: its tangent would be dropped beside the autograd function.
-void no_tangents(at::TensorList ts, const char* what) {
-  for (const Tensor& t : ts)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what,
-                                " has no forward-mode derivative");
+// Looking for a tangent takes 20 ns a tensor, so callers ask once whether there
+// can be any.
+bool dual_level() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
+
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what,
+                              " has no forward-mode derivative");
 }
 
 // ------------------------------------------------------------------ group norm
@@ -163,8 +167,11 @@ Norm norm_check(const variable_list& xs, bool maps, const py::object& spatial_sh
   TORCH_CHECK_VALUE(first.is_cuda(),
                     "pyramid_group_norm requires CUDA tensors. Got CPU tensors instead.");
   dtype_code(first, "pyramid_group_norm");
-  no_tangents(xs, "pyramid_group_norm");
-  no_tangents({weight.value_or(Tensor()), bias.value_or(Tensor())}, "pyramid_group_norm");
+  if (dual_level()) {
+    for (const Tensor& t : xs) no_tangent(t, "pyramid_group_norm");
+    for (const auto* p : {&weight, &bias})
+      if (*p) no_tangent(**p, "pyramid_group_norm");
+  }
   for (const Tensor& t : xs) {
     TORCH_CHECK_VALUE(maps ? t.dim() >= 3 : t.dim() == 3,
                       "x must be (B, K, C), or levels of (B, *spatial, C); got ", t.sizes());
@@ -316,7 +323,7 @@ std::pair<Tensor, Tensor> norm_forward(const Norm& n, const variable_list& xs,
 variable_list norm_backward(const Norm& n, const variable_list& xs, const optional<Tensor>& weight,
                             const optional<Tensor>& bias, const Tensor& stats,
                             const Tensor& grad_y) {
-  no_tangents(grad_y, "pyramid_group_norm's backward");
+  if (dual_level()) no_tangent(grad_y, "pyramid_group_norm's backward");
   at::NoGradGuard no_grad;
   const Tensor& first = xs[0];
   const c10::cuda::CUDAGuard guard(first.device());
@@ -431,8 +438,11 @@ Tensor rotary_check(at::TensorList xs, const Tensor& positions, const Tensor& in
   const Tensor& first = xs[0];
   TORCH_CHECK_VALUE(first.is_cuda(), "rotary requires CUDA tensors. Got CPU tensors instead.");
   dtype_code(first, "rotary");
-  no_tangents(xs, "rotary");
-  no_tangents({positions, inv_freq}, "rotary");
+  if (dual_level()) {
+    for (const Tensor& x : xs) no_tangent(x, "rotary");
+    no_tangent(positions, "rotary");
+    no_tangent(inv_freq, "rotary");
+  }
   TORCH_CHECK(!at::GradMode::is_enabled() || !inv_freq.requires_grad(),
               "rotary forms no gradient for inv_freq: detach it");
   TORCH_CHECK_VALUE(first.dim() == 4, "expected (B, Q, H, C), got ", first.sizes());
@@ -528,7 +538,8 @@ variable_list rotary_forward(at::TensorList xs, const Tensor& positions, const T
 // Gradients of the tensors and, with their inputs given, of the positions.
 variable_list rotary_backward(at::TensorList grads, at::TensorList inputs, const Tensor& positions,
                               const Tensor& inv_freq, const Tensor& axis_index, bool interleaved) {
-  no_tangents(grads, "rotary's backward");
+  if (dual_level())
+    for (const Tensor& g : grads) no_tangent(g, "rotary's backward");
   at::NoGradGuard no_grad;
   variable_list gys, gxs, ins;
   for (const Tensor& g : grads) {
@@ -783,12 +794,13 @@ void adamw_step(const py::object& params, const py::object& grads, const py::dic
   std::vector<int64_t> counts(n), steps(n);
   std::vector<Tensor> kept, changed;
   changed.reserve(n);
+  const bool dual = dual_level();
   for (int64_t i = 0; i < n; ++i) {
     const Tensor& p = tensor_of(PySequence_Fast_GET_ITEM(ps.ptr(), i), "params");
     PyObject* o = PySequence_Fast_GET_ITEM(gs.ptr(), i);
     TORCH_CHECK_VALUE(p.scalar_type() == dtype && p.device() == device,
                       "the tensors of a step must share their dtype and device");
-    no_tangents(p, "adamw_step");
+    if (dual) no_tangent(p, "adamw_step");
     p_at[i] = p.data_ptr();
     counts[i] = p.numel();
     g_at[i] = nullptr;
@@ -801,7 +813,7 @@ void adamw_step(const py::object& params, const py::object& grads, const py::dic
     TORCH_CHECK_VALUE(g.layout() == at::kStrided, "gradients must be dense, got ", g.layout());
     TORCH_CHECK_VALUE(g.scalar_type() == dtype && g.device() == device, "gradients must be ",
                       dtype, " on ", device, ", as the tensors");
-    no_tangents(g, "adamw_step");
+    if (dual) no_tangent(g, "adamw_step");
     TORCH_CHECK_VALUE(g.sizes() == p.sizes(), "gradient ", g.sizes(), " for a tensor ", p.sizes());
     if (dense && g.is_contiguous()) {
       g_at[i] = g.data_ptr();
