@@ -611,64 +611,65 @@ std::pair<Tensor, Tensor> rotary_qk(const Tensor& q, const Tensor& k, const Tens
 struct Step {
   int64_t stride, lo, hi;
 };
+using Steps = std::array<Step, 7>;  // three of each tensor, and one within a run
 
-bool meets(const std::vector<Step>& steps, size_t first, int64_t goal, int& tries) {
-  if (first == steps.size()) return goal == 0;
+bool meets(const Step* at, const Step* end, int64_t goal, int& tries) {
+  if (at == end) return goal == 0;
   if (--tries < 0) return true;
   int64_t lo = 0, hi = 0;  // what the steps behind can add
-  for (size_t i = first + 1; i < steps.size(); ++i) {
-    lo += steps[i].lo * steps[i].stride;
-    hi += steps[i].hi * steps[i].stride;
+  for (const Step* s = at + 1; s != end; ++s) {
+    lo += s->lo * s->stride;
+    hi += s->hi * s->stride;
   }
-  const auto [stride, least, most] = steps[first];
   auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
-  const int64_t from = std::max(least, -floor_div(hi - goal, stride)),
-                to = std::min(most, floor_div(goal - lo, stride));
+  const int64_t from = std::max(at->lo, -floor_div(hi - goal, at->stride)),
+                to = std::min(at->hi, floor_div(goal - lo, at->stride));
   for (int64_t n = from; n <= to; ++n)
-    if (meets(steps, first + 1, goal - n * stride, tries)) return true;
+    if (meets(at + 1, end, goal - n * at->stride, tries)) return true;
   return false;
 }
 
-void sort_steps(std::vector<Step>& steps) {
-  std::sort(steps.begin(), steps.end(),
+void sort_steps(Steps& steps, size_t count) {
+  std::sort(steps.begin(), steps.begin() + count,
             [](const Step& x, const Step& y) { return x.stride > y.stride; });
 }
 
 // Whether two elements of (B, Q, H) runs of `run` bytes lie at one address.
 bool overlaps_itself(const Tensor& x, int64_t run) {
-  std::vector<Step> steps{{1, 1 - run, run - 1}};
+  Steps steps{{{1, 1 - run, run - 1}}};
+  size_t count = 1;
   for (int64_t d = 0; d < 3; ++d)
     if (const int64_t n = x.size(d) - 1; n > 0)
-      steps.push_back({x.stride(d) * x.element_size(), -n, n});
-  sort_steps(steps);
+      steps[count++] = {x.stride(d) * x.element_size(), -n, n};
+  sort_steps(steps, count);
   int tries = 1 << 12;
-  for (; steps.size() > 1; steps.erase(steps.begin())) {  // the first index that differs
-    std::vector<Step> rest = steps;
-    rest[0].lo = 1;
-    if (meets(rest, 0, 0, tries)) return true;
+  for (size_t i = 0; i + 1 < count; ++i) {  // the first index that differs
+    steps[i].lo = 1;
+    if (meets(&steps[i], &steps[0] + count, 0, tries)) return true;
   }
   return false;
 }
 
 // Whether an element of a's runs lies at the address of one of b's.
 bool overlap(const Tensor& a, const Tensor& b, int64_t run) {
-  std::vector<Step> all{{1, 1 - run, run - 1}}, steps;
+  Steps steps{{{1, 1 - run, run - 1}}};
+  size_t all = 1, count = 1;
   for (int64_t d = 0; d < 3; ++d) {
-    if (a.size(d) > 1) all.push_back({a.stride(d) * a.element_size(), 0, a.size(d) - 1});
-    if (b.size(d) > 1) all.push_back({b.stride(d) * b.element_size(), 1 - b.size(d), 0});
+    if (a.size(d) > 1) steps[all++] = {a.stride(d) * a.element_size(), 0, a.size(d) - 1};
+    if (b.size(d) > 1) steps[all++] = {b.stride(d) * b.element_size(), 1 - b.size(d), 0};
   }
-  sort_steps(all);
-  for (const Step& s : all) {  // those of one stride are one
-    if (!steps.empty() && steps.back().stride == s.stride) {
-      steps.back().lo += s.lo;
-      steps.back().hi += s.hi;
+  sort_steps(steps, all);
+  for (size_t i = 1; i < all; ++i) {  // those of one stride are one
+    if (steps[count - 1].stride == steps[i].stride) {
+      steps[count - 1].lo += steps[i].lo;
+      steps[count - 1].hi += steps[i].hi;
     } else {
-      steps.push_back(s);
+      steps[count++] = steps[i];
     }
   }
   int tries = 1 << 12;
-  return meets(steps, 0, static_cast<char*>(b.data_ptr()) - static_cast<char*>(a.data_ptr()),
-               tries);
+  return meets(&steps[0], &steps[0] + count,
+               static_cast<char*>(b.data_ptr()) - static_cast<char*>(a.data_ptr()), tries);
 }
 
 // Refuses tensors whose heads' first `run` bytes lie twice in memory, within one
@@ -765,9 +766,21 @@ Tensor laid_out(const Tensor& p, const Tensor& g) {
   return g;
 }
 
+// Refuses a parameter whose elements lie in another order than when its states
+// were made; the stride of an axis of one element says nothing.
+void same_order(const Tensor& p, const Tensor& then) {
+  if (p.strides() == then.strides()) return;
+  for (int64_t d = 0; d < p.dim(); ++d)
+    TORCH_CHECK_VALUE(p.size(d) <= 1 || p.stride(d) == then.stride(d), "a parameter ", p.sizes(),
+                      " has strides ", p.strides(), " and had ", then.strides(),
+                      " when its states were made: change its memory format before the first step");
+}
+
+// layouts: None, or for each parameter a tensor of the strides that its states were made for.
 void adamw_step(const py::object& params, const py::object& grads, const py::dict& state,
                 const py::object& step, double lr, double beta1, double beta2, double eps,
-                double weight_decay, int64_t seed, const optional<Tensor>& grad_scale) {
+                double weight_decay, int64_t seed, const optional<Tensor>& grad_scale,
+                const py::object& layouts) {
   at::NoGradGuard no_grad;
   const py::object ps = py::reinterpret_steal<py::object>(
       PySequence_Fast(params.ptr(), "params must be a sequence of tensors"));
@@ -795,12 +808,17 @@ void adamw_step(const py::object& params, const py::object& grads, const py::dic
   std::vector<Tensor> kept, changed;
   changed.reserve(n);
   const bool dual = dual_level();
+  TORCH_CHECK(layouts.is_none() ||
+                  (PyList_Check(layouts.ptr()) && PyList_GET_SIZE(layouts.ptr()) == n),
+              "layouts must be a list of ", n, " tensors");
   for (int64_t i = 0; i < n; ++i) {
     const Tensor& p = tensor_of(PySequence_Fast_GET_ITEM(ps.ptr(), i), "params");
     PyObject* o = PySequence_Fast_GET_ITEM(gs.ptr(), i);
     TORCH_CHECK_VALUE(p.scalar_type() == dtype && p.device() == device,
                       "the tensors of a step must share their dtype and device");
     if (dual) no_tangent(p, "adamw_step");
+    if (!layouts.is_none())
+      same_order(p, tensor_of(PyList_GET_ITEM(layouts.ptr(), i), "layouts"));
     p_at[i] = p.data_ptr();
     counts[i] = p.numel();
     g_at[i] = nullptr;

@@ -122,7 +122,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor | None],
         RuntimeError: under CUDA graph capture, where `step` would be frozen.
     """
     _lib.binding().adamw_step(params, grads, state, step, lr, betas[0], betas[1], eps,
-                              weight_decay, seed & 0xFFFFFFFF, grad_scale)
+                              weight_decay, seed & 0xFFFFFFFF, grad_scale, None)
 
 
 def adamw_state_values(state: dict[str, Tensor]) -> tuple[Tensor, Tensor]:
@@ -157,16 +157,8 @@ class _Part:
         master = master and params[0].dtype != torch.float32
         self.state = adamw_state([p.detach() for p in params], bits, master)
         self.steps = [0] * len(params)
-        # the states' order of elements, of parameters that a change of memory format could move
-        self.laid_out = [(p, p.stride()) for p in params if p.dim() > 2]
-
-    def check(self) -> None:
-        """ValueError where the states lie in another order than their parameter's elements."""
-        for p, strides in self.laid_out:
-            if p.stride() != strides and _order(p.shape, p.stride()) != _order(p.shape, strides):
-                raise ValueError(f"a parameter {tuple(p.shape)} has strides {p.stride()} and had "
-                                 f"{strides} when its states were made: change its memory format "
-                                 "before the first step")
+        # the order of the states' elements, which a step holds its parameters to
+        self.layouts = [torch.empty_strided(p.shape, p.stride(), device="meta") for p in params]
 
     def own(self, i: int, at: int) -> dict[str, Tensor]:
         """Parameter i's part of each state tensor."""
@@ -259,11 +251,11 @@ class AdamW(torch.optim.Optimizer):
                 grads = [p.grad for p in part.params]
                 if all(g is None for g in grads):
                     continue
-                part.check()
                 steps = [s + (g is not None) for s, g in zip(part.steps, grads)]
-                adamw_step(part.params, grads, part.state, step=[max(s, 1) for s in steps],
-                           lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                           weight_decay=group["weight_decay"], seed=self.seed)
+                _lib.binding().adamw_step(part.params, grads, part.state,
+                                          [max(s, 1) for s in steps], group["lr"],
+                                          *group["betas"], group["eps"], group["weight_decay"],
+                                          self.seed & 0xFFFFFFFF, None, part.layouts)
                 part.steps = steps
         return loss
 
