@@ -14,9 +14,10 @@ constexpr int64_t kSMs = 148;
 // 128: 336 MB a pass where 200 were wanted).
 constexpr int64_t kDirectPiece = 128, kPiece = 256;
 // Bytes of x in a tile.  Direct: as many tiles as CTAs run at once, nearly (of
-// the 2D encoder's 41 MB, 632 tiles where 592 run took 32 us forward, 556 take
+// the 2D encoder's 41 MB, 632 tiles where 592 run took 32 us forward, 576 take
 // 27), but no fewer bytes than the first.  Else the third, or the second where
-// there would be few tiles.
+// there would be few tiles.  At once: four CTAs an SM forward and, as its
+// application has, three backward.
 constexpr int64_t kSmallTile = 16 << 10, kMediumTile = 64 << 10, kTile = 128 << 10;
 // The one launch: the narrowest piece of a row, and from where on whole lines.
 constexpr int64_t kOncePiece = 32, kOnceMuch = 32 << 20;

@@ -266,7 +266,7 @@ __device__ __forceinline__ void norm_wait_previous() {
 // MIXED, here and below: a vector holds channels of several groups (groups of
 // no whole vectors: 320 channels in 32).  Sums are then carried per channel.
 // Read in pieces of 4 or 2 bytes, 168 MB of bf16 with 10 channels a group take
-// 169 us forward and 392 backward; in such vectors 129 and 232.
+// 169 us forward and 392 backward; in such vectors 143 and 219.
 template <typename T, int VB, bool DIRECT, bool MIXED, int U>
 __device__ void norm_stats(const NormArgs& a, const NormTile& t) {
   using P = Pairs<T, VB>;
@@ -568,7 +568,7 @@ __device__ void norm_apply(const NormArgs& a, const NormTile& t) {
 }
 
 // A unit that is one tile, and no more than kNormOnceVectors vectors a thread.
-// Of a pyramid of 1 360 x 256 in fp32, 6.8 us where two launches end after 10.5;
+// Of a pyramid of 1 360 x 256 in fp32, 7.0 us where two launches end after 10.5;
 // a call takes 7.7 us of the host instead of 10.3.
 template <typename T, int VB, int ACT>
 __global__ void __launch_bounds__(kNormOnceThreads, 2)
