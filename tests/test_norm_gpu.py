@@ -329,6 +329,23 @@ def test_not_finite_stays_in_its_group(bad):
     assert torch.equal(y[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16], ids=ids)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("rows,C,G", PLANS)
+def test_not_finite_stays_in_its_group_in_every_plan(rows, C, G, bad, dt):
+    """In the first tile, whose mean the others are joined from, and in the last."""
+    for at in (0, rows - 1):
+        x = features(2, [rows], C, dt)
+        clean = msda.pyramid_group_norm(x, [(rows,)], G)
+        c = min(C - 1, 10)
+        x[1, at, c] = bad
+        y = msda.pyramid_group_norm(x, [(rows,)], G)
+        hit = torch.zeros_like(y, dtype=torch.bool)
+        group = c // (C // G) * (C // G)
+        hit[1, :, group:group + C // G] = True
+        assert bool(y[hit].isnan().all()) and torch.equal(y[~hit], clean[~hit])
+
+
 @pytest.mark.parametrize("activation", ["none", "silu", "gelu"])
 def test_gradient_against_differences(activation):
     """<gradient, d> and the change of <y, g> along d, by central differences of the kernel's own
